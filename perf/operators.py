@@ -19,39 +19,39 @@ DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 def listed():
     return [
         # one decoded token of one request at a benchmark width: launch latency
-        dict(name="norm fwd, 1 row", op="fwd", rows=1, h=4096, dtype="bf16", post=True, pre=True, gates=0, res_scale="none"),
+        dict(name="norm_fwd_1", op="fwd", rows=1, h=4096, dtype="bf16", post=True, pre=True, gates=0, res_scale="none"),
         # a decode batch, every token with its own gate
-        dict(name="norm fwd, 64 gated rows", op="fwd", rows=64, h=8192, dtype="fp16", post=True, pre=True, gates=64,
+        dict(name="norm_fwd_64", op="fwd", rows=64, h=8192, dtype="fp16", post=True, pre=True, gates=64,
              res_scale="one"),
         # prompts: 17 sequences of 59 tokens, one gate per sequence, learned residual scale per channel
-        dict(name="norm fwd, 1003 rows", op="fwd", rows=1003, h=5120, dtype="fp16", post=True, pre=True, gates=17,
+        dict(name="norm_fwd_1003", op="fwd", rows=1003, h=5120, dtype="fp16", post=True, pre=True, gates=17,
              res_scale="column"),
         # a training step: the row count and width of the RMSNorm benchmark, 8 sequences
-        dict(name="norm fwd, 32768 rows", op="fwd", rows=32768, h=4096, dtype="bf16", post=True, pre=True, gates=8,
+        dict(name="norm_fwd_32768", op="fwd", rows=32768, h=4096, dtype="bf16", post=True, pre=True, gates=8,
              res_scale="one"),
         # gradients of a short batch: 4 sequences of 59 tokens
-        dict(name="norm bwd, 236 rows", op="bwd", rows=236, h=2048, dtype="bf16", post=True, pre=True, gates=4,
+        dict(name="norm_bwd_236", op="bwd", rows=236, h=2048, dtype="bf16", post=True, pre=True, gates=4,
              res_scale="one"),
         # gradients with one gate per token, an odd number of tokens
-        dict(name="norm bwd, 4099 rows", op="bwd", rows=4099, h=5120, dtype="fp16", post=True, pre=True, gates=4099,
+        dict(name="norm_bwd_4099", op="bwd", rows=4099, h=5120, dtype="fp16", post=True, pre=True, gates=4099,
              res_scale="none"),
         # gradients of a training step at the wide benchmark width, everything learned
-        dict(name="norm bwd, 16384 rows", op="bwd", rows=16384, h=8192, dtype="bf16", post=True, pre=True, gates=8,
+        dict(name="norm_bwd_16384", op="bwd", rows=16384, h=8192, dtype="bf16", post=True, pre=True, gates=8,
              res_scale="column"),
         # one decoded token, one adapter
-        dict(name="lora, 1 token", op="lora", m=1, n=4096, k=4096, rank=16, pool=8, active=1, order="mixed", dtype="bf16",
+        dict(name="lora_1", op="lora", m=1, n=4096, k=4096, rank=16, pool=8, active=1, order="mixed", dtype="bf16",
              terms=False),
         # a decode batch of many requests: 32 adapters in use among 64 tokens, some tokens without one
-        dict(name="lora, 64 tokens", op="lora", m=64, n=14336, k=4096, rank=16, pool=64, active=32, order="mixed",
+        dict(name="lora_64", op="lora", m=64, n=14336, k=4096, rank=16, pool=64, active=32, order="mixed",
              dtype="bf16", terms=False),
         # a wider decode batch on the down projection, larger rank, with the norm's row scale, bias and residual
-        dict(name="lora, 128 tokens", op="lora", m=128, n=4096, k=14336, rank=64, pool=32, active=20, order="mixed",
+        dict(name="lora_128", op="lora", m=128, n=4096, k=14336, rank=64, pool=32, active=20, order="mixed",
              dtype="fp16", terms=True),
         # a few prompts of uneven length, sizes that are no multiple of any tile
-        dict(name="lora, 1003 tokens", op="lora", m=1003, n=4104, k=5128, rank=24, pool=16, active=5, order="runs",
+        dict(name="lora_1003", op="lora", m=1003, n=4104, k=5128, rank=24, pool=16, active=5, order="runs",
              dtype="fp16", terms=False),
         # prompts of 8 requests at once at the largest benchmark projection of this kind
-        dict(name="lora, 4096 tokens", op="lora", m=4096, n=14336, k=4096, rank=16, pool=16, active=8, order="runs",
+        dict(name="lora_4096", op="lora", m=4096, n=14336, k=4096, rank=16, pool=16, active=8, order="runs",
              dtype="bf16", terms=True),
     ]
 
