@@ -336,6 +336,52 @@ int pg_rmsnorm_bwd_static(void *dx, float *dgamma, const void *dy, const void *x
                           int dtype, void *stream);
 
 /*
+ * The boundary between two blocks of a network in one pass over `rows` rows of length h: norm of a block's output u,
+ * its gate, the scaled residual, and the norm in front of the next block.  With rstd(v) = rsqrt(mean(v^2) + eps),
+ *     p = (u * rstd(u)) * gamma_post                    (gamma_post null: p = u)
+ *     s = round_to_dtype(res_scale * residual + gate * p)       the new residual stream
+ *     y = round_to_dtype((s * rstd(s)) * gamma_pre)             from s before its rounding
+ * u, residual, s, y: [rows, h] of `dtype`, dense; all arithmetic in fp32.  h % 8 == 0, rows < 2^31.
+ *   gamma_post  [h] fp32 or null
+ *   gate        [gate_rows, h] of `dtype`, or null with gate_rows 0.  gate_rows divides rows; consecutive
+ *               rows / gate_rows rows share a gate: 1 = one for all, the number of sequences = one for each
+ *               (sequences of one length), rows = one for each token
+ *   res_scale   fp32, res_scale_len elements: h (one per column) or 1; or null with res_scale_len 0
+ *   gamma_pre   [h] fp32, and y; or both null
+ * s may be residual itself and y may be u itself; no other overlap of outputs and inputs.  No scratch memory.
+ * The reference project has neither this operator nor its parts.
+ */
+int pg_rmsnorm_residual_fwd(void *s, void *y, const void *u, const void *residual, const float *gamma_post,
+                            const void *gate, int64_t gate_rows, const float *res_scale, int64_t res_scale_len,
+                            const float *gamma_pre, int64_t rows, int64_t h, float eps, int dtype, void *stream);
+
+/* Bytes of scratch pg_rmsnorm_residual_bwd needs for this shape on the current device. */
+size_t pg_rmsnorm_residual_bwd_workspace_bytes(int64_t rows, int64_t h, int64_t gate_rows);
+
+/*
+ * Gradients of pg_rmsnorm_residual_fwd, from dy (gradient of y; null together with gamma_pre) and ds (gradient that
+ * reaches s past y, along the residual stream; null: none, then dy is needed).  With shat = s * rstd(s),
+ * uhat = u * rstd(u), w = dy * gamma_pre, D the whole gradient of s and e = gate * D:
+ *     D          = ds + rstd(s) * (w - shat * mean(w * shat))
+ *     dresidual  = round_to_dtype(res_scale * D)
+ *     du         = round_to_dtype(rstd(u) * (e * gamma_post - uhat * mean(e * gamma_post * uhat)));  without gamma_post e
+ *     dgamma_pre = sum_r dy * shat      dgamma_post = sum_r e * uhat      dres_scale = sum_r D * residual    (fp32)
+ *     dgate      = round_to_dtype(sum over the gate's rows of D * p)
+ * rstd is computed again from s (as the forward pass stored it) and u.  s is needed with gamma_pre only, u with
+ * gamma_post or dgate, residual with dres_scale.  dgamma_post, dgate, dres_scale and dgamma_pre may be null (not
+ * wanted); they need the tensor they are the gradient of.  dres_scale has res_scale_len elements: with 1 the sum runs
+ * over the columns too.  The sums over rows are deterministic: parts in `workspace` (at least
+ * pg_rmsnorm_residual_bwd_workspace_bytes bytes, 256-byte aligned, no initialisation, private to the call until its
+ * kernels have finished) are added in a fixed order.  dresidual may be ds itself, du may be u or dy itself; no other overlap.
+ * rows == 0 zero-fills the sums.
+ */
+int pg_rmsnorm_residual_bwd(void *du, void *dresidual, float *dgamma_post, void *dgate, float *dres_scale,
+                            float *dgamma_pre, const void *dy, const void *ds, const void *s, const void *u,
+                            const void *residual, const float *gamma_post, const void *gate, int64_t gate_rows,
+                            const float *res_scale, int64_t res_scale_len, const float *gamma_pre, int64_t rows,
+                            int64_t h, float eps, int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * Roofline probes, the sm_100a counterparts of the reference's stand-alone probes
  * (test/cpp/test_wmma_compute.cpp:142-173, the README's "PEAK" column; and
  * test/cpp/test_memory_bandwidth.cpp:95-114).

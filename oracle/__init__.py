@@ -239,3 +239,100 @@ def rmsnorm_inputs(rows: int, h: int, dtype: torch.dtype, seed: int):
     dy = torch.randn(rows, h, generator=g).to(dtype)
     gamma = 1 + 0.1 * torch.randn(h, generator=g)
     return x, dy, gamma
+
+
+# ------------------------------------------------ norms around a gated residual ----
+# PARITY UNPINNED: the reference has neither operator; these restate the definitions in float64, on the inputs' device,
+# together with per-element bounds on what an fp32 evaluation may be off by.
+#
+# Bounds.  The sums over a row are sums of h products in some tree order: each of a row's at most 64 serial additions,
+# 5 shuffle levels and 32 warp sums rounds by 2^-24, so a sum of positive terms is within 2^-17 of itself, rstd (its
+# inverse square root) within 2^-18 + 2^-22, and a sum of mixed terms within 2^-17 of the sum of their absolute values.
+# REL = 2^-17 covers a product of such a factor with the few roundings of the elementwise arithmetic.
+
+REL = 2.0 ** -17
+
+
+def _residual_terms(u, residual, gamma_post, gate, res_scale, eps):
+    u = u.double()
+    rows, h = u.shape
+    one = torch.ones(1, 1, dtype=torch.float64, device=u.device)
+    rstd = torch.rsqrt(u.pow(2).mean(-1, keepdim=True) + eps) if gamma_post is not None else one
+    gp = gamma_post.double()[None, :] if gamma_post is not None else one
+    g = one if gate is None else gate.double().repeat_interleave(rows // gate.shape[0], dim=0)
+    al = one if res_scale is None else res_scale.double()[None, :]
+    return u, rstd, gp, g, al
+
+
+def rmsnorm_residual_fwd(u, residual, gamma_post=None, gate=None, res_scale=None, gamma_pre=None, eps: float = 1e-6):
+    """(s, y, bound of s, bound of y) unrounded, float64; y and its bound None without gamma_pre."""
+    u, rstd, gp, g, al = _residual_terms(u, residual, gamma_post, gate, res_scale, eps)
+    a, b = al * residual.double(), g * (u * rstd * gp)
+    s = a + b
+    es = REL * (a.abs() + b.abs())
+    if gamma_pre is None:
+        return s, None, es, None
+    rs = torch.rsqrt(s.pow(2).mean(-1, keepdim=True) + eps)
+    y = s * rs * gamma_pre.double()
+    # rstd(s) moves by rstd^2 * mean(|s| * error of s) relatively
+    ey = es * rs * gamma_pre.double().abs() + y.abs() * (REL + rs * rs * (s.abs() * es).mean(-1, keepdim=True))
+    return s, y, es, ey
+
+
+def rmsnorm_residual_bwd(dy, ds, s, u, residual=None, gamma_post=None, gate=None, res_scale=None, gamma_pre=None,
+                         eps: float = 1e-6, serial_rows: int = 512):
+    """{name: (gradient, bound)} unrounded, float64.  serial_rows: rows that are added one after the other at most."""
+    shape = (s if s is not None else u if u is not None else ds).shape
+    dev = (ds if ds is not None else dy).device
+    rows, h = shape
+    ref = u if u is not None else torch.zeros(shape, device=dev)
+    ud, rstd, gp, g, al = _residual_terms(ref, residual, gamma_post, gate, res_scale, eps)
+    D = ds.double() if ds is not None else torch.zeros(shape, dtype=torch.float64, device=dev)
+    eD = torch.zeros_like(D)
+    out = {}
+    step = (min(rows, serial_rows) + 64) * 2.0 ** -24
+    if gamma_pre is not None:
+        sd = s.double()
+        rs = torch.rsqrt(sd.pow(2).mean(-1, keepdim=True) + eps)
+        sh, w = sd * rs, dy.double() * gamma_pre.double()
+        c = (w * sh).mean(-1, keepdim=True)
+        D = D + rs * (w - sh * c)
+        eD = REL * ((ds.double().abs() if ds is not None else 0) + rs * (w.abs() + sh.abs() * (c.abs() + (w * sh).abs().mean(-1, keepdim=True))))
+        t = dy.double() * sh
+        out["dgamma_pre"] = (t.sum(0), ((REL + step) * t.abs()).sum(0))
+    out["dresidual"] = (al * D, al.abs() * (eD + REL * D.abs()))
+    if res_scale is not None and residual is not None:
+        t, e = D * residual.double(), (eD + (REL + step) * D.abs()) * residual.double().abs()
+        one = res_scale.numel() == 1
+        out["dres_scale"] = (t.sum().view(1), e.sum().view(1)) if one else (t.sum(0), e.sum(0))
+    uh = ud * rstd
+    if gate is not None and u is not None:
+        p = uh * gp
+        G = gate.shape[0]
+        out["dgate"] = ((D * p).view(G, -1, h).sum(1), ((eD + (REL + step) * D.abs()) * p.abs()).view(G, -1, h).sum(1))
+    e = g * D
+    ee = g.abs() * (eD + REL * D.abs())
+    if gamma_post is None:
+        out["du"] = (e.expand(shape), ee.expand(shape))
+    else:
+        t = e * uh
+        out["dgamma_post"] = (t.sum(0), ((ee + (REL + step) * e.abs()) * uh.abs()).sum(0))
+        v = e * gp
+        ev = ee * gp.abs() + REL * v.abs()
+        c = (v * uh).mean(-1, keepdim=True)
+        ec = ((ev + REL * v.abs()) * uh.abs()).mean(-1, keepdim=True)
+        out["du"] = (rstd * (v - uh * c), rstd * (ev + uh.abs() * (ec + REL * c.abs())) + REL * (rstd * (v - uh * c)).abs())
+    return out
+
+
+def rmsnorm_residual_inputs(rows: int, h: int, dtype: torch.dtype, seed: int, *, post=True, gates=0, res_scale=0, pre=True):
+    """Seeded inputs of the operator: u, residual, ds, dy ~ N(0,1), gains ~ N(1, 0.1), gate ~ N(0, 0.5)."""
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g)    # noqa: E731
+    x = {"u": n(rows, h).to(dtype), "residual": n(rows, h).to(dtype), "ds": n(rows, h).to(dtype),
+         "dy": n(rows, h).to(dtype) if pre else None}
+    x["gamma_post"] = 1 + 0.1 * n(h) if post else None
+    x["gamma_pre"] = 1 + 0.1 * n(h) if pre else None
+    x["gate"] = (0.5 * n(gates, h)).to(dtype) if gates else None
+    x["res_scale"] = 1 + 0.1 * n(res_scale) if res_scale else None
+    return x

@@ -13,6 +13,8 @@ epilogue is a plain cast and whose schema is not annotated):
 * ``gemm_peak_fused``: row scale, bias and residual folded into the GEMM epilogue;
 * ``fold_gamma`` + ``rms_norm_linear``: RMSNorm followed by a projection as ONE
   GEMM over the raw activations (rstd applied per row in the epilogue);
+* ``rms_norm_residual_fwd`` / ``rms_norm_residual_bwd``: the norm after a block, its gate,
+  the scaled residual and the norm before the next block in one pass, and the gradients;
 * ``torch.ops.PeakGemm.*_out`` / ``gemm_peak_fused`` / ``rms_norm_rstd``: schemas
   that mark the written tensors, with fake implementations registered here, so
   the operators survive ``torch.compile`` tracing and functionalisation.
@@ -134,16 +136,71 @@ def rms_norm_linear(out: torch.Tensor, x: torch.Tensor, w_folded: torch.Tensor, 
     return rstd
 
 
+def _flat(t: torch.Tensor | None, h: int) -> torch.Tensor | None:
+    return t.view(-1, h) if t is not None else None
+
+
+def rms_norm_residual_fwd(s: torch.Tensor, y: torch.Tensor | None, u: torch.Tensor, residual: torch.Tensor, *,
+                          gamma_post: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                          res_scale: torch.Tensor | None = None, gamma_pre: torch.Tensor | None = None,
+                          eps: float = 1e-6) -> None:
+    """From one block to the next: the new residual stream ``s`` and its norm ``y``, written in place.
+
+        p = rms_norm(u, gamma_post)                      (``gamma_post`` None: p = u)
+        s = res_scale * residual + gate * p
+        y = rms_norm(s, gamma_pre)                       (``y`` and ``gamma_pre`` both None: not computed)
+
+    ``u``: a block's output; s, y, u, residual: [..., h] float16/bfloat16; gamma_post, gamma_pre: [h] float32.
+    ``gate``: [..., h] of u's dtype, its rows dividing u's rows: with g rows, consecutive rows / g rows share one (one
+    row: for all; one per sequence of a padded batch; one per token).  ``res_scale``: float32, [h] or [1].  fp32
+    arithmetic; y comes from s before its rounding.  ``s`` may be ``residual`` itself and ``y`` may be ``u`` itself.
+    """
+    assert u.dtype in [torch.half, torch.bfloat16]
+    h = u.shape[-1]
+    assert s.shape == u.shape and residual.shape == u.shape and (y is None or y.shape == u.shape)
+    assert (y is None) == (gamma_pre is None)
+    torch.ops.PeakGemm.rms_norm_residual_fwd(s.view(-1, h), _flat(y, h), u.view(-1, h), residual.view(-1, h), gamma_post,
+                                             _flat(gate, h), res_scale, gamma_pre, eps)
+
+
+def rms_norm_residual_bwd(du: torch.Tensor, dresidual: torch.Tensor, dy: torch.Tensor | None, ds: torch.Tensor | None,
+                          s: torch.Tensor | None, u: torch.Tensor | None, *, residual: torch.Tensor | None = None,
+                          gamma_post: torch.Tensor | None = None, gate: torch.Tensor | None = None,
+                          res_scale: torch.Tensor | None = None, gamma_pre: torch.Tensor | None = None,
+                          dgamma_post: torch.Tensor | None = None, dgate: torch.Tensor | None = None,
+                          dres_scale: torch.Tensor | None = None, dgamma_pre: torch.Tensor | None = None,
+                          eps: float = 1e-6) -> None:
+    """Gradients of rms_norm_residual_fwd, written in place; pass None for a gradient that is not wanted.
+
+    ``dy``: gradient of y (None without ``gamma_pre``); ``ds``: gradient that reaches s past y, along the residual
+    stream (None: there is none).  ``s`` as the forward pass stored it (needed with ``gamma_pre``), ``u`` (needed with
+    ``gamma_post`` or ``dgate``), ``residual`` (needed with ``dres_scale``).  ``du``, ``dresidual``: [..., h];
+    ``dgate`` has gate's shape and dtype; ``dgamma_post``, ``dgamma_pre``, ``dres_scale``: float32, the shapes of what
+    they are gradients of.  Sums over rows are formed in fp32 in a fixed order.  ``dresidual`` may be ``ds`` itself,
+    ``du`` may be ``u`` or ``dy`` itself.
+    """
+    assert du.dtype in [torch.half, torch.bfloat16]
+    h = du.shape[-1]
+    for t in (dresidual, dy, ds, s, u, residual):
+        assert t is None or t.shape == du.shape
+    for d, t in ((dgamma_post, gamma_post), (dgate, gate), (dres_scale, res_scale), (dgamma_pre, gamma_pre)):
+        assert d is None or (t is not None and d.shape == t.shape)
+    torch.ops.PeakGemm.rms_norm_residual_bwd(du.view(-1, h), dresidual.view(-1, h), dgamma_post, _flat(dgate, h),
+                                             dres_scale, dgamma_pre, _flat(dy, h), _flat(ds, h), _flat(s, h), _flat(u, h),
+                                             _flat(residual, h), gamma_post, _flat(gate, h), res_scale, gamma_pre, eps)
+
+
 def _register_fakes() -> None:
     """Fake (meta) implementations: every annotated operator only writes into tensors it is given."""
     def _nothing(*args, **kwargs):
         return None
 
-    for name in ("gemm_peak_out", "rms_norm_fwd_out", "rms_norm_bwd_out", "rms_norm_rstd", "gemm_peak_fused"):
+    for name in ("gemm_peak_out", "rms_norm_fwd_out", "rms_norm_bwd_out", "rms_norm_rstd", "gemm_peak_fused",
+                 "rms_norm_residual_fwd", "rms_norm_residual_bwd"):
         torch.library.register_fake(f"PeakGemm::{name}")(_nothing)
 
 
 _register_fakes()
 
 __all__ = ["gemm_peak", "rms_norm_fwd", "rms_norm_bwd", "gemm_peak_fused", "fold_gamma", "rms_norm_linear",
-           "TORCH_LIB_PATH", "DEVICE_LIB_PATH"]
+           "rms_norm_residual_fwd", "rms_norm_residual_bwd", "TORCH_LIB_PATH", "DEVICE_LIB_PATH"]

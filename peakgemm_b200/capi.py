@@ -44,6 +44,10 @@ SIGNATURES = {
     "pg_rmsnorm_bwd_workspace_bytes": (_sz, [_i64, _i64]),
     "pg_rmsnorm_bwd": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _f, _i, _p, _sz, _p]),
     "pg_rmsnorm_bwd_static": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _f, _i, _p]),
+    "pg_rmsnorm_residual_fwd": (_i, [_p, _p, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i64, _f, _i, _p]),
+    "pg_rmsnorm_residual_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "pg_rmsnorm_residual_bwd": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p, _i64, _p, _i64, _i64,
+                                     _f, _i, _p, _sz, _p]),
 }
 PG_STATIC_SCRATCH_BYTES = 160 * 8192 * 4
 
@@ -256,3 +260,39 @@ def rmsnorm_bwd_static(dx, dgamma, dy, x, gamma, eps: float = 1e-6, stream=None)
     check(lib().pg_rmsnorm_bwd_static(dx.data_ptr(), dgamma.data_ptr(), dy.data_ptr(), x.data_ptr(),
                                       gamma.data_ptr(), rows, h, eps, dtype_code(x.dtype), _stream_ptr(stream)),
           "pg_rmsnorm_bwd_static")
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
+
+
+def _len0(t):
+    return t.shape[0] if t is not None else 0
+
+
+def rmsnorm_residual_fwd(s, y, u, residual, *, gamma_post=None, gate=None, res_scale=None, gamma_pre=None,
+                         eps: float = 1e-6, stream=None) -> None:
+    """pg_rmsnorm_residual_fwd on 2-D tensors; absent terms are None."""
+    rows, h = u.shape
+    check(lib().pg_rmsnorm_residual_fwd(s.data_ptr(), _ptr(y), u.data_ptr(), residual.data_ptr(), _ptr(gamma_post),
+                                        _ptr(gate), _len0(gate), _ptr(res_scale), _len0(res_scale), _ptr(gamma_pre),
+                                        rows, h, eps, dtype_code(u.dtype), _stream_ptr(stream)),
+          "pg_rmsnorm_residual_fwd")
+
+
+def rmsnorm_residual_bwd_workspace_bytes(rows: int, h: int, gate_rows: int = 0) -> int:
+    return int(lib().pg_rmsnorm_residual_bwd_workspace_bytes(rows, h, gate_rows))
+
+
+def rmsnorm_residual_bwd(du, dresidual, dy, ds, s, u, workspace, *, residual=None, gamma_post=None, gate=None,
+                         res_scale=None, gamma_pre=None, dgamma_post=None, dgate=None, dres_scale=None,
+                         dgamma_pre=None, eps: float = 1e-6, stream=None) -> None:
+    """pg_rmsnorm_residual_bwd on 2-D tensors; absent terms and unwanted gradients are None."""
+    rows, h = du.shape
+    check(lib().pg_rmsnorm_residual_bwd(du.data_ptr(), dresidual.data_ptr(), _ptr(dgamma_post), _ptr(dgate),
+                                        _ptr(dres_scale), _ptr(dgamma_pre), _ptr(dy), _ptr(ds), _ptr(s), _ptr(u),
+                                        _ptr(residual), _ptr(gamma_post), _ptr(gate), _len0(gate), _ptr(res_scale),
+                                        _len0(res_scale), _ptr(gamma_pre), rows, h, eps, dtype_code(du.dtype),
+                                        workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+                                        _stream_ptr(stream)),
+          "pg_rmsnorm_residual_bwd")

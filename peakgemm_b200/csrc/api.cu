@@ -33,6 +33,20 @@ int from_launch(int r, cudaError_t e) {
 
 constexpr int64_t kMaxDim = (int64_t(1) << 31) - 1;
 
+// The arguments that pg_rmsnorm_residual_fwd and _bwd share.
+int check_residual_terms(const float *gamma_post, const void *gate, int64_t gate_rows, const float *res_scale,
+                         int64_t res_scale_len, const float *gamma_pre, int64_t rows, int64_t h, int dtype) {
+    if (rows < 0 || h <= 0 || gate_rows < 0) return PG_ERR_BAD_ARG;
+    if (dtype != PG_F16 && dtype != PG_BF16) return PG_ERR_BAD_ARG;
+    if ((gate != nullptr) != (gate_rows > 0) || (res_scale != nullptr) != (res_scale_len > 0)) return PG_ERR_BAD_ARG;
+    if (res_scale && res_scale_len != 1 && res_scale_len != h) return PG_ERR_BAD_ARG;
+    if (gate && rows % gate_rows != 0) return PG_ERR_BAD_ARG;
+    if (h % 8 != 0 || h > kMaxDim || rows > kMaxDim) return PG_ERR_UNSUPPORTED;
+    if (!aligned16(gamma_post) || !aligned16(gate) || !aligned16(gamma_pre)) return PG_ERR_MISALIGNED;
+    if (res_scale_len > 1 && !aligned16(res_scale)) return PG_ERR_MISALIGNED;
+    return PG_OK;
+}
+
 }  // namespace
 
 namespace pg {
@@ -284,6 +298,70 @@ int pg_rmsnorm_bwd(void *dx, float *dgamma, const void *dy, const void *x, const
         return PG_ERR_WORKSPACE;
     pg::RmsBwdArgs a{dx, dgamma, dy, x, gamma, rows, h, eps, dtype == PG_BF16, workspace};
     e = pg::rmsnorm_bwd_launch(a, ctas, s);
+    return e == cudaSuccess ? PG_OK : cuda_fail(e);
+}
+
+int pg_rmsnorm_residual_fwd(void *s, void *y, const void *u, const void *residual, const float *gamma_post,
+                            const void *gate, int64_t gate_rows, const float *res_scale, int64_t res_scale_len,
+                            const float *gamma_pre, int64_t rows, int64_t h, float eps, int dtype, void *stream) {
+    const int st = check_residual_terms(gamma_post, gate, gate_rows, res_scale, res_scale_len, gamma_pre, rows, h, dtype);
+    if (st != PG_OK) return st;
+    if (rows == 0) return PG_OK;
+    if ((y != nullptr) != (gamma_pre != nullptr)) return PG_ERR_BAD_ARG;
+    if (!s || !u || !residual) return PG_ERR_BAD_ARG;
+    if (!aligned16(s) || !aligned16(y) || !aligned16(u) || !aligned16(residual)) return PG_ERR_MISALIGNED;
+    const pg::RmsResidualFwdArgs a{{gamma_post, gate, gate_rows, res_scale, res_scale_len == 1, gamma_pre, rows, h, eps,
+                                    dtype == PG_BF16}, s, y, u, residual};
+    const cudaError_t e = pg::rmsnorm_residual_fwd_launch(a, static_cast<cudaStream_t>(stream));
+    return e == cudaSuccess ? PG_OK : cuda_fail(e);
+}
+
+size_t pg_rmsnorm_residual_bwd_workspace_bytes(int64_t rows, int64_t h, int64_t gate_rows) {
+    if (rows <= 0 || h <= 0 || gate_rows < 0 || h % 8 != 0 || h > kMaxDim || rows > kMaxDim) return 0;
+    size_t bytes = 0;
+    if (pg::rmsnorm_residual_bwd_bytes(rows, h, gate_rows, &bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return bytes;
+}
+
+int pg_rmsnorm_residual_bwd(void *du, void *dresidual, float *dgamma_post, void *dgate, float *dres_scale,
+                            float *dgamma_pre, const void *dy, const void *ds, const void *s, const void *u,
+                            const void *residual, const float *gamma_post, const void *gate, int64_t gate_rows,
+                            const float *res_scale, int64_t res_scale_len, const float *gamma_pre, int64_t rows,
+                            int64_t h, float eps, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+    const int st = check_residual_terms(gamma_post, gate, gate_rows, res_scale, res_scale_len, gamma_pre, rows, h, dtype);
+    if (st != PG_OK) return st;
+    if ((dgamma_post && !gamma_post) || (dgate && !gate) || (dres_scale && !res_scale) || (dgamma_pre && !gamma_pre))
+        return PG_ERR_BAD_ARG;
+    if (!aligned16(dgamma_post) || !aligned16(dgate) || !aligned16(dgamma_pre) ||
+        (res_scale_len > 1 && !aligned16(dres_scale)))
+        return PG_ERR_MISALIGNED;
+    cudaStream_t q = static_cast<cudaStream_t>(stream);
+    if (rows == 0) {   // empty sums
+        const size_t row = static_cast<size_t>(h) * sizeof(float);
+        cudaError_t e = cudaSuccess;
+        if (dgamma_post) e = cudaMemsetAsync(dgamma_post, 0, row, q);
+        if (e == cudaSuccess && dgamma_pre) e = cudaMemsetAsync(dgamma_pre, 0, row, q);
+        if (e == cudaSuccess && dres_scale) e = cudaMemsetAsync(dres_scale, 0, static_cast<size_t>(res_scale_len) * sizeof(float), q);
+        if (e == cudaSuccess && dgate) e = cudaMemsetAsync(dgate, 0, static_cast<size_t>(gate_rows) * h * 2, q);
+        return e == cudaSuccess ? PG_OK : cuda_fail(e);
+    }
+    if ((dy != nullptr) != (gamma_pre != nullptr) || (!dy && !ds)) return PG_ERR_BAD_ARG;
+    if (!du || !dresidual || !workspace || (dy && !s) || ((gamma_post || dgate) && !u) || (dres_scale && !residual))
+        return PG_ERR_BAD_ARG;
+    if (!aligned16(du) || !aligned16(dresidual) || !aligned16(dy) || !aligned16(ds) || !aligned16(s) || !aligned16(u) ||
+        !aligned16(residual) || (reinterpret_cast<uintptr_t>(workspace) & 255u))
+        return PG_ERR_MISALIGNED;
+    size_t need = 0;
+    cudaError_t e = pg::rmsnorm_residual_bwd_bytes(rows, h, gate_rows, &need);
+    if (e != cudaSuccess) return cuda_fail(e);
+    if (workspace_bytes < need) return PG_ERR_WORKSPACE;
+    const pg::RmsResidualBwdArgs a{{gamma_post, gate, gate_rows, res_scale, res_scale_len == 1, gamma_pre, rows, h, eps,
+                                    dtype == PG_BF16}, du, dresidual, dgamma_post, dgate, dres_scale, dgamma_pre, dy, ds,
+                                   s, u, residual, workspace};
+    e = pg::rmsnorm_residual_bwd_launch(a, q);
     return e == cudaSuccess ? PG_OK : cuda_fail(e);
 }
 

@@ -39,6 +39,37 @@ cudaError_t rmsnorm_bwd_launch(const RmsBwdArgs &a, int ctas, cudaStream_t strea
 cudaError_t rmsnorm_rstd_launch(float *rstd, const void *x, int64_t rows, int64_t h, float eps, bool bf16,
                                 cudaStream_t stream);
 
+// The norms around a block, its gate and the scaled residual (rmsnorm_residual.cu).  Null pointers: the term is absent.
+struct RmsResidualTerms {
+    const float *gamma_post;   // [h]: norm of the block's output u; null: u itself
+    const void *gate;          // [gate_rows, h] 16-bit, consecutive rows / gate_rows rows share one; null: 1
+    int64_t gate_rows;
+    const float *res_scale;    // [h] or [1]; null: 1
+    bool res_scale_one;        // res_scale has one element
+    const float *gamma_pre;    // [h]: norm of the new residual stream s; null: no y
+    int64_t rows, h;
+    float eps;
+    bool bf16;
+};
+struct RmsResidualFwdArgs {
+    RmsResidualTerms t;
+    void *s, *y;
+    const void *u, *residual;
+};
+struct RmsResidualBwdArgs {
+    RmsResidualTerms t;
+    void *du, *dresidual;
+    float *dgamma_post;
+    void *dgate;
+    float *dres_scale, *dgamma_pre;
+    const void *dy, *ds, *s, *u, *residual;
+    void *workspace;
+};
+cudaError_t rmsnorm_residual_fwd_launch(const RmsResidualFwdArgs &a, cudaStream_t stream);
+// Scratch of the backward pass for this shape on the current device.
+cudaError_t rmsnorm_residual_bwd_bytes(int64_t rows, int64_t h, int64_t gate_rows, size_t *bytes);
+cudaError_t rmsnorm_residual_bwd_launch(const RmsResidualBwdArgs &a, cudaStream_t stream);
+
 // Bulk-copy staged variants (rmsnorm_staged.cu), used for 2048 <= h <= 16384.
 bool rmsnorm_staged_supported(int64_t h, bool bwd);
 cudaError_t rmsnorm_staged_ctas(int64_t rows, int64_t h, bool bwd, int *ctas, int *partial_rows);

@@ -20,7 +20,8 @@
 // is kept verbatim for compatibility; next to it every operator has a twin `<name>_out` whose schema
 // marks the written tensors, registered for the CUDA key only (so fake/meta tracing never reaches the
 // kernels; the fake implementations live in the Python package).  gemm_peak_fused and rms_norm_rstd
-// (fused epilogue, RMSNorm folded into the projection) exist only in the annotated form.
+// (fused epilogue, RMSNorm folded into the projection) and rms_norm_residual_fwd / _bwd (the norms around a
+// block with its gate and the scaled residual) exist only in the annotated form.
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
@@ -194,6 +195,105 @@ void gemm_peak_fused(Tensor &d, const Tensor &a, const Tensor &b, const std::opt
                  "gemm_peak_fused");
 }
 
+// ------------------------------------------- norms around a gated residual ----
+
+using OptTensor = std::optional<Tensor>;
+
+void *opt_ptr(const OptTensor &t) { return t ? t->data_ptr() : nullptr; }
+float *opt_f32(const OptTensor &t) { return t ? t->data_ptr<float>() : nullptr; }
+
+// `t`, where given, is a dense tensor of `type` with `numel` elements on like's device.
+void check_opt(const OptTensor &t, const Tensor &like, at::ScalarType type, int64_t numel, const char *op, const char *what) {
+    if (!t) return;
+    TORCH_CHECK(t->is_cuda() && t->device() == like.device(), op, ": ", what, " must be on the other tensors' CUDA device");
+    TORCH_CHECK(t->is_contiguous() && t->scalar_type() == type && t->numel() == numel, op, ": ", what,
+                " must be contiguous, of type ", type, " and have ", numel, " elements");
+}
+
+struct ResidualTerms {
+    int64_t rows, h, gate_rows, res_scale_len;
+    int dtype;
+};
+
+ResidualTerms check_residual_terms(const Tensor &u, const OptTensor &gamma_post, const OptTensor &gate,
+                                   const OptTensor &res_scale, const OptTensor &gamma_pre, const char *op) {
+    TORCH_CHECK(u.is_cuda(), op, ": tensors must be on a CUDA device");
+    TORCH_CHECK(u.dim() >= 1 && u.is_contiguous(), op, ": tensors must be contiguous [..., h]");
+    ResidualTerms t;
+    t.dtype = dtype_code(u, op);
+    t.h = u.size(-1);
+    t.rows = t.h > 0 ? u.numel() / t.h : 0;
+    check_opt(gamma_post, u, at::kFloat, t.h, op, "gamma_post");
+    check_opt(gamma_pre, u, at::kFloat, t.h, op, "gamma_pre");
+    t.gate_rows = 0;
+    if (gate) {
+        TORCH_CHECK(gate->dim() >= 1 && gate->size(-1) == t.h, op, ": gate must be [..., h]");
+        t.gate_rows = t.h > 0 ? gate->numel() / t.h : 0;
+        TORCH_CHECK(t.gate_rows > 0 && t.rows % t.gate_rows == 0, op, ": the rows of gate must divide the rows of u");
+        check_opt(gate, u, u.scalar_type(), t.gate_rows * t.h, op, "gate");
+    }
+    t.res_scale_len = res_scale ? res_scale->numel() : 0;
+    TORCH_CHECK(!res_scale || t.res_scale_len == 1 || t.res_scale_len == t.h, op, ": res_scale must have 1 or h elements");
+    check_opt(res_scale, u, at::kFloat, t.res_scale_len, op, "res_scale");
+    return t;
+}
+
+void rms_norm_residual_fwd(Tensor &s, const OptTensor &y, const Tensor &u, const Tensor &residual,
+                           const OptTensor &gamma_post, const OptTensor &gate, const OptTensor &res_scale,
+                           const OptTensor &gamma_pre, double eps) {
+    const char *op = "rms_norm_residual_fwd";
+    const ResidualTerms t = check_residual_terms(u, gamma_post, gate, res_scale, gamma_pre, op);
+    TORCH_CHECK(y.has_value() == gamma_pre.has_value(), op, ": y and gamma_pre come together");
+    check_opt(s, u, u.scalar_type(), u.numel(), op, "s");
+    check_opt(y, u, u.scalar_type(), u.numel(), op, "y");
+    check_opt(residual, u, u.scalar_type(), u.numel(), op, "residual");
+    c10::DeviceGuard device_guard(u.device());
+    auto stream = at::cuda::getCurrentCUDAStream();
+    check_status(pg_rmsnorm_residual_fwd(s.data_ptr(), opt_ptr(y), u.data_ptr(), residual.data_ptr(), opt_f32(gamma_post),
+                                         opt_ptr(gate), t.gate_rows, opt_f32(res_scale), t.res_scale_len,
+                                         opt_f32(gamma_pre), t.rows, t.h, static_cast<float>(eps), t.dtype,
+                                         stream.stream()),
+                 op);
+}
+
+void rms_norm_residual_bwd(Tensor &du, Tensor &dresidual, const OptTensor &dgamma_post, const OptTensor &dgate,
+                           const OptTensor &dres_scale, const OptTensor &dgamma_pre, const OptTensor &dy,
+                           const OptTensor &ds, const OptTensor &s, const OptTensor &u, const OptTensor &residual,
+                           const OptTensor &gamma_post, const OptTensor &gate, const OptTensor &res_scale,
+                           const OptTensor &gamma_pre, double eps) {
+    const char *op = "rms_norm_residual_bwd";
+    const ResidualTerms t = check_residual_terms(du, gamma_post, gate, res_scale, gamma_pre, op);
+    const at::ScalarType type = du.scalar_type();
+    const int64_t n = du.numel();
+    TORCH_CHECK(dy.has_value() == gamma_pre.has_value(), op, ": dy and gamma_pre come together");
+    TORCH_CHECK(dy || ds, op, ": at least one of dy and ds is needed");
+    TORCH_CHECK(s || !gamma_pre, op, ": gamma_pre needs s");
+    TORCH_CHECK(u || !(gamma_post || dgate), op, ": gamma_post and dgate need u");
+    TORCH_CHECK(residual || !dres_scale, op, ": dres_scale needs residual");
+    TORCH_CHECK((gamma_post || !dgamma_post) && (gate || !dgate) && (res_scale || !dres_scale) && (gamma_pre || !dgamma_pre),
+                op, ": a gradient needs the tensor it is the gradient of");
+    check_opt(dresidual, du, type, n, op, "dresidual");
+    check_opt(dy, du, type, n, op, "dy");
+    check_opt(ds, du, type, n, op, "ds");
+    check_opt(s, du, type, n, op, "s");
+    check_opt(u, du, type, n, op, "u");
+    check_opt(residual, du, type, n, op, "residual");
+    check_opt(dgamma_post, du, at::kFloat, t.h, op, "dgamma_post");
+    check_opt(dgamma_pre, du, at::kFloat, t.h, op, "dgamma_pre");
+    check_opt(dgate, du, type, t.gate_rows * t.h, op, "dgate");
+    check_opt(dres_scale, du, at::kFloat, t.res_scale_len, op, "dres_scale");
+    c10::DeviceGuard device_guard(du.device());
+    auto stream = at::cuda::getCurrentCUDAStream();
+    const size_t ws_bytes = pg_rmsnorm_residual_bwd_workspace_bytes(t.rows, t.h, t.gate_rows);
+    Tensor ws = at::empty({static_cast<int64_t>(ws_bytes > 0 ? ws_bytes : 16)}, du.options().dtype(at::kByte));
+    check_status(pg_rmsnorm_residual_bwd(du.data_ptr(), dresidual.data_ptr(), opt_f32(dgamma_post), opt_ptr(dgate),
+                                         opt_f32(dres_scale), opt_f32(dgamma_pre), opt_ptr(dy), opt_ptr(ds), opt_ptr(s),
+                                         opt_ptr(u), opt_ptr(residual), opt_f32(gamma_post), opt_ptr(gate), t.gate_rows,
+                                         opt_f32(res_scale), t.res_scale_len, opt_f32(gamma_pre), t.rows, t.h,
+                                         static_cast<float>(eps), t.dtype, ws.data_ptr(), ws_bytes, stream.stream()),
+                 op);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(PeakGemm, m) {
@@ -210,6 +310,11 @@ TORCH_LIBRARY(PeakGemm, m) {
     m.def("rms_norm_rstd(Tensor(a!) rstd, Tensor x, float eps) -> ()");
     m.def("gemm_peak_fused(Tensor(a!) d, Tensor a, Tensor b, Tensor? row_scale, Tensor? bias, Tensor? residual, "
           "bool pdl=False) -> ()");
+    m.def("rms_norm_residual_fwd(Tensor(a!) s, Tensor(b!)? y, Tensor u, Tensor residual, Tensor? gamma_post, Tensor? gate, "
+          "Tensor? res_scale, Tensor? gamma_pre, float eps) -> ()");
+    m.def("rms_norm_residual_bwd(Tensor(a!) du, Tensor(b!) dresidual, Tensor(c!)? dgamma_post, Tensor(d!)? dgate, "
+          "Tensor(e!)? dres_scale, Tensor(f!)? dgamma_pre, Tensor? dy, Tensor? ds, Tensor? s, Tensor? u, "
+          "Tensor? residual, Tensor? gamma_post, Tensor? gate, Tensor? res_scale, Tensor? gamma_pre, float eps) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(PeakGemm, CUDA, m) {
@@ -218,4 +323,6 @@ TORCH_LIBRARY_IMPL(PeakGemm, CUDA, m) {
     m.impl("rms_norm_bwd_out", &rms_norm_bwd_out);
     m.impl("rms_norm_rstd", &rms_norm_rstd);
     m.impl("gemm_peak_fused", &gemm_peak_fused);
+    m.impl("rms_norm_residual_fwd", &rms_norm_residual_fwd);
+    m.impl("rms_norm_residual_bwd", &rms_norm_residual_bwd);
 }
