@@ -170,6 +170,33 @@ int pg_hgemm_fused(void *d, const void *a, const void *b,
                    int dtype, int flags, void *stream);
 
 /*
+ * pg_hgemm_fused with low-rank adapters of many requests beside the shared weights: row i of the batch (a token)
+ * uses adapter t = ids[i] of a pool, or none,
+ *     d[i,j] = round_to_dtype(row_scale[i] * (sum_k a[i,k] b[j,k] + scale[t] * sum_r v[i,r] lora_b[t,j,r]) + bias[j]
+ *                             + residual[i,j]),        v[i,r] = sum_k a[i,k] lora_a[t,r,k]
+ * with fp32 sums and optional terms as there.
+ *   lora_a   [adapters, rank, k] of `dtype`, dense: the down projections, in the weights' layout
+ *   lora_b   [adapters, n, rank] of `dtype`, dense: the up projections, in the weights' layout
+ *   ids      [m] int32, any order; an id outside 0 .. adapters-1 (e.g. -1): the row has no adapter
+ *   scale    [adapters] fp32, or null (1)
+ * An adapter of a smaller rank is padded with zeros in lora_a or lora_b, and finite values in the other.  With
+ * row_scale = rstd, fold gamma into lora_a as into b.  adapters == 0 is pg_hgemm_fused.
+ * rank % 8 == 0, 8 <= rank <= 512, adapters * rank and adapters * n < 2^31; otherwise pg_hgemm_fused's
+ * preconditions.  residual may be d itself.  workspace: pg_hgemm_lora_workspace_bytes bytes, 256-byte aligned device
+ * memory, no initialisation, private to the call until its kernels have finished.
+ * The reference project has no adapters.
+ */
+size_t pg_hgemm_lora_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank);
+int pg_hgemm_lora(void *d, const void *a, const void *b,
+                  int64_t m, int64_t n, int64_t k,
+                  int64_t lda, int64_t ldb, int64_t ldd,
+                  const void *lora_a, const void *lora_b, const int32_t *ids,
+                  int64_t adapters, int64_t rank, const float *scale,
+                  const float *row_scale, const void *bias,
+                  const void *residual, int64_t ldr,
+                  int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
  * fp32 C[m,n] = A[m,k] * B[n,k]^T with true fp32 FMA accumulation (CUDA cores, no
  * TF32): the float branch of the gemm_peak operator, where the reference calls
  * sgemm::sgemm_peak (src/ops/gemm.cpp:34-43, src/impl/sgemm_impl.h:310-320) — by its

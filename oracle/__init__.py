@@ -336,3 +336,62 @@ def rmsnorm_residual_inputs(rows: int, h: int, dtype: torch.dtype, seed: int, *,
     x["gate"] = (0.5 * n(gates, h)).to(dtype) if gates else None
     x["res_scale"] = 1 + 0.1 * n(res_scale) if res_scale else None
     return x
+
+
+# --------------------------------------------------- adapters beside a projection ----
+# PARITY UNPINNED: the reference has no adapters; the definition in float64, on the inputs' device.
+
+def gemm_lora(a, b, lora_a, lora_b, ids, scale=None, row_scale=None, bias=None, residual=None):
+    """(d, bound) unrounded, float64.
+
+    bound: fp32 sums of products in another order are within 2^-17 of the sum of absolute values (gemm_fused_slack);
+    v = scale * a A^T may be rounded once to the 16-bit type before the second product: half a step, eps / 2 of itself
+    (and half the smallest step, where v is below the normal range)."""
+    L, r, k = lora_a.shape
+    ids = ids.long()
+    u16 = torch.finfo(a.dtype).eps / 2
+    tiny = torch.finfo(a.dtype).smallest_normal * torch.finfo(a.dtype).eps / 2
+    x, w = a.double(), b.double()
+    d, e = x @ w.t(), 2.0 ** -17 * (x.abs() @ w.abs().t())
+    for i in range(L):
+        t = (ids == i).nonzero()[:, 0]
+        if t.numel() == 0:
+            continue
+        s = 1.0 if scale is None else float(scale[i])
+        A, B = lora_a[i].double(), lora_b[i].double()
+        v = s * (x[t] @ A.t())
+        ev = u16 * v.abs() + tiny + 2.0 ** -17 * abs(s) * (x[t].abs() @ A.abs().t())
+        d[t] += v @ B.t()
+        e[t] += (ev + 2.0 ** -17 * v.abs()) @ B.abs().t()
+    if row_scale is not None:
+        d, e = d * row_scale.double()[:, None], e * row_scale.double().abs()[:, None]
+    for term in (bias, residual):
+        if term is not None:
+            d = d + term.double()
+            e = e + 2.0 ** -23 * term.double().abs()
+    return d, e + 2.0 ** -22 * d.abs()
+
+
+def gemm_lora_inputs(m: int, n: int, k: int, adapters: int, rank: int, dtype: torch.dtype, seed: int, ids: str = "mixed"):
+    """Seeded inputs: x ~ N(0,1), W ~ N(0, 0.02), A ~ N(0, 1/k), B ~ N(0, 0.02), scales in [0.5, 2); about an eighth of
+    the rows without an adapter.  ids: "mixed" token by token, "runs" of one adapter each, "one", "none"."""
+    g = torch.Generator().manual_seed(seed)
+    n_ = lambda *s: torch.randn(*s, generator=g)    # noqa: E731
+    x = {"a": n_(m, k).to(dtype), "b": (0.02 * n_(n, k)).to(dtype), "lora_a": (k ** -0.5 * n_(adapters, rank, k)).to(dtype),
+         "lora_b": (0.02 * n_(adapters, n, rank)).to(dtype), "scale": 0.5 + 1.5 * torch.rand(adapters, generator=g)}
+    i = torch.randint(0, adapters, (m,), generator=g)
+    i[torch.rand(m, generator=g) < 0.125] = -1
+    if ids == "runs":
+        i = i.sort().values
+    elif ids == "one":
+        i[:] = adapters - 1
+    elif ids == "none":
+        i[:] = -1
+    x["ids"] = i.int()
+    return x
+
+
+def gemm_lora_terms(m: int, n: int, dtype: torch.dtype, seed: int):
+    g = torch.Generator().manual_seed(seed)
+    return {"row_scale": 0.5 + torch.rand(m, generator=g), "bias": torch.randn(n, generator=g).to(dtype),
+            "residual": torch.randn(m, n, generator=g).to(dtype)}

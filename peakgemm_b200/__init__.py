@@ -13,6 +13,7 @@ epilogue is a plain cast and whose schema is not annotated):
 * ``gemm_peak_fused``: row scale, bias and residual folded into the GEMM epilogue;
 * ``fold_gamma`` + ``rms_norm_linear``: RMSNorm followed by a projection as ONE
   GEMM over the raw activations (rstd applied per row in the epilogue);
+* ``gemm_peak_lora``: the projection with every token's low-rank adapter beside the weights;
 * ``rms_norm_residual_fwd`` / ``rms_norm_residual_bwd``: the norm after a block, its gate,
   the scaled residual and the norm before the next block in one pass, and the gradients;
 * ``torch.ops.PeakGemm.*_out`` / ``gemm_peak_fused`` / ``rms_norm_rstd``: schemas
@@ -109,6 +110,30 @@ def gemm_peak_fused(d: torch.Tensor, a: torch.Tensor, b: torch.Tensor, *, row_sc
     torch.ops.PeakGemm.gemm_peak_fused(d2, a2, b, rs, bias, res, pdl)
 
 
+def gemm_peak_lora(d: torch.Tensor, a: torch.Tensor, b: torch.Tensor, lora_a: torch.Tensor, lora_b: torch.Tensor,
+                   ids: torch.Tensor, *, scale: torch.Tensor | None = None, row_scale: torch.Tensor | None = None,
+                   bias: torch.Tensor | None = None, residual: torch.Tensor | None = None) -> None:
+    """gemm_peak_fused with low-rank adapters of many requests beside the shared weights, in place.
+
+        d[t] = row_scale[t] * (a[t] @ b^T + scale[i] * (a[t] @ lora_a[i]^T) @ lora_b[i]^T) + bias + residual[t],  i = ids[t]
+
+    ``lora_a``: [L, r, k], ``lora_b``: [L, n, r], of a's dtype, r a multiple of 8 up to 512 (pad smaller ranks with zeros);
+    ``ids``: int32, one per row of ``a``, in any order; an id outside 0..L-1 (such as -1) means no adapter.  ``scale``:
+    float32 [L].  The other terms as in ``gemm_peak_fused``; with ``row_scale`` = rstd (``rms_norm_linear``) fold gamma
+    into lora_a as into the weights: ``fold_gamma(lora_a.view(-1, k), gamma).view_as(lora_a)``.
+    """
+    assert a.dtype in [torch.half, torch.bfloat16]
+    k = a.shape[-1]
+    n = b.shape[0]
+    assert b.shape[1] == k and lora_a.shape[2] == k and lora_b.shape == (lora_a.shape[0], n, lora_a.shape[1])
+    a2 = a.view(-1, k)
+    d2 = d.view(-1, n)
+    assert d2.shape[0] == a2.shape[0] and ids.numel() == a2.shape[0]
+    rs = row_scale.view(-1) if row_scale is not None else None
+    res = residual.view(-1, n) if residual is not None else None
+    torch.ops.PeakGemm.gemm_peak_lora(d2, a2, b, lora_a, lora_b, ids.view(-1), scale, rs, bias, res)
+
+
 def fold_gamma(w: torch.Tensor, gamma: torch.Tensor) -> torch.Tensor:
     """Weights with RMSNorm's gain folded in: w'[n, k] = round(w[n, k] * gamma[k]).  Done once per weight."""
     assert w.shape[1] == gamma.shape[0]
@@ -196,11 +221,11 @@ def _register_fakes() -> None:
         return None
 
     for name in ("gemm_peak_out", "rms_norm_fwd_out", "rms_norm_bwd_out", "rms_norm_rstd", "gemm_peak_fused",
-                 "rms_norm_residual_fwd", "rms_norm_residual_bwd"):
+                 "gemm_peak_lora", "rms_norm_residual_fwd", "rms_norm_residual_bwd"):
         torch.library.register_fake(f"PeakGemm::{name}")(_nothing)
 
 
 _register_fakes()
 
 __all__ = ["gemm_peak", "rms_norm_fwd", "rms_norm_bwd", "gemm_peak_fused", "fold_gamma", "rms_norm_linear",
-           "rms_norm_residual_fwd", "rms_norm_residual_bwd", "TORCH_LIB_PATH", "DEVICE_LIB_PATH"]
+           "gemm_peak_lora", "rms_norm_residual_fwd", "rms_norm_residual_bwd", "TORCH_LIB_PATH", "DEVICE_LIB_PATH"]

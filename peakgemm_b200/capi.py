@@ -27,6 +27,9 @@ SIGNATURES = {
     "pg_hgemm_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "pg_hgemm_ws": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i, _p, _sz, _p]),
     "pg_hgemm_fused": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _i, _i, _p]),
+    "pg_hgemm_lora_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "pg_hgemm_lora": (_i, [_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _i64, _p, _p, _p, _p, _i64, _i,
+                           _p, _sz, _p]),
     "pg_rmsnorm_rstd": (_i, [_p, _p, _i64, _i64, ctypes.c_float, _i, _p]),
     "pg_hgemm_multi": (_i, [ctypes.POINTER(_p), _i, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _p]),
     "pg_hgemm_mcast": (_i, [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i, _i, _p]),
@@ -141,6 +144,26 @@ def hgemm_fused(d, a, b, *, row_scale=None, bias=None, residual=None, pdl: bool 
                               ptr(residual), ldr, dtype_code(a.dtype), PG_FUSED_PDL if pdl else 0,
                               _stream_ptr(stream))
     check(st, "pg_hgemm_fused")
+
+
+def hgemm_lora_workspace_bytes(m: int, n: int, k: int, adapters: int, rank: int) -> int:
+    return int(lib().pg_hgemm_lora_workspace_bytes(m, n, k, adapters, rank))
+
+
+def hgemm_lora(d, a, b, lora_a, lora_b, ids, workspace, *, scale=None, row_scale=None, bias=None, residual=None,
+               stream=None) -> None:
+    """pg_hgemm_lora on 2-D matrices (row pitches as they are) and a dense pool lora_a [L, R, k], lora_b [L, n, R]."""
+    m, k = a.shape
+    n = b.shape[0]
+    ptr = lambda t: t.data_ptr() if t is not None else None
+    ldr = (residual.stride(0) if m > 1 else n) if residual is not None else 0
+    st = lib().pg_hgemm_lora(d.data_ptr(), a.data_ptr(), b.data_ptr(), m, n, k, a.stride(0) if m > 1 else k,
+                             b.stride(0) if n > 1 else k, d.stride(0) if m > 1 else n, lora_a.data_ptr(),
+                             lora_b.data_ptr(), ids.data_ptr(), lora_a.shape[0], lora_a.shape[1], ptr(scale),
+                             ptr(row_scale), ptr(bias), ptr(residual), ldr, dtype_code(a.dtype), ptr(workspace),
+                             workspace.numel() * workspace.element_size() if workspace is not None else 0,
+                             _stream_ptr(stream))
+    check(st, "pg_hgemm_lora")
 
 
 def rmsnorm_rstd(rstd, x, eps: float = 1e-6, stream=None) -> None:

@@ -7,6 +7,7 @@
 #include "../../include/peakgemm.h"
 #include "gemm_sm100.h"
 #include "host_util.h"
+#include "lora.h"
 #include "rmsnorm.h"
 #include "sgemm.h"
 
@@ -32,6 +33,7 @@ int from_launch(int r, cudaError_t e) {
 }
 
 constexpr int64_t kMaxDim = (int64_t(1) << 31) - 1;
+constexpr int64_t kMaxRank = 512;
 
 // The arguments that pg_rmsnorm_residual_fwd and _bwd share.
 int check_residual_terms(const float *gamma_post, const void *gate, int64_t gate_rows, const float *res_scale,
@@ -165,13 +167,14 @@ int pg_hgemm_mcast(void *c_local, void *c_multicast, const void *a, const void *
     return from_launch(r, e);
 }
 
-int pg_hgemm_fused(void *d, const void *a, const void *b, int64_t m, int64_t n, int64_t k, int64_t lda,
-                   int64_t ldb, int64_t ldd, const float *row_scale, const void *bias, const void *residual,
-                   int64_t ldr, int dtype, int flags, void *stream) {
-    if (m < 0 || n < 0 || k < 0) return PG_ERR_BAD_ARG;
-    if (dtype != PG_F16 && dtype != PG_BF16) return PG_ERR_BAD_ARG;
-    if (flags & ~PG_FUSED_PDL) return PG_ERR_BAD_ARG;
-    if (m == 0 || n == 0) return PG_OK;
+}  // extern "C"
+
+namespace {
+
+// The arguments that pg_hgemm_fused and pg_hgemm_lora share, with m, n > 0; fills `g`.
+int fused_args(pg::GemmArgs &g, void *d, const void *a, const void *b, int64_t m, int64_t n, int64_t k, int64_t lda,
+               int64_t ldb, int64_t ldd, const float *row_scale, const void *bias, const void *residual, int64_t ldr,
+               int dtype) {
     if (k == 0) return PG_ERR_UNSUPPORTED;
     if (!d || !a || !b) return PG_ERR_BAD_ARG;
     if (lda < k || ldb < k || ldd < n) return PG_ERR_BAD_ARG;
@@ -183,14 +186,60 @@ int pg_hgemm_fused(void *d, const void *a, const void *b, int64_t m, int64_t n, 
     if ((bias && !aligned16(bias)) || (residual && !aligned16(residual)) ||
         (row_scale && (reinterpret_cast<uintptr_t>(row_scale) & 3u)))
         return PG_ERR_MISALIGNED;
-    pg::GemmArgs g{d, a, b, m, n, k, lda, ldb, ldd, dtype == PG_BF16};
+    g = pg::GemmArgs{d, a, b, m, n, k, lda, ldb, ldd, dtype == PG_BF16};
     g.row_scale = row_scale;
     g.bias = bias;
     g.residual = residual;
     g.ldr = residual ? ldr : 0;
+    return PG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int pg_hgemm_fused(void *d, const void *a, const void *b, int64_t m, int64_t n, int64_t k, int64_t lda,
+                   int64_t ldb, int64_t ldd, const float *row_scale, const void *bias, const void *residual,
+                   int64_t ldr, int dtype, int flags, void *stream) {
+    if (m < 0 || n < 0 || k < 0) return PG_ERR_BAD_ARG;
+    if (dtype != PG_F16 && dtype != PG_BF16) return PG_ERR_BAD_ARG;
+    if (flags & ~PG_FUSED_PDL) return PG_ERR_BAD_ARG;
+    if (m == 0 || n == 0) return PG_OK;
+    pg::GemmArgs g;
+    const int st = fused_args(g, d, a, b, m, n, k, lda, ldb, ldd, row_scale, bias, residual, ldr, dtype);
+    if (st != PG_OK) return st;
     g.pdl_wait = (flags & PG_FUSED_PDL) != 0;
     cudaError_t e = cudaSuccess;
     const int r = pg::hgemm_launch(g, 0, 0, 0, static_cast<cudaStream_t>(stream), &e);
+    return from_launch(r, e);
+}
+
+size_t pg_hgemm_lora_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank) {
+    if (m <= 0 || n <= 0 || k <= 0 || adapters <= 0 || rank <= 0 || rank > kMaxRank || m > kMaxDim) return 0;
+    return pg::lora_workspace_bytes(m, n, k, adapters, rank);
+}
+
+int pg_hgemm_lora(void *d, const void *a, const void *b, int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb,
+                  int64_t ldd, const void *lora_a, const void *lora_b, const int32_t *ids, int64_t adapters,
+                  int64_t rank, const float *scale, const float *row_scale, const void *bias, const void *residual,
+                  int64_t ldr, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+    if (m < 0 || n < 0 || k < 0 || adapters < 0) return PG_ERR_BAD_ARG;
+    if (dtype != PG_F16 && dtype != PG_BF16) return PG_ERR_BAD_ARG;
+    if (m == 0 || n == 0) return PG_OK;
+    if (adapters == 0)
+        return pg_hgemm_fused(d, a, b, m, n, k, lda, ldb, ldd, row_scale, bias, residual, ldr, dtype, 0, stream);
+    pg::GemmArgs g;
+    const int st = fused_args(g, d, a, b, m, n, k, lda, ldb, ldd, row_scale, bias, residual, ldr, dtype);
+    if (st != PG_OK) return st;
+    if (!lora_a || !lora_b || !ids || !workspace || rank <= 0) return PG_ERR_BAD_ARG;
+    if (rank % 8 != 0 || rank > kMaxRank || adapters > kMaxDim / rank || adapters > kMaxDim / n) return PG_ERR_UNSUPPORTED;
+    if (!aligned16(lora_a) || !aligned16(lora_b) || ((reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(scale)) & 3u) ||
+        (reinterpret_cast<uintptr_t>(workspace) & 255u))
+        return PG_ERR_MISALIGNED;
+    if (workspace_bytes < pg::lora_workspace_bytes(m, n, k, adapters, rank)) return PG_ERR_WORKSPACE;
+    const pg::LoraArgs l{lora_a, lora_b, ids, scale, adapters, rank, workspace};
+    cudaError_t e = cudaSuccess;
+    const int r = pg::hgemm_lora_launch(g, l, static_cast<cudaStream_t>(stream), &e);
     return from_launch(r, e);
 }
 

@@ -20,7 +20,7 @@
 // is kept verbatim for compatibility; next to it every operator has a twin `<name>_out` whose schema
 // marks the written tensors, registered for the CUDA key only (so fake/meta tracing never reaches the
 // kernels; the fake implementations live in the Python package).  gemm_peak_fused and rms_norm_rstd
-// (fused epilogue, RMSNorm folded into the projection) and rms_norm_residual_fwd / _bwd (the norms around a
+// (fused epilogue, RMSNorm folded into the projection), gemm_peak_lora (adapters beside the weights) and rms_norm_residual_fwd / _bwd (the norms around a
 // block with its gate and the scaled residual) exist only in the annotated form.
 
 #include <ATen/ATen.h>
@@ -155,49 +155,98 @@ void rms_norm_rstd(Tensor &rstd, const Tensor &x, double eps) {
                  "rms_norm_rstd");
 }
 
-// d[m,n] = row_scale[:,None] * (a[m,k] @ b[n,k]^T) + bias[None,:] + residual, each term optional.
-void gemm_peak_fused(Tensor &d, const Tensor &a, const Tensor &b, const std::optional<Tensor> &row_scale,
-                     const std::optional<Tensor> &bias, const std::optional<Tensor> &residual, bool pdl) {
-    TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && d.dim() == 2, "gemm_peak_fused: a [m,k], b [n,k], d [m,n]");
+using OptTensor = std::optional<Tensor>;
+
+struct FusedTerms {
+    int64_t m, n, k;
+    int dtype;
+    const float *row_scale = nullptr;
+    const void *bias = nullptr, *residual = nullptr;
+};
+
+// The arguments that gemm_peak_fused and gemm_peak_lora share.
+FusedTerms check_fused_terms(const Tensor &d, const Tensor &a, const Tensor &b, const OptTensor &row_scale,
+                             const OptTensor &bias, const OptTensor &residual, const char *op) {
+    TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && d.dim() == 2, op, ": a [m,k], b [n,k], d [m,n]");
     TORCH_CHECK(d.is_contiguous() && a.is_contiguous() && b.is_contiguous());
-    TORCH_CHECK(a.is_cuda() && b.is_cuda() && d.is_cuda() && a.device() == b.device() && a.device() == d.device(),
-                "gemm_peak_fused: tensors must be on one CUDA device");
-    TORCH_CHECK(a.scalar_type() == b.scalar_type() && a.scalar_type() == d.scalar_type(),
-                "gemm_peak_fused: a, b, d must have one dtype");
-    const int64_t m = a.size(0), k = a.size(1), n = b.size(0);
-    TORCH_CHECK(b.size(1) == k && d.size(0) == m && d.size(1) == n, "gemm_peak_fused: shapes do not match");
-    const float *rs = nullptr;
-    const void *bias_p = nullptr, *res_p = nullptr;
+    TORCH_CHECK(a.is_cuda() && b.is_cuda() && d.is_cuda() && a.device() == b.device() && a.device() == d.device(), op,
+                ": tensors must be on one CUDA device");
+    TORCH_CHECK(a.scalar_type() == b.scalar_type() && a.scalar_type() == d.scalar_type(), op,
+                ": a, b, d must have one dtype");
+    FusedTerms f;
+    f.m = a.size(0);
+    f.k = a.size(1);
+    f.n = b.size(0);
+    TORCH_CHECK(b.size(1) == f.k && d.size(0) == f.m && d.size(1) == f.n, op, ": shapes do not match");
     if (row_scale) {
         TORCH_CHECK(row_scale->is_cuda() && row_scale->device() == a.device() && row_scale->is_contiguous() &&
-                        row_scale->scalar_type() == at::kFloat && row_scale->numel() == m,
-                    "gemm_peak_fused: row_scale must be float32 [m] on a's device");
-        rs = row_scale->data_ptr<float>();
+                        row_scale->scalar_type() == at::kFloat && row_scale->numel() == f.m,
+                    op, ": row_scale must be float32 [m] on a's device");
+        f.row_scale = row_scale->data_ptr<float>();
     }
     if (bias) {
         TORCH_CHECK(bias->is_cuda() && bias->device() == a.device() && bias->is_contiguous() &&
-                        bias->scalar_type() == a.scalar_type() && bias->numel() == n,
-                    "gemm_peak_fused: bias must be [n] of a's dtype on a's device");
-        bias_p = bias->data_ptr();
+                        bias->scalar_type() == a.scalar_type() && bias->numel() == f.n,
+                    op, ": bias must be [n] of a's dtype on a's device");
+        f.bias = bias->data_ptr();
     }
     if (residual) {
         TORCH_CHECK(residual->is_cuda() && residual->device() == a.device() && residual->is_contiguous() &&
                         residual->scalar_type() == a.scalar_type() && residual->dim() == 2 &&
-                        residual->size(0) == m && residual->size(1) == n,
-                    "gemm_peak_fused: residual must be [m,n] of a's dtype on a's device");
-        res_p = residual->data_ptr();
+                        residual->size(0) == f.m && residual->size(1) == f.n,
+                    op, ": residual must be [m,n] of a's dtype on a's device");
+        f.residual = residual->data_ptr();
     }
-    const int dt = dtype_code(a, "gemm_peak_fused");
+    f.dtype = dtype_code(a, op);
+    return f;
+}
+
+// d[m,n] = row_scale[:,None] * (a[m,k] @ b[n,k]^T) + bias[None,:] + residual, each term optional.
+void gemm_peak_fused(Tensor &d, const Tensor &a, const Tensor &b, const OptTensor &row_scale, const OptTensor &bias,
+                     const OptTensor &residual, bool pdl) {
+    const FusedTerms f = check_fused_terms(d, a, b, row_scale, bias, residual, "gemm_peak_fused");
     c10::DeviceGuard device_guard(a.device());
     auto stream = at::cuda::getCurrentCUDAStream();
-    check_status(pg_hgemm_fused(d.data_ptr(), a.data_ptr(), b.data_ptr(), m, n, k, k, k, n, rs, bias_p, res_p, n, dt,
-                                pdl ? PG_FUSED_PDL : 0, stream.stream()),
+    check_status(pg_hgemm_fused(d.data_ptr(), a.data_ptr(), b.data_ptr(), f.m, f.n, f.k, f.k, f.k, f.n, f.row_scale,
+                                f.bias, f.residual, f.n, f.dtype, pdl ? PG_FUSED_PDL : 0, stream.stream()),
                  "gemm_peak_fused");
 }
 
-// ------------------------------------------- norms around a gated residual ----
+// The same with every row's adapter beside b: lora_a [L,r,k], lora_b [L,n,r], ids [m].
+void gemm_peak_lora(Tensor &d, const Tensor &a, const Tensor &b, const Tensor &lora_a, const Tensor &lora_b,
+                    const Tensor &ids, const OptTensor &scale, const OptTensor &row_scale, const OptTensor &bias,
+                    const OptTensor &residual) {
+    const char *op = "gemm_peak_lora";
+    const FusedTerms f = check_fused_terms(d, a, b, row_scale, bias, residual, op);
+    TORCH_CHECK(lora_a.dim() == 3 && lora_b.dim() == 3 && ids.dim() == 1, op, ": lora_a [L,r,k], lora_b [L,n,r], ids [m]");
+    const int64_t adapters = lora_a.size(0), rank = lora_a.size(1);
+    TORCH_CHECK(lora_a.size(2) == f.k && lora_b.size(0) == adapters && lora_b.size(1) == f.n && lora_b.size(2) == rank &&
+                    ids.size(0) == f.m,
+                op, ": the adapters' shapes do not match");
+    TORCH_CHECK(lora_a.device() == a.device() && lora_b.device() == a.device() && ids.device() == a.device(), op,
+                ": tensors must be on one CUDA device");
+    TORCH_CHECK(lora_a.is_contiguous() && lora_b.is_contiguous() && ids.is_contiguous(), op,
+                ": lora_a, lora_b and ids must be contiguous");
+    TORCH_CHECK(lora_a.scalar_type() == a.scalar_type() && lora_b.scalar_type() == a.scalar_type(), op,
+                ": lora_a and lora_b must have a's dtype");
+    TORCH_CHECK(ids.scalar_type() == at::kInt, op, ": ids must be int32");
+    if (scale)
+        TORCH_CHECK(scale->device() == a.device() && scale->is_contiguous() && scale->scalar_type() == at::kFloat &&
+                        scale->numel() == adapters,
+                    op, ": scale must be float32 [L] on a's device");
+    c10::DeviceGuard device_guard(a.device());
+    auto stream = at::cuda::getCurrentCUDAStream();
+    // scratch from torch's caching allocator, as for gemm_peak
+    const size_t ws_bytes = pg_hgemm_lora_workspace_bytes(f.m, f.n, f.k, adapters, rank);
+    Tensor ws = at::empty({static_cast<int64_t>(ws_bytes > 0 ? ws_bytes : 16)}, a.options().dtype(at::kByte));
+    check_status(pg_hgemm_lora(d.data_ptr(), a.data_ptr(), b.data_ptr(), f.m, f.n, f.k, f.k, f.k, f.n, lora_a.data_ptr(),
+                               lora_b.data_ptr(), ids.data_ptr<int32_t>(), adapters, rank,
+                               scale ? scale->data_ptr<float>() : nullptr, f.row_scale, f.bias, f.residual, f.n, f.dtype,
+                               ws.data_ptr(), ws_bytes, stream.stream()),
+                 op);
+}
 
-using OptTensor = std::optional<Tensor>;
+// ------------------------------------------- norms around a gated residual ----
 
 void *opt_ptr(const OptTensor &t) { return t ? t->data_ptr() : nullptr; }
 float *opt_f32(const OptTensor &t) { return t ? t->data_ptr<float>() : nullptr; }
@@ -310,6 +359,8 @@ TORCH_LIBRARY(PeakGemm, m) {
     m.def("rms_norm_rstd(Tensor(a!) rstd, Tensor x, float eps) -> ()");
     m.def("gemm_peak_fused(Tensor(a!) d, Tensor a, Tensor b, Tensor? row_scale, Tensor? bias, Tensor? residual, "
           "bool pdl=False) -> ()");
+    m.def("gemm_peak_lora(Tensor(a!) d, Tensor a, Tensor b, Tensor lora_a, Tensor lora_b, Tensor ids, Tensor? scale, "
+          "Tensor? row_scale, Tensor? bias, Tensor? residual) -> ()");
     m.def("rms_norm_residual_fwd(Tensor(a!) s, Tensor(b!)? y, Tensor u, Tensor residual, Tensor? gamma_post, Tensor? gate, "
           "Tensor? res_scale, Tensor? gamma_pre, float eps) -> ()");
     m.def("rms_norm_residual_bwd(Tensor(a!) du, Tensor(b!) dresidual, Tensor(c!)? dgamma_post, Tensor(d!)? dgate, "
@@ -323,6 +374,7 @@ TORCH_LIBRARY_IMPL(PeakGemm, CUDA, m) {
     m.impl("rms_norm_bwd_out", &rms_norm_bwd_out);
     m.impl("rms_norm_rstd", &rms_norm_rstd);
     m.impl("gemm_peak_fused", &gemm_peak_fused);
+    m.impl("gemm_peak_lora", &gemm_peak_lora);
     m.impl("rms_norm_residual_fwd", &rms_norm_residual_fwd);
     m.impl("rms_norm_residual_bwd", &rms_norm_residual_bwd);
 }
