@@ -28,6 +28,7 @@ int from_launch(int r, cudaError_t e) {
         case pg::kLaunchOk: return PG_OK;
         case pg::kLaunchCuda: return cuda_fail(e);
         case pg::kLaunchNotSm100: return PG_ERR_NOT_SM100;
+        case pg::kLaunchTooLarge: return PG_ERR_UNSUPPORTED;
         default: return PG_ERR_BAD_ARG;
     }
 }
@@ -216,7 +217,12 @@ int pg_hgemm_fused(void *d, const void *a, const void *b, int64_t m, int64_t n, 
 
 size_t pg_hgemm_lora_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank) {
     if (m <= 0 || n <= 0 || k <= 0 || adapters <= 0 || rank <= 0 || rank > kMaxRank || m > kMaxDim) return 0;
-    return pg::lora_workspace_bytes(m, n, k, adapters, rank);
+    size_t bytes = 0;
+    if (pg::lora_workspace_bytes(m, n, k, adapters, rank, &bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return bytes;
 }
 
 int pg_hgemm_lora(void *d, const void *a, const void *b, int64_t m, int64_t n, int64_t k, int64_t lda, int64_t ldb,
@@ -236,9 +242,12 @@ int pg_hgemm_lora(void *d, const void *a, const void *b, int64_t m, int64_t n, i
     if (!aligned16(lora_a) || !aligned16(lora_b) || ((reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(scale)) & 3u) ||
         (reinterpret_cast<uintptr_t>(workspace) & 255u))
         return PG_ERR_MISALIGNED;
-    if (workspace_bytes < pg::lora_workspace_bytes(m, n, k, adapters, rank)) return PG_ERR_WORKSPACE;
+    if (workspace_bytes < static_cast<size_t>(m) * rank * 2) return PG_ERR_WORKSPACE;     // too small on any device
+    size_t need = 0;
+    cudaError_t e = pg::lora_workspace_bytes(m, n, k, adapters, rank, &need);
+    if (e != cudaSuccess) return cuda_fail(e);
+    if (workspace_bytes < need) return PG_ERR_WORKSPACE;
     const pg::LoraArgs l{lora_a, lora_b, ids, scale, adapters, rank, workspace};
-    cudaError_t e = cudaSuccess;
     const int r = pg::hgemm_lora_launch(g, l, static_cast<cudaStream_t>(stream), &e);
     return from_launch(r, e);
 }

@@ -71,7 +71,9 @@
 #include <stdlib.h>
 
 #include "gemm_sm100.h"
+#include "gemm_common.cuh"
 #include "host_util.h"
+#include "lora_epilogue.cuh"
 #include "ptx.cuh"
 
 namespace pg {
@@ -80,10 +82,6 @@ using namespace ptx;
 
 namespace {
 
-constexpr uint32_t kBM = 128;           // rows of A per CTA
-constexpr uint32_t kBK = 64;            // k elements per stage = one 128-byte swizzle row
-constexpr uint32_t kUmmaK = 16;         // k elements per tcgen05.mma (16-bit inputs)
-constexpr uint32_t kThreads = 192;
 constexpr uint32_t kEpiWarps = 4;
 // The two-row-block kernel (MT == 2) runs 8 epilogue warps: two per tensor-memory lane quarter, each holding
 // 128 columns of one accumulator in registers, so that an accumulator is handed back after ONE round of loads.
@@ -93,15 +91,11 @@ constexpr uint32_t kStoreCols = 64;     // columns per TMA store box (128 bytes)
 constexpr uint32_t kStoreRows = 32;     // rows per TMA store box (one warp's lanes)
 constexpr uint32_t kStageBufBytes = kStoreRows * kStoreCols * 2;  // 4096
 #ifdef PG_TEST_SHORT_WAIT
-// Test build (libPeakGemm_device_waittest.so, never shipped as the product): waits give up after 2 ms, and a
-// switch in device memory makes ONE signal go missing, so that the give-up path itself can be exercised: the
-// waiting role records its code, the CTA drains, the kernel returns and the context stays usable.  The missing
+// Test build: a switch in device memory makes ONE signal go missing, so that the give-up path itself can be exercised:
+// the waiting role records its code, the CTA drains, the kernel returns and the context stays usable.  The missing
 // signal is chosen so that nothing is in flight when the roles drain: the MMAs have completed, only the
 // "accumulator ready" commit is withheld, so the epilogue warps are the ones that give up.
-constexpr uint64_t kWaitTimeoutNs = 2000000ull;
 __device__ int g_test_withhold_acc_commit;
-#else
-constexpr uint64_t kWaitTimeoutNs = 2000000000ull;                // 2 s
 #endif
 // Default switches.  ncu sweep at 8192^3 (pair kernel, band height 8): serpentine + A evict-last reads 943 MB
 // from DRAM against 1051 MB with no hints; an evict-first hint on B costs +60 %.
@@ -122,15 +116,6 @@ enum : uint32_t {
     // last tiles of the one before.  Behind any other kernel the wait returns when that kernel has completed: the
     // ordinary stream order.
     kFlagPdl = 128u,
-};
-
-// Codes written to the device status word (role that gave up).
-enum : int {
-    kStProducerEmpty = 1,
-    kStMmaFull = 2,
-    kStMmaAccEmpty = 3,
-    kStEpiAccFull = 4,
-    kStEpiTailFlag = 5,
 };
 
 template <int CTA_GROUP, int BN, int STAGES, int MT = 1>
@@ -154,16 +139,12 @@ struct Cfg {
     // full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], then tmem slot + abort flag
     static constexpr uint32_t kNumBars = 2 * STAGES + 4;
     static constexpr uint32_t kOffMisc = kOffBar + kNumBars * 8;
-    static constexpr uint32_t kSmemBytes = kOffMisc + 16 + 1024;  // + slack to align the base to 1024
+    static constexpr uint32_t kOffInfo = kOffMisc + 16;           // LORA: what each stage holds
+    static constexpr uint32_t kSmemBytes = kOffInfo + STAGES * 4 + 1024;  // + slack to align the base to 1024
     static_assert(kTmemCols == 128 || kTmemCols == 256 || kTmemCols == 512, "tmem columns: power of 2");
     static_assert(kSmemBytes <= 232448, "exceeds 227 KiB of shared memory");
     static_assert(BN % kStoreCols == 0, "BN must be a multiple of the store box");
     static_assert((BN / CTA_GROUP) % 8 == 0 && BN % 16 == 0 && BN <= 256, "invalid MMA N");
-};
-
-struct WaitCtx {
-    volatile uint32_t *abort_flag;  // shared memory
-    int *status;                    // global memory
 };
 
 // Destinations of the output tile: the epilogue stores every 32 x 64 box to each of them from the
@@ -250,28 +231,6 @@ __device__ __forceinline__ float epi_row_scale(const EpiArgs &epi, bool row_ok, 
     if (!epi.row_scale) return 1.f;
     if (epi.pdl_wait) asm volatile("griddepcontrol.wait;" ::: "memory");
     return row_ok ? *(epi.row_scale + row) : 1.f;
-}
-
-// Bounded mbarrier wait.  Returns false if the wait was abandoned.  The clock is
-// only consulted every 1024 failed probes (each probe already suspends the thread
-// for a hardware-defined interval), so the common short wait costs nothing extra.
-__device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const WaitCtx &ctx, int code) {
-    if (mbar_try_wait(bar, parity)) return true;
-    uint64_t t0 = 0;
-    uint32_t spins = 0;
-    while (true) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((++spins & 1023u) == 0) {
-            if (*ctx.abort_flag) return false;
-            const uint64_t now = globaltimer_ns();
-            if (t0 == 0) t0 = now;
-            else if (now - t0 > kWaitTimeoutNs) {
-                *ctx.abort_flag = 1;
-                if (ctx.status) atomicCAS(ctx.status, 0, code);
-                return false;
-            }
-        }
-    }
 }
 
 // Grouped raster: tile t -> (mi, ni).  Tiles are numbered down the rows of a band
@@ -409,13 +368,13 @@ __device__ __forceinline__ bool wait_count_patiently(const uint32_t *counter, ui
     return true;
 }
 
-template <int CTA_GROUP, int BN, int STAGES, int MT, bool BF16>
+template <int CTA_GROUP, int BN, int STAGES, int MT, bool BF16, bool LORA>
 __global__ void __launch_bounds__(MT == 2 ? kThreadsWide : kThreads, 1)
 hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                      const __grid_constant__ CUtensorMap tm_b,
                      const __grid_constant__ DstMaps tm_c, uint32_t n_dst,
                      uint32_t M, uint32_t N, uint32_t K, uint32_t group_m, uint32_t flags, const EpiArgs epi,
-                     const TailArgs tail, int *status) {
+                     const TailArgs tail, int *status, const __grid_constant__ LoraParam<LORA> lora) {
     using C = Cfg<CTA_GROUP, BN, STAGES, MT>;
     constexpr uint32_t kBlockM = kBM * CTA_GROUP;         // rows one MMA covers
     constexpr uint32_t kTileM = kBlockM * MT;
@@ -437,6 +396,7 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
     const uint32_t tmem_slot = smem_base + C::kOffMisc;
     volatile uint32_t *tmem_slot_gen = reinterpret_cast<volatile uint32_t *>(smem_gen + C::kOffMisc);
     volatile uint32_t *abort_flag = tmem_slot_gen + 1;
+    volatile uint32_t *stage_info = reinterpret_cast<volatile uint32_t *>(smem_gen + C::kOffInfo);
     const WaitCtx ctx{abort_flag, status};
 
     const uint32_t m_tiles = (M + kTileM - 1) / kTileM;
@@ -462,6 +422,10 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
         prefetch_tensormap(&tm_a);
         prefetch_tensormap(&tm_b);
         for (uint32_t d = 0; d < n_dst; ++d) prefetch_tensormap(&tm_c.m[d]);
+        if constexpr (LORA) {
+            prefetch_tensormap(&lora.tm_v);
+            prefetch_tensormap(&lora.tm_b);
+        }
     }
     if (warp == 1) {
         tmem_alloc<CTA_GROUP>(tmem_slot, C::kTmemCols);
@@ -499,8 +463,18 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                 tile_coords(group_m, u.tile, m_tiles, n_tiles, mi, ni, (flags & kFlagSerpentine) != 0);
                 const int32_t row_a = static_cast<int32_t>(mi * kTileM + rank * kBM);    // + mt * kBlockM
                 const int32_t row_b = static_cast<int32_t>(ni * BN + rank * C::kBRows);
-                for (uint32_t kb = u.kb0; kb < u.kb1; ++kb) {
-                    if (tail.wave_sync != nullptr && leader) {
+                LoraBlocks extra;                    // the adapters' k-blocks behind the product's own
+                for (uint32_t kb = u.kb0; kb < u.kb1 + extra.count; ++kb) {
+                    const bool own = !LORA || kb < u.kb1;
+                    if constexpr (LORA) {
+                        // The last block of the product has to know whether the tile ends with it: from here on the
+                        // down projections must be there.
+                        if (kb + 1 == u.kb1) {
+                            if (it == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+                            extra.open(lora.d, mi);
+                        }
+                    }
+                    if (own && tail.wave_sync != nullptr && leader) {
                         // Synchronisation points of the producers (the first k-block of every tile and every
                         // sync_kb-th after it): a worker announces that it has reached the point, and sync_lag
                         // k-blocks later waits until every worker of this wave of tiles has.  Workers that share an
@@ -521,6 +495,7 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                         // wait until the MMAs that read this stage have completed
                         ok = wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty);
                         if (!ok) break;
+                        if constexpr (LORA) stage_info[stage] = extra.info(lora.d, kb, u.kb1);
                         if constexpr (CTA_GROUP == 2) {
                             mbar_arrive_cluster(peer_empty0 + stage * 8);   // relay to the peer
                             mbar_arrive_expect_tx(bar_full + stage * 8, 2 * C::kStageBytes);
@@ -535,6 +510,22 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     const uint32_t dst_b = smem_base + C::kOffB + stage * C::kBBytes;
                     const int32_t kx = static_cast<int32_t>(kb * kBK);
                     const uint32_t fb = (CTA_GROUP == 2) ? full0 + stage * 8 : bar_full + stage * 8;
+                    if constexpr (LORA) {
+                        if (!own) {
+                            const int32_t rx = extra.next(lora.d);
+#pragma unroll
+                            for (uint32_t mt = 0; mt < MT; ++mt) {
+                                const uint32_t da = dst_a + mt * C::kABox;
+                                const int32_t rv = extra.v_row + static_cast<int32_t>(mt * kBlockM + rank * kBM);
+                                if constexpr (CTA_GROUP == 2) tma_load_2d_pair(da, &lora.tm_v, fb, rx, rv);
+                                else tma_load_2d(da, &lora.tm_v, fb, rx, rv);
+                            }
+                            if constexpr (CTA_GROUP == 2) tma_load_2d_pair(dst_b, &lora.tm_b, fb, rx, extra.b_row + row_b);
+                            else tma_load_2d(dst_b, &lora.tm_b, fb, rx, extra.b_row + row_b);
+                            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                            continue;
+                        }
+                    }
 #pragma unroll
                     for (uint32_t mt = 0; mt < MT; ++mt) {
                         const uint32_t da = dst_a + mt * C::kABox;
@@ -574,10 +565,17 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     if (!ok) break;
                     tc_fence_after_sync();
                 }
-                for (uint32_t kb = u.kb0; kb < u.kb1; ++kb) {
+                bool last = false;
+                for (uint32_t kb = u.kb0; LORA ? !last : kb < u.kb1; ++kb) {
                     ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                     if (!ok) break;
                     tc_fence_after_sync();
+                    uint32_t steps = kBK / kUmmaK;
+                    if constexpr (LORA) {
+                        const uint32_t info = stage_info[stage];
+                        steps = info & 7u;
+                        last = (info & kLoraLast) != 0;
+                    }
                     const uint64_t db = smem_desc_k_sw128(smem_base + C::kOffB + stage * C::kBBytes);
 #pragma unroll
                     for (uint32_t mt = 0; mt < MT; ++mt) {
@@ -595,6 +593,7 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
 #pragma unroll
                         for (uint32_t k = 0; k < kBK / kUmmaK; ++k) {
                             // 16 elements of k = 32 bytes inside the 128-byte swizzle row = +2 in the >>4 address field
+                            if (LORA && k >= steps) break;
                             umma_f16<CTA_GROUP>(tmem_d, da + 2 * k, db + 2 * k, idesc,
                                                 (kb != u.kb0 || k != 0u) ? 1u : 0u);
                         }
@@ -621,7 +620,7 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
         }
         __syncwarp();
     } else {
-        if (pdl) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (pdl || LORA) asm volatile("griddepcontrol.wait;" ::: "memory");
         if constexpr (MT == 2) {
             // ===== epilogue, two row blocks per CTA: 8 warps =====
             // Warp w reads lane quarter w % 4 (the hardware rule) and column half (w - 2) / 4 of each accumulator:
@@ -666,6 +665,11 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     if (lane == 0) mbar_arrive_cluster(acc_empty_leader + mt * 8);
                     const bool row_ok = row0 + lane < M;
                     const float rs = fused ? epi_row_scale(epi, row_ok, row0 + lane) : 1.f;
+                    if constexpr (LORA) {
+#pragma unroll
+                        for (uint32_t cb = 0; cb < 4; ++cb)
+                            lora_repair<BF16>(v[cb], lora.d, mi, row0 + lane, ni * BN + half * 128u + cb * 32u, M);
+                    }
                     if (wide_boxes) {
                         // Stores that cross NVLink (peer destinations, or a multicast one): two 32 x 64 boxes with
                         // 128-byte rows over the warp's whole staging area, one at a time.  Half as many, twice as
@@ -860,6 +864,11 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                             d[3] = __float_as_uint(__uint_as_float(d[3]) + p.w);
                         }
                     }
+                    if constexpr (LORA) {
+#pragma unroll
+                        for (uint32_t cb = 0; cb < 2; ++cb)
+                            lora_repair<BF16>(v[cb], lora.d, mi, row0 + lane, ni * BN + ch * kStoreCols + cb * 32u, M);
+                    }
                     // the store issued two chunks ago from this buffer must have finished reading it
                     if (lane == 0) bulk_wait_group_read<1>();
                     __syncwarp();
@@ -970,15 +979,17 @@ struct SkCfg {
     static constexpr uint32_t kOffBar = kOffRecv + kBM * BN * 4;       // full[STAGES], empty[STAGES], acc_full
     static constexpr uint32_t kNumBars = 2 * STAGES + 1;
     static constexpr uint32_t kOffMisc = kOffBar + kNumBars * 8;
-    static constexpr uint32_t kSmemBytes = kOffMisc + 16 + 1024;
+    static constexpr uint32_t kOffInfo = kOffMisc + 16;                // LORA: what each stage holds
+    static constexpr uint32_t kSmemBytes = kOffInfo + STAGES * 4 + 1024;
     static_assert(kTmemCols == 32 || kTmemCols == 64 || kTmemCols == 128 || kTmemCols == 256, "tmem columns");
     static_assert(kSmemBytes <= 232448, "exceeds 227 KiB of shared memory");
 };
 
-template <int BN, int STAGES, bool BF16>
+template <int BN, int STAGES, bool BF16, bool LORA>
 __global__ void __launch_bounds__(kThreads, 1)
 hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
-                    uint16_t *c, uint32_t ldc, uint32_t M, uint32_t N, uint32_t K, const EpiArgs epi, int *status) {
+                    uint16_t *c, uint32_t ldc, uint32_t M, uint32_t N, uint32_t K, const EpiArgs epi, int *status,
+                    const __grid_constant__ LoraParam<LORA> lora) {
     using C = SkCfg<BN, STAGES>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -996,6 +1007,7 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
     const uint32_t tmem_slot = smem_base + C::kOffMisc;
     volatile uint32_t *tmem_slot_gen = reinterpret_cast<volatile uint32_t *>(smem_gen + C::kOffMisc);
     volatile uint32_t *abort_flag = tmem_slot_gen + 1;
+    volatile uint32_t *stage_info = reinterpret_cast<volatile uint32_t *>(smem_gen + C::kOffInfo);
     const WaitCtx ctx{abort_flag, status};
 
     const uint32_t m_tiles = (M + kBM - 1) / kBM;
@@ -1016,6 +1028,10 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
         fence_mbar_init();
         prefetch_tensormap(&tm_a);
         prefetch_tensormap(&tm_b);
+        if constexpr (LORA) {
+            prefetch_tensormap(&lora.tm_v);
+            prefetch_tensormap(&lora.tm_b);
+        }
     }
     if (warp == 1) {
         tmem_alloc<1>(tmem_slot, C::kTmemCols);
@@ -1035,9 +1051,28 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             uint32_t stage = 0, phase = 0;
             // the weights pass through once (evict first); the activations are what every CTA re-reads (evict last)
             const uint64_t pol_stream = l2_policy_evict_first(), pol_keep = l2_policy_evict_last();
-            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+            LoraBlocks extra;   // this CTA's share of the adapters' k-blocks (CTAs without a k-slice get none)
+            for (uint32_t kb = kb0; kb < kb1 + extra.count; ++kb) {
+                if constexpr (LORA) {
+                    if (kb + 1 == kb1) {
+                        asm volatile("griddepcontrol.wait;" ::: "memory");
+                        extra.open(lora.d, mi, rank, (k_blocks + per - 1) / per);
+                    }
+                }
                 if (!wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty)) break;
+                if constexpr (LORA) stage_info[stage] = extra.info(lora.d, kb, kb1);
                 mbar_arrive_expect_tx(bar_full + stage * 8, C::kStageBytes);
+                if constexpr (LORA) {
+                    if (kb >= kb1) {
+                        const int32_t rx = extra.next(lora.d);
+                        tma_load_2d(smem_base + C::kOffA + stage * C::kABytes, &lora.tm_v, bar_full + stage * 8, rx,
+                                    extra.v_row);
+                        tma_load_2d(smem_base + C::kOffB + stage * C::kBBytes, &lora.tm_b, bar_full + stage * 8, rx,
+                                    extra.b_row + static_cast<int32_t>(ni * BN));
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                        continue;
+                    }
+                }
                 const int32_t kx = static_cast<int32_t>(kb * kBK);
                 tma_load_2d_hint(smem_base + C::kOffA + stage * C::kABytes, &tm_a, bar_full + stage * 8, kx,
                                  static_cast<int32_t>(mi * kBM), pol_keep);
@@ -1052,15 +1087,24 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             constexpr uint32_t idesc = instr_desc_f16(BF16, kBM, BN);
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+            bool last = false;
+            for (uint32_t kb = kb0; LORA ? !last : kb < kb1; ++kb) {
                 ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                 if (!ok) break;
                 tc_fence_after_sync();
+                uint32_t steps = kBK / kUmmaK;
+                if constexpr (LORA) {
+                    const uint32_t info = stage_info[stage];
+                    steps = info & 7u;
+                    last = (info & kLoraLast) != 0;
+                }
                 const uint64_t da = smem_desc_k_sw128(smem_base + C::kOffA + stage * C::kABytes);
                 const uint64_t db = smem_desc_k_sw128(smem_base + C::kOffB + stage * C::kBBytes);
 #pragma unroll
-                for (uint32_t k = 0; k < kBK / kUmmaK; ++k)
+                for (uint32_t k = 0; k < kBK / kUmmaK; ++k) {
+                    if (LORA && k >= steps) break;
                     umma_f16<1>(tmem_base, da + 2 * k, db + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                }
                 umma_commit<1>(bar_empty + stage * 8);
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
@@ -1110,7 +1154,7 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
 
     if (warp >= 2) {
         // ===== reduce my W columns and store them =====
-        if (epi.pdl_all) asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (epi.pdl_all || LORA) asm volatile("griddepcontrol.wait;" ::: "memory");
         const uint32_t q = warp & 3u;
         const uint32_t row = q * 32u + lane;
         const uint32_t grow = mi * kBM + row;
@@ -1152,6 +1196,7 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     }
                     const uint32_t gcol = ni * BN + rank * W + 8u * g;
                     if (grow < M && gcol < N) {
+                        if constexpr (LORA) lora_repair<BF16, 8>(f, lora.d, mi, grow, gcol, M);
                         if (fused) epi_apply8<BF16>(f, rs, epi, true, grow, gcol);
                         uint4 out;
                         out.x = pack2<BF16>(f[0], f[1]);
@@ -1462,7 +1507,8 @@ struct SnCfg {
     static constexpr uint32_t kOffBar = kOffT + STAGES * kTBytes;
     static constexpr uint32_t kNumBars = 2 * STAGES + 1;
     static constexpr uint32_t kOffMisc = kOffBar + kNumBars * 8;
-    static constexpr uint32_t kOffRecv = (kOffMisc + 16 + 15) & ~15u;   // [TOK/4][S slots x 128/S rows][4] fp32, S > 1 only
+    static constexpr uint32_t kOffInfo = kOffMisc + 16;                 // LORA: what each stage holds
+    static constexpr uint32_t kOffRecv = (kOffInfo + STAGES * 4 + 15) & ~15u;   // [TOK/4][S slots x 128/S rows][4] fp32, S > 1 only
     static constexpr uint32_t kRecvBytes = kBM * TOK * 4;
     static constexpr uint32_t kSmemNoRecv = kOffRecv + 1024;
     static constexpr uint32_t kSmemBytes = kSmemNoRecv + kRecvBytes;
@@ -1471,10 +1517,11 @@ struct SnCfg {
     static_assert(TOK == 16 || TOK == 32 || TOK == 64, "token tile");
 };
 
-template <int TOK, int STAGES, bool BF16>
+template <int TOK, int STAGES, bool BF16, bool LORA>
 __global__ void __launch_bounds__(kThreads, 1)
 hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_constant__ CUtensorMap tm_w,
-                    uint16_t *c, uint32_t ldc, uint32_t M, uint32_t N, uint32_t K, const EpiArgs epi, int *status) {
+                    uint16_t *c, uint32_t ldc, uint32_t M, uint32_t N, uint32_t K, const EpiArgs epi, int *status,
+                    const __grid_constant__ LoraParam<LORA> lora) {
     using C = SnCfg<TOK, STAGES>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -1492,6 +1539,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
     const uint32_t tmem_slot = smem_base + C::kOffMisc;
     volatile uint32_t *tmem_slot_gen = reinterpret_cast<volatile uint32_t *>(smem_gen + C::kOffMisc);
     volatile uint32_t *abort_flag = tmem_slot_gen + 1;
+    volatile uint32_t *stage_info = reinterpret_cast<volatile uint32_t *>(smem_gen + C::kOffInfo);
     const WaitCtx ctx{abort_flag, status};
 
     const uint32_t ni = blockIdx.x / S;               // which 128 weight rows
@@ -1510,6 +1558,10 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
         fence_mbar_init();
         prefetch_tensormap(&tm_tok);
         prefetch_tensormap(&tm_w);
+        if constexpr (LORA) {
+            prefetch_tensormap(&lora.tm_v);
+            prefetch_tensormap(&lora.tm_b);
+        }
     }
     if (warp == 1) {
         tmem_alloc<1>(tmem_slot, C::kTmemCols);
@@ -1531,9 +1583,28 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
             uint32_t stage = 0, phase = 0;
             // the weights pass through once (evict first); the activations are what every CTA re-reads (evict last)
             const uint64_t pol_stream = l2_policy_evict_first(), pol_keep = l2_policy_evict_last();
-            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+            LoraBlocks extra;   // this CTA's share of the adapters' k-blocks (CTAs without a k-slice get none)
+            for (uint32_t kb = kb0; kb < kb1 + extra.count; ++kb) {
+                if constexpr (LORA) {
+                    if (kb + 1 == kb1) {
+                        asm volatile("griddepcontrol.wait;" ::: "memory");
+                        extra.open(lora.d, 0, rank, (k_blocks + per - 1) / per);
+                    }
+                }
                 if (!wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty)) break;
+                if constexpr (LORA) stage_info[stage] = extra.info(lora.d, kb, kb1);
                 mbar_arrive_expect_tx(bar_full + stage * 8, C::kStageBytes);
+                if constexpr (LORA) {
+                    if (kb >= kb1) {
+                        const int32_t rx = extra.next(lora.d);
+                        tma_load_2d(smem_base + C::kOffW + stage * C::kWBytes, &lora.tm_b, bar_full + stage * 8, rx,
+                                    extra.b_row + static_cast<int32_t>(ni * kBM));
+                        tma_load_2d(smem_base + C::kOffT + stage * C::kTBytes, &lora.tm_v, bar_full + stage * 8, rx,
+                                    extra.v_row);
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                        continue;
+                    }
+                }
                 const int32_t kx = static_cast<int32_t>(kb * kBK);
                 tma_load_2d_hint(smem_base + C::kOffW + stage * C::kWBytes, &tm_w, bar_full + stage * 8, kx,
                                  static_cast<int32_t>(ni * kBM), pol_stream);
@@ -1548,15 +1619,24 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
             constexpr uint32_t idesc = instr_desc_f16(BF16, kBM, TOK);
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            for (uint32_t kb = kb0; kb < kb1; ++kb) {
+            bool last = false;
+            for (uint32_t kb = kb0; LORA ? !last : kb < kb1; ++kb) {
                 ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                 if (!ok) break;
                 tc_fence_after_sync();
+                uint32_t steps = kBK / kUmmaK;
+                if constexpr (LORA) {
+                    const uint32_t info = stage_info[stage];
+                    steps = info & 7u;
+                    last = (info & kLoraLast) != 0;
+                }
                 const uint64_t dw = smem_desc_k_sw128(smem_base + C::kOffW + stage * C::kWBytes);
                 const uint64_t dt = smem_desc_k_sw128(smem_base + C::kOffT + stage * C::kTBytes);
 #pragma unroll
-                for (uint32_t k = 0; k < kBK / kUmmaK; ++k)
+                for (uint32_t k = 0; k < kBK / kUmmaK; ++k) {
+                    if (LORA && k >= steps) break;
                     umma_f16<1>(tmem_base, dw + 2 * k, dt + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                }
                 umma_commit<1>(bar_empty + stage * 8);
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
@@ -1604,7 +1684,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
             cluster_wait();
         }
         if (owner == rank) {
-            if (epi.pdl_all) asm volatile("griddepcontrol.wait;" ::: "memory");
+            if (epi.pdl_all || LORA) asm volatile("griddepcontrol.wait;" ::: "memory");
             const float *recv = reinterpret_cast<const float *>(smem_gen + C::kOffRecv);
             for (uint32_t r2 = 0; r2 < S; ++r2) {
                 if (r2 == rank) continue;
@@ -1618,6 +1698,16 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
             // C[mi, n] = D[n, mi]: for each token the 32 lanes of a warp write 32 consecutive columns of C
             const uint32_t n_glob = ni * kBM + row;
             if (n_glob < N) {
+                if constexpr (LORA) {
+                    bool bad = false;
+#pragma unroll
+                    for (uint32_t mi = 0; mi < TOK; ++mi) bad |= mi < M && f[mi] != f[mi];
+                    if (bad) {
+#pragma unroll
+                        for (uint32_t mi = 0; mi < TOK; ++mi)
+                            if (mi < M && f[mi] != f[mi]) f[mi] = lora_exact<BF16>(lora.d, 0, mi, n_glob, f[mi]);
+                    }
+                }
                 if (epi.any()) {
                     // thread = one column of C: its bias once, then per token the row scale (one address for the
                     // whole warp) and the residual element (32 consecutive columns per warp)
@@ -1795,16 +1885,30 @@ bool pdl_enabled() {
 }
 
 EpiArgs make_epi(const GemmArgs &g) {
-    EpiArgs e;
+    EpiArgs e = {};
     e.row_scale = g.row_scale;
     e.bias = static_cast<const uint16_t *>(g.bias);
     e.residual = static_cast<const uint16_t *>(g.residual);
     e.ldr = static_cast<uint32_t>(g.ldr);
     e.pdl_wait = (g.pdl_wait && g.row_scale) ? 1u : 0u;
-    e.pdl_all = (!e.pdl_wait && pdl_enabled()) ? 1u : 0u;
+    e.pdl_all = (!e.pdl_wait && !g.lora && pdl_enabled()) ? 1u : 0u;
     e.mc_dst = static_cast<uint16_t *>(g.mc_dst);
     e.ld_mc = static_cast<uint32_t>(g.ldc);
     return e;
+}
+
+// The kernels' adapter argument: tensor maps of V (box of v_rows rows) and of the up projections (box of b_rows rows).
+bool fill_lora(LoraParam<false> *, const GemmArgs &, uint32_t, uint32_t) { return true; }
+bool fill_lora(LoraParam<true> *p, const GemmArgs &g, uint32_t v_rows, uint32_t b_rows) {
+    const LoraGemm &l = *g.lora;
+    const int64_t groups = (g.m + l.group_rows - 1) / l.group_rows;
+    p->d = {l.ids, l.table, static_cast<const uint16_t *>(l.v), static_cast<const uint16_t *>(l.b),
+            static_cast<const uint16_t *>(g.a), static_cast<const uint16_t *>(g.b), g.lda, g.ldb,
+            static_cast<uint32_t>(g.k), static_cast<uint32_t>(g.n), static_cast<uint32_t>(l.rank),
+            static_cast<uint32_t>((l.rank + kBK - 1) / kBK), static_cast<uint32_t>(l.max_slots),
+            static_cast<uint32_t>(l.group_rows), static_cast<uint32_t>(l.table_stride)};
+    return make_tmap(&p->tm_v, l.v, groups * l.max_slots * l.group_rows, l.rank, l.rank, v_rows, g.bf16, false) &&
+           make_tmap(&p->tm_b, l.b, l.adapters * g.n, l.rank, l.rank, b_rows, g.bf16, false);
 }
 
 // Launch attributes common to the three kernels: the cluster shape, and for a caller that chained this
@@ -1867,10 +1971,10 @@ void plan_tail(int64_t m, int64_t n, int64_t k, int workers, uint32_t *full_tile
 
 namespace {
 
-template <int CTA_GROUP, int BN, int STAGES, int MT, bool BF16>
+template <int CTA_GROUP, int BN, int STAGES, int MT, bool BF16, bool LORA = false>
 cudaError_t launch(const GemmArgs &g, const DeviceInfo &d, int sms, cudaStream_t stream) {
     using C = Cfg<CTA_GROUP, BN, STAGES, MT>;
-    auto kernel = hgemm_tcgen05_kernel<CTA_GROUP, BN, STAGES, MT, BF16>;
+    auto kernel = hgemm_tcgen05_kernel<CTA_GROUP, BN, STAGES, MT, BF16, LORA>;
     static DeviceOnce smem_once;
     {
         const cudaError_t e = allow_dynamic_smem(smem_once, kernel, C::kSmemBytes);
@@ -1888,6 +1992,8 @@ cudaError_t launch(const GemmArgs &g, const DeviceInfo &d, int sms, cudaStream_t
         if (!make_tmap(&tm_c.m[1 + i], g.extra_dst[i], g.m, g.n, g.ldc, kStoreRows, BF16, true, store_box_cols))
             return cudaErrorInvalidValue;
     const uint32_t n_dst = 1u + static_cast<uint32_t>(g.n_extra_dst);
+    LoraParam<LORA> lora;
+    if (!fill_lora(&lora, g, kBM, C::kBRows)) return cudaErrorInvalidValue;
 
     const uint32_t tile_m = kBM * CTA_GROUP * MT;
     const uint64_t m_tiles = (g.m + tile_m - 1) / tile_m;
@@ -1958,7 +2064,7 @@ cudaError_t launch(const GemmArgs &g, const DeviceInfo &d, int sms, cudaStream_t
         ++cfg.numAttrs;
         const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tm_a, tm_b, tm_c, n_dst, static_cast<uint32_t>(g.m),
                                                  static_cast<uint32_t>(g.n), static_cast<uint32_t>(g.k), group_m,
-                                                 flags, make_epi(g), tail, d.status_word);
+                                                 flags, make_epi(g), tail, d.status_word, lora);
         if (e == cudaSuccess) return e;
         cudaGetLastError();
         cfg.numAttrs = fill_attrs(attr, CTA_GROUP, g);
@@ -1967,16 +2073,17 @@ cudaError_t launch(const GemmArgs &g, const DeviceInfo &d, int sms, cudaStream_t
     // An ordinary (not cooperative) launch goes out under programmatic stream serialisation, see kFlagPdl.  Not
     // when the caller chained this GEMM behind the kernel that produces row_scale: that mode has its own, later wait.
     uint32_t launch_flags = flags;
-    if (pdl_enabled() && !(g.pdl_wait && g.row_scale)) launch_flags |= kFlagPdl;    // fill_attrs set the attribute
+    // Nor with adapters: there the previous launch is the down projection, and only what reads its result waits.
+    if (pdl_enabled() && !(g.pdl_wait && g.row_scale) && !LORA) launch_flags |= kFlagPdl;    // fill_attrs set the attribute
     return cudaLaunchKernelEx(&cfg, kernel, tm_a, tm_b, tm_c, n_dst, static_cast<uint32_t>(g.m),
                               static_cast<uint32_t>(g.n), static_cast<uint32_t>(g.k), group_m, launch_flags,
-                              make_epi(g), tail, d.status_word);
+                              make_epi(g), tail, d.status_word, lora);
 }
 
-template <int BN, int STAGES, bool BF16>
+template <int BN, int STAGES, bool BF16, bool LORA = false>
 cudaError_t launch_splitk(const GemmArgs &g, const DeviceInfo &d, int split, cudaStream_t stream) {
     using C = SkCfg<BN, STAGES>;
-    auto kernel = hgemm_splitk_kernel<BN, STAGES, BF16>;
+    auto kernel = hgemm_splitk_kernel<BN, STAGES, BF16, LORA>;
     static DeviceOnce smem_once;
     {
         const cudaError_t e = allow_dynamic_smem(smem_once, kernel, C::kSmemBytes);
@@ -1986,6 +2093,8 @@ cudaError_t launch_splitk(const GemmArgs &g, const DeviceInfo &d, int split, cud
     if (!make_tmap(&tm_a, g.a, g.m, g.k, g.lda, kBM, BF16, false) ||
         !make_tmap(&tm_b, g.b, g.n, g.k, g.ldb, BN, BF16, false))
         return cudaErrorInvalidValue;
+    LoraParam<LORA> lora;
+    if (!fill_lora(&lora, g, kBM, BN)) return cudaErrorInvalidValue;
     const uint64_t tiles = ((g.m + kBM - 1) / kBM) * ((g.n + BN - 1) / BN);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(tiles * split), 1, 1);
@@ -1998,7 +2107,7 @@ cudaError_t launch_splitk(const GemmArgs &g, const DeviceInfo &d, int split, cud
     (void)d;
     return cudaLaunchKernelEx(&cfg, kernel, tm_a, tm_b, static_cast<uint16_t *>(g.c), static_cast<uint32_t>(g.ldc),
                               static_cast<uint32_t>(g.m), static_cast<uint32_t>(g.n), static_cast<uint32_t>(g.k),
-                              make_epi(g), d.status_word);
+                              make_epi(g), d.status_word, lora);
 }
 
 template <int ROWS, int BN, int STAGES, bool BF16>
@@ -2070,10 +2179,10 @@ cudaError_t launch_pair_splitk_any(const GemmArgs &g, const DeviceInfo &d, int b
                   : launch_pair_splitk<ROWS, 128, kStages128, false>(g, d, pairs, stream);
 }
 
-template <int TOK, int STAGES, bool BF16>
+template <int TOK, int STAGES, bool BF16, bool LORA>
 cudaError_t launch_skinny(const GemmArgs &g, const DeviceInfo &d, int split, cudaStream_t stream) {
     using C = SnCfg<TOK, STAGES>;
-    auto kernel = hgemm_skinny_kernel<TOK, STAGES, BF16>;
+    auto kernel = hgemm_skinny_kernel<TOK, STAGES, BF16, LORA>;
     static DeviceOnce smem_once;
     {
         const cudaError_t e = allow_dynamic_smem(smem_once, kernel, C::kSmemBytes);
@@ -2083,6 +2192,8 @@ cudaError_t launch_skinny(const GemmArgs &g, const DeviceInfo &d, int split, cud
     if (!make_tmap(&tm_tok, g.a, g.m, g.k, g.lda, TOK, BF16, false) ||
         !make_tmap(&tm_w, g.b, g.n, g.k, g.ldb, kBM, BF16, false))
         return cudaErrorInvalidValue;
+    LoraParam<LORA> lora;
+    if (!fill_lora(&lora, g, TOK, kBM)) return cudaErrorInvalidValue;
     const uint64_t tiles = (g.n + kBM - 1) / kBM;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(tiles * split), 1, 1);
@@ -2094,7 +2205,7 @@ cudaError_t launch_skinny(const GemmArgs &g, const DeviceInfo &d, int split, cud
     cfg.numAttrs = fill_attrs(attr, static_cast<unsigned>(split), g);
     return cudaLaunchKernelEx(&cfg, kernel, tm_tok, tm_w, static_cast<uint16_t *>(g.c), static_cast<uint32_t>(g.ldc),
                               static_cast<uint32_t>(g.m), static_cast<uint32_t>(g.n), static_cast<uint32_t>(g.k),
-                              make_epi(g), d.status_word);
+                              make_epi(g), d.status_word, lora);
 }
 
 // Cluster size for the skinny kernel: the largest S in {1,2,4,8} that keeps tiles * S within ~1.1 waves
@@ -2118,7 +2229,7 @@ int choose_skinny_split(const GemmArgs &g, int slots) {
 // 24 KiB (184.2 -> 198.4).  17-32 tokens with one wave of tiles that one CTA per SM leaves unsplit (82-162 tiles):
 // two per SM with 4 x 20 KiB and k split in two, 32 x 14336 x 4096 24.0 -> 22.9 (23.4), 32 x 11008 x 4096
 // 22.1 -> 19.5 (20.5), 32 x 14336 x 8192 40.6 -> 41.3 (39.4).
-template <bool BF16>
+template <bool BF16, bool LORA = false>
 cudaError_t launch_skinny_any(const GemmArgs &g, const DeviceInfo &d, int sms, int forced_split, cudaStream_t stream) {
     const int64_t tiles = (g.n + 127) / 128;
     const bool two = g.m <= 16 || (g.m <= 32 && tiles > sms);
@@ -2129,17 +2240,17 @@ cudaError_t launch_skinny_any(const GemmArgs &g, const DeviceInfo &d, int sms, i
     static const bool env_two32 = tune_env_int("PEAKGEMM_TUNE_SKINNY_TWO32", 1) != 0;
     if (env_two32 && forced_split <= 0 && !two && g.m > 16 && g.m <= 32 && sp == 1 && tiles * 20 <= sms * 22 &&
         (g.k + 63) / 64 >= 8)
-        return launch_skinny<32, 4, BF16>(g, d, 2, stream);
-    if (g.m <= 16) return sp == 1 ? launch_skinny<16, 6, BF16>(g, d, sp, stream) : launch_skinny<16, 5, BF16>(g, d, sp, stream);
-    if (g.m <= 32) return two && sp == 1 ? launch_skinny<32, 5, BF16>(g, d, sp, stream)
-                                         : launch_skinny<32, 10, BF16>(g, d, sp, stream);
-    return launch_skinny<64, 8, BF16>(g, d, sp, stream);
+        return launch_skinny<32, 4, BF16, LORA>(g, d, 2, stream);
+    if (g.m <= 16) return sp == 1 ? launch_skinny<16, 6, BF16, LORA>(g, d, sp, stream) : launch_skinny<16, 5, BF16, LORA>(g, d, sp, stream);
+    if (g.m <= 32) return two && sp == 1 ? launch_skinny<32, 5, BF16, LORA>(g, d, sp, stream)
+                                         : launch_skinny<32, 10, BF16, LORA>(g, d, sp, stream);
+    return launch_skinny<64, 8, BF16, LORA>(g, d, sp, stream);
 }
 
-template <int CTA_GROUP, int BN, int STAGES, int MT = 1>
+template <int CTA_GROUP, int BN, int STAGES, int MT = 1, bool LORA = false>
 cudaError_t launch_dt(const GemmArgs &g, const DeviceInfo &d, int sms, cudaStream_t stream) {
-    return g.bf16 ? launch<CTA_GROUP, BN, STAGES, MT, true>(g, d, sms, stream)
-                  : launch<CTA_GROUP, BN, STAGES, MT, false>(g, d, sms, stream);
+    return g.bf16 ? launch<CTA_GROUP, BN, STAGES, MT, true, LORA>(g, d, sms, stream)
+                  : launch<CTA_GROUP, BN, STAGES, MT, false, LORA>(g, d, sms, stream);
 }
 
 }  // namespace
@@ -2248,6 +2359,84 @@ void plan_one_tile_row(const GemmArgs &g, int sms, int *block_n, int *split) {
             if (t < best) { best = t; *block_n = bn; *split = sp; }
         }
     }
+}
+
+// The kernel for a product with adapters: the automatic choice among the kernels that carry them (not the pair split-K
+// kernel, nor the tail split through a workspace).  variant as in hgemm_launch.
+void choose_lora(const GemmArgs &g, int sms, int *variant, int *block_n, int *split) {
+    *variant = 0;
+    *block_n = 0;
+    *split = 0;
+    if (g.m <= 64) {
+        *variant = 4;
+        return;
+    }
+    if (g.m <= 128) {
+        plan_one_tile_row(g, sms, block_n, split);
+        *variant = *split >= 2 ? 3 : 1;
+        return;
+    }
+    if (g.m <= 256 && g.k >= 2048) {
+        choose_splitk(g, sms, 0, block_n, split);
+        if (*split >= 2) {
+            *variant = 3;
+            return;
+        }
+    }
+    *block_n = 0;
+    choose_config(g, sms, variant, block_n);
+}
+
+int lora_group_rows(int64_t m, int64_t n, int64_t k, int sms) {
+    const GemmArgs g{nullptr, nullptr, nullptr, m, n, k, k, k, n, true};
+    int variant, block_n, split;
+    choose_lora(g, sms, &variant, &block_n, &split);
+    if (variant == 4) return m <= 16 ? 16 : m <= 32 ? 32 : 64;      // the skinny kernel's token tile
+    return variant == 5 ? 512 : variant == 2 ? 256 : 128;
+}
+
+int hgemm_launch_with_lora(const GemmArgs &g, cudaStream_t stream, cudaError_t *cuda_err) {
+    DeviceInfo *d = nullptr;
+    cudaError_t e = device_info(&d);
+    if (e != cudaSuccess) { *cuda_err = e; return kLaunchCuda; }
+    if (d->cc_major != 10) return kLaunchNotSm100;
+    const int sms = d->sm_count;
+    int variant, block_n, split;
+    choose_lora(g, sms, &variant, &block_n, &split);
+    if (variant == 4) {
+        e = g.bf16 ? launch_skinny_any<true, true>(g, *d, sms, 0, stream) : launch_skinny_any<false, true>(g, *d, sms, 0, stream);
+    } else if (variant == 3 && block_n == 128) {
+        e = g.bf16 ? launch_splitk<128, 5, true, true>(g, *d, split, stream) : launch_splitk<128, 5, false, true>(g, *d, split, stream);
+    } else if (variant == 3) {
+        e = g.bf16 ? launch_splitk<64, 8, true, true>(g, *d, split, stream) : launch_splitk<64, 8, false, true>(g, *d, split, stream);
+    } else if (variant == 1) {
+        e = block_n == 256 ? launch_dt<1, 256, 4, 1, true>(g, *d, sms, stream)
+          : block_n == 128 ? launch_dt<1, 128, 6, 1, true>(g, *d, sms, stream)
+                           : launch_dt<1, 64, 8, 1, true>(g, *d, sms, stream);
+    } else if (variant == 2) {
+        e = block_n == 256 ? launch_dt<2, 256, 6, 1, true>(g, *d, sms, stream)
+          : block_n == 128 ? launch_dt<2, 128, 8, 1, true>(g, *d, sms, stream)
+                           : launch_dt<2, 64, 8, 1, true>(g, *d, sms, stream);
+    } else {
+        e = launch_dt<2, 256, 4, 2, true>(g, *d, sms, stream);
+    }
+    if (e != cudaSuccess) { *cuda_err = e; return kLaunchCuda; }
+    return kLaunchOk;
+}
+
+cudaError_t gemm_device(int *sm_count, int *cc_major, int **status) {
+    DeviceInfo *d = nullptr;
+    const cudaError_t e = device_info(&d);
+    if (e != cudaSuccess) return e;
+    *sm_count = d->sm_count;
+    *cc_major = d->cc_major;
+    *status = d->status_word;
+    return cudaSuccess;
+}
+
+bool gemm_operand_map(CUtensorMap *tm, const void *base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_rows,
+                      bool bf16) {
+    return make_tmap(tm, base, rows, cols, ld, box_rows, bf16, false);
 }
 
 int hgemm_launch(const GemmArgs &g, int variant, int block_n, int max_sms, cudaStream_t stream,

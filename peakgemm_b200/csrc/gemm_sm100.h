@@ -1,9 +1,17 @@
 // Internal interface between the C ABI (api.cu) and the GEMM kernels (gemm_sm100.cu).
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 namespace pg {
+
+// What the GEMM kernels need to add the adapters' up projections (see lora_epilogue.cuh).
+struct LoraGemm {
+    const int32_t *ids, *table;
+    const void *v, *b;
+    int64_t adapters, rank, max_slots, group_rows, table_stride;
+};
 
 struct GemmArgs {
     void *c;
@@ -26,15 +34,28 @@ struct GemmArgs {
                                         // multimem.st instead of TMA stores to c; c must still be a local address
     void *workspace = nullptr;          // optional scratch for the tail split of the 256-wide CTA-pair kernel
     size_t workspace_bytes = 0;
+    const LoraGemm *lora = nullptr;     // adapters beside b (hgemm_launch_with_lora only)
 };
 
-enum LaunchResult { kLaunchOk = 0, kLaunchCuda = 1, kLaunchNotSm100 = 2, kLaunchBadConfig = 3 };
+enum LaunchResult { kLaunchOk = 0, kLaunchCuda = 1, kLaunchNotSm100 = 2, kLaunchBadConfig = 3, kLaunchTooLarge = 4 };
 
 // variant: 0 auto, 1 = one CTA per tile, 2 = CTA pair per tile, 3 = cluster split-K, 4 = skinny,
 // 5 = CTA pair with two row blocks per CTA (512 x 256 tiles); block_n: 0 auto, 64, 128, 256.
 // max_sms: 0 = all SMs, else an upper bound on the SMs the persistent grid occupies.
 int hgemm_launch(const GemmArgs &g, int variant, int block_n, int max_sms, cudaStream_t stream,
                  cudaError_t *cuda_err);
+
+// g's product and terms with the adapters of g.lora, whose v and table the previous launch on the stream writes: the
+// product's own k-blocks run beside that launch.  lora_group_rows: the rows that share a slot table, for a device with
+// `sms` SMs.
+int hgemm_launch_with_lora(const GemmArgs &g, cudaStream_t stream, cudaError_t *cuda_err);
+int lora_group_rows(int64_t m, int64_t n, int64_t k, int sms);
+
+// SM count, compute capability and status word of the current device; a tensor map of a row-major 16-bit matrix with
+// a box of box_rows x 64 elements, 128-byte swizzle.
+cudaError_t gemm_device(int *sm_count, int *cc_major, int **status);
+bool gemm_operand_map(CUtensorMap *tm, const void *base, int64_t rows, int64_t cols, int64_t ld, uint32_t box_rows,
+                      bool bf16);
 
 // Resolves variant/block_n == 0 to concrete values for a device with sm_count SMs.
 void choose_config(const GemmArgs &g, int sm_count, int *variant, int *block_n);

@@ -1,104 +1,334 @@
 // A projection with low-rank adapters of many requests at once: row t of the batch uses adapter i = ids[t],
 //     d[t] = row_scale[t] * (a[t] * b^T + scale[i] * (a[t] * A_i^T) * B_i^T) + bias + residual[t].
-// First form, plain: v = scale * a * A^T (one warp per element, fp32), then one thread per element of d.
+//
+// Two launches.  This file's kernel is the down projection, v[t] = scale * a[t] * A_i^T; the GEMM kernels of
+// gemm_sm100.cu run the product and take the up projection along as further k-blocks (lora_epilogue.cuh).  The GEMM is
+// launched under programmatic stream serialisation: it streams the shared weights while this kernel runs and waits for
+// it only in front of the tile's last block.
+//
+// Down projection, per 128 rows of a (one tile): the adapters that occur in the tile's group of rows are listed in the
+// order of their first row; their A_i, `rank` rows of k elements each, stand below one another as the second operand,
+// cut into chunks of 64 rows.  One cluster per tile and chunk computes 128 x 64 with tcgen05 (every row of a against
+// every listed adapter: the tensor pipe has time to spare, a and A_i are what costs), each CTA of the cluster a slice
+// of k; the partial sums meet through distributed shared memory in rank order.  Each CTA then writes its columns of V:
+// the scaled value, rounded once to the 16-bit type (the next product's operand type), for the rows that use the
+// adapter, zeros for the others (selected, not multiplied: a row's NaN stays its own).
 
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "gemm_common.cuh"
 #include "host_util.h"
 #include "lora.h"
-#include "rms_vec.cuh"
+#include "ptx.cuh"
 
 namespace pg {
+
+using namespace ptx;
+
 namespace {
 
-// v[t, r] = scale * sum_k a[t, k] A[ids[t], r, k], 0 without an adapter.
+constexpr uint32_t kChunk = 64;              // columns (adapter rows) of a tile
+constexpr uint32_t kStages = 4;
+constexpr uint32_t kXBytes = kBM * kBK * 2;
+constexpr uint32_t kWBytes = kChunk * kBK * 2;
+constexpr uint32_t kMaxGroup = 512;
+constexpr uint32_t kOffX = 0;
+constexpr uint32_t kOffW = kOffX + kStages * kXBytes;
+constexpr uint32_t kOffRecv = kOffW + kStages * kWBytes;        // [S slots][64/S/4][128 rows][4] fp32
+constexpr uint32_t kOffBar = kOffRecv + kBM * kChunk * 4;       // full[], empty[], acc_full
+constexpr uint32_t kOffMisc = kOffBar + (2 * kStages + 1) * 8;  // tensor-memory slot, abort flag, slot count
+constexpr uint32_t kOffPiece = kOffMisc + 16;                   // first row of A of each piece of the chunk
+constexpr uint32_t kOffIds = kOffPiece + 8 * 4;                 // the group's adapter ids, -1: none
+constexpr uint32_t kOffSlots = kOffIds + kMaxGroup * 4;         // the adapters that occur
+constexpr uint32_t kSmem = kOffSlots + kMaxGroup * 4 + 1024;
+
+struct Shrink {
+    const int32_t *ids;
+    const float *scale;
+    int32_t *table;
+    uint4 *v;
+    uint32_t m, k, adapters, rank, max_slots, group_rows, table_stride;
+    uint32_t piece;                // rows of A per load: 8 .. 64, divides rank and 64
+};
+
 template <bool BF16>
-__global__ void __launch_bounds__(256)
-lora_shrink_kernel(float *v, const uint4 *a, int64_t lda8, const LoraArgs l, int64_t m, int k8) {
-    const int64_t warp = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
-    if (warp >= m * l.rank) return;
-    const int lane = threadIdx.x & 31;
-    const int64_t t = warp / l.rank, r = warp - t * l.rank;
-    const int id = l.ids[t];
-    float sum = 0.f;
-    if (id >= 0 && id < l.adapters) {
-        const uint4 *x = a + t * lda8, *w = static_cast<const uint4 *>(l.a) + (static_cast<int64_t>(id) * l.rank + r) * k8;
-        for (int i = lane; i < k8; i += 32) {
-            float f[8], g[8];
-            vec_unpack<BF16>(x[i], f);
-            vec_unpack<BF16>(w[i], g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(f[e], g[e], sum);
+__global__ void __launch_bounds__(kThreads, 1)
+lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a, const Shrink p,
+                   int *status) {
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+    uint8_t *smem = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+    const uint32_t lane = threadIdx.x & 31u;
+    const uint32_t S = cluster_nctarank(), rank = cluster_ctarank();
+    const uint32_t cols = kChunk / S;                                  // columns this CTA finally owns
+    const uint32_t bar_full = smem_base + kOffBar, bar_empty = bar_full + kStages * 8, bar_acc = bar_empty + kStages * 8;
+    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + kOffMisc);
+    volatile uint32_t *abort_flag = misc + 1;
+    const WaitCtx ctx{abort_flag, status};
+    int32_t *piece_row = reinterpret_cast<int32_t *>(smem + kOffPiece);
+    int32_t *ids = reinterpret_cast<int32_t *>(smem + kOffIds), *slots = reinterpret_cast<int32_t *>(smem + kOffSlots);
+
+    const uint32_t row0 = blockIdx.x / S * kBM;                        // the tile's first row
+    const uint32_t group = row0 / p.group_rows, group0 = group * p.group_rows;
+    const uint32_t k_blocks = (p.k + kBK - 1) / kBK, per = (k_blocks + S - 1) / S;
+    const uint32_t kb0 = min(k_blocks, rank * per), kb1 = min(k_blocks, kb0 + per);
+    const bool has_k = kb1 > kb0;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < kStages; ++s) {
+            mbar_init(bar_full + s * 8, 1);
+            mbar_init(bar_empty + s * 8, 1);
         }
-        if (l.scale) sum *= l.scale[id];
+        mbar_init(bar_acc, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+        prefetch_tensormap(&tm_x);
+        prefetch_tensormap(&tm_a);
     }
-    sum = warp_sum_f32(sum);
-    if (lane == 0) v[warp] = sum;
+    if (warp == 1) {
+        tmem_alloc<1>(smem_base + kOffMisc, kChunk);
+        tmem_relinquish<1>();
+    }
+    // Everything before this launch has completed: the next launch, the GEMM, may read what they wrote at once.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    for (uint32_t i = threadIdx.x; i < p.group_rows; i += kThreads) {
+        const int32_t id = group0 + i < p.m ? p.ids[group0 + i] : -1;
+        ids[i] = id >= 0 && static_cast<uint32_t>(id) < p.adapters ? id : -1;
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = misc[0];
+    if (warp == 2) {
+        // The distinct ids in the order of their first row: 32 rows at a time, first against each other, then against
+        // the list so far.
+        uint32_t n = 0;
+        for (uint32_t r = 0; r < p.group_rows; r += 32) {
+            const int32_t id = r + lane < p.group_rows ? ids[r + lane] : -1;
+            const uint32_t same = __match_any_sync(0xffffffffu, id);       // every lane takes part
+            bool fresh = id >= 0 && __ffs(same) - 1 == static_cast<int>(lane);
+            for (uint32_t e = 0; e < n; ++e) fresh = fresh && slots[e] != id;
+            const uint32_t who = __ballot_sync(0xffffffffu, fresh);
+            if (fresh) slots[n + __popc(who & ((1u << lane) - 1u))] = id;
+            n += __popc(who);
+            __syncwarp();
+        }
+        if (lane == 0) misc[2] = n;
+    }
+    __syncthreads();
+    const uint32_t n_slots = misc[2], a_rows = n_slots * p.rank, chunks = (a_rows + kChunk - 1) / kChunk;
+    if (rank == 0 && blockIdx.y == 0 && row0 == group0) {
+        int32_t *t = p.table + static_cast<size_t>(group) * p.table_stride;
+        if (threadIdx.x == 0) t[0] = static_cast<int32_t>(n_slots);
+        for (uint32_t i = threadIdx.x; i < n_slots; i += kThreads) t[4 + i] = slots[i];
+    }
+    __syncwarp();              // the cluster barrier wants whole warps
+    cluster_arrive();          // every CTA of the cluster is running before anyone writes into its shared memory
+    cluster_wait();
+
+    uint32_t stage = 0, phase = 0, acc_phase = 0;
+    for (uint32_t c = blockIdx.y; c < chunks; c += gridDim.y, acc_phase ^= 1u) {
+        const uint32_t live = min(kChunk, a_rows - c * kChunk);       // columns of this chunk that exist
+        if (warp == 0) {
+            if (lane == 0) {
+                const uint32_t pieces = live / p.piece;
+                for (uint32_t i = 0; i < pieces; ++i) {
+                    const uint32_t at = c * kChunk + i * p.piece, slot = at / p.rank;
+                    piece_row[i] = slots[slot] * static_cast<int32_t>(p.rank) + static_cast<int32_t>(at - slot * p.rank);
+                }
+                const uint64_t keep = l2_policy_evict_last(), stream = l2_policy_evict_first();
+                for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                    if (!wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty)) break;
+                    const uint32_t full = bar_full + stage * 8;
+                    mbar_arrive_expect_tx(full, kXBytes + live * kBK * 2);
+                    const int32_t kx = static_cast<int32_t>(kb * kBK);
+                    tma_load_2d_hint(smem_base + kOffX + stage * kXBytes, &tm_x, full, kx, static_cast<int32_t>(row0), keep);
+                    for (uint32_t i = 0; i < pieces; ++i)
+                        tma_load_2d_hint(smem_base + kOffW + stage * kWBytes + i * p.piece * kBK * 2, &tm_a, full, kx,
+                                         piece_row[i], stream);
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                }
+            }
+            __syncwarp();
+        } else if (warp == 1) {
+            if (lane == 0 && has_k) {
+                // columns that do not exist hold what was in shared memory; they are not stored
+                constexpr uint32_t idesc = instr_desc_f16(BF16, kBM, kChunk);
+                bool ok = true;
+                for (uint32_t kb = kb0; kb < kb1; ++kb) {
+                    ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const uint64_t dx = smem_desc_k_sw128(smem_base + kOffX + stage * kXBytes);
+                    const uint64_t dw = smem_desc_k_sw128(smem_base + kOffW + stage * kWBytes);
+#pragma unroll
+                    for (uint32_t k = 0; k < kBK / kUmmaK; ++k)
+                        umma_f16<1>(tmem, dx + 2 * k, dw + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
+                    umma_commit<1>(bar_empty + stage * 8);
+                    if (++stage == kStages) { stage = 0; phase ^= 1u; }
+                }
+                if (ok) umma_commit<1>(bar_acc);
+            }
+            __syncwarp();
+        } else {
+            // my partial sums of the columns each peer owns go to that peer
+            const uint32_t q = warp & 3u, row = q * 32u + lane;
+            bool ok = has_k;
+            if (has_k) {
+                ok = wait_bar(bar_acc, acc_phase, ctx, kStEpiAccFull);
+                ok = __all_sync(0xffffffffu, ok);
+                tc_fence_after_sync();
+            }
+            float f[kChunk];
+#pragma unroll
+            for (uint32_t h = 0; h < 2; ++h) {
+                uint32_t v[32];
+                if (ok) {
+                    tmem_ld_32x32b_x32(tmem + ((q * 32u) << 16) + h * 32u, v);
+                    tmem_ld_wait();
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) f[h * 32 + i] = ok ? __uint_as_float(v[i]) : 0.f;
+            }
+            tc_fence_before_sync();
+            const uint32_t recv = smem_base + kOffRecv;
+#pragma unroll
+            for (uint32_t j = 0; j < kChunk / 4; ++j) {
+                const uint32_t owner = 4 * j / cols;
+                const uint32_t dst = recv + ((rank * (cols / 4) + (4 * j - owner * cols) / 4) * kBM + row) * 16u;
+                st_cluster_v4(mapa(dst, owner), f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+            }
+        }
+        __syncwarp();
+        cluster_arrive();          // all parts delivered
+        cluster_wait();
+        if (warp >= 2) {
+            const uint32_t row = (warp & 3u) * 32u + lane, in_group = row0 + row - group0;
+            if (in_group < p.group_rows && row0 + row < p.m) {
+                const int32_t id = ids[in_group];
+                const float4 *recv = reinterpret_cast<const float4 *>(smem + kOffRecv);
+                for (uint32_t g = 0; g < cols / 8; ++g) {
+                    const uint32_t local = rank * cols + 8 * g, at = c * kChunk + local;
+                    if (local >= live) break;
+                    const uint32_t slot = at / p.rank, r = at - slot * p.rank;
+                    uint4 out = make_uint4(0, 0, 0, 0);
+                    if (slots[slot] == id) {
+                        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                        for (uint32_t s = 0; s < S; ++s) {
+                            const float4 *src = recv + (s * (cols / 4) + 2 * g) * kBM + row;
+                            const float4 a = src[0], b = src[kBM];
+                            f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
+                            f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
+                        }
+                        const float scale = p.scale ? p.scale[id] : 1.f;
+                        out.x = pack2<BF16>(f[0] * scale, f[1] * scale);
+                        out.y = pack2<BF16>(f[2] * scale, f[3] * scale);
+                        out.z = pack2<BF16>(f[4] * scale, f[5] * scale);
+                        out.w = pack2<BF16>(f[6] * scale, f[7] * scale);
+                    }
+                    const int64_t v_row = (static_cast<int64_t>(group) * p.max_slots + slot) * p.group_rows + in_group;
+                    p.v[(v_row * p.rank + r) / 8] = out;
+                }
+            }
+        }
+        if (c + gridDim.y < chunks) {      // the receive buffer and the accumulator are free again everywhere
+            __syncwarp();
+            cluster_arrive();
+            cluster_wait();
+            tc_fence_after_sync();
+        }
+    }
+    __syncthreads();
+    if (*abort_flag) __nanosleep(50000);
+    if (warp == 1) {
+        tc_fence_after_sync();
+        tmem_dealloc<1>(tmem, kChunk);
+    }
 }
 
-// d[t, j] = row_scale * (sum_k a[t, k] b[j, k] + sum_r v[t, r] B[ids[t], j, r]) + bias[j] + residual[t, j].
-template <bool BF16>
-__global__ void __launch_bounds__(256)
-lora_expand_kernel(const GemmArgs g, const LoraArgs l, const float *v) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (i >= g.m * g.n) return;
-    const int64_t t = i / g.n, j = i - t * g.n;
-    const int id = l.ids[t];
-    float sum = 0.f, unused, x;
-    {
-        const uint4 *p = static_cast<const uint4 *>(g.a) + t * (g.lda / 8), *q = static_cast<const uint4 *>(g.b) + j * (g.ldb / 8);
-        for (int64_t c = 0; c < g.k / 8; ++c) {
-            float f[8], w[8];
-            vec_unpack<BF16>(p[c], f);
-            vec_unpack<BF16>(q[c], w);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(f[e], w[e], sum);
-        }
-    }
-    if (id >= 0 && id < l.adapters) {
-        const uint4 *w = static_cast<const uint4 *>(l.b) + (static_cast<int64_t>(id) * g.n + j) * (l.rank / 8);
-        for (int r = 0; r < l.rank / 8; ++r) {
-            float f[8];
-            vec_unpack<BF16>(w[r], f);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) sum = fmaf(f[e], v[t * l.rank + 8 * r + e], sum);
-        }
-    }
-    if (g.row_scale) sum *= g.row_scale[t];
-    if (g.bias) {
-        ptx::unpack2<BF16>(static_cast<const uint16_t *>(g.bias)[j], x, unused);
-        sum += x;
-    }
-    if (g.residual) {
-        ptx::unpack2<BF16>(static_cast<const uint16_t *>(g.residual)[t * g.ldr + j], x, unused);
-        sum += x;
-    }
-    static_cast<uint16_t *>(g.c)[t * g.ldc + j] = static_cast<uint16_t>(ptx::pack2<BF16>(sum, 0.f) & 0xffffu);
+struct Plan {
+    int64_t group_rows, groups, max_slots, table_stride, v_rows;
+    size_t off_v, bytes;
+};
+
+Plan make_plan(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank, int sms) {
+    Plan p;
+    p.group_rows = lora_group_rows(m, n, k, sms);
+    p.groups = (m + p.group_rows - 1) / p.group_rows;
+    p.max_slots = adapters < p.group_rows ? adapters : p.group_rows;
+    p.table_stride = 4 + p.max_slots;
+    p.v_rows = p.groups * p.max_slots * p.group_rows;
+    p.off_v = (static_cast<size_t>(p.groups) * p.table_stride * 4 + 255) / 256 * 256;
+    p.bytes = p.off_v + static_cast<size_t>(p.v_rows) * rank * 2;
+    return p;
 }
 
 }  // namespace
 
-size_t lora_workspace_bytes(int64_t m, int64_t, int64_t, int64_t, int64_t rank) {
-    return (static_cast<size_t>(m) * rank * sizeof(float) + 255) / 256 * 256;
+cudaError_t lora_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank, size_t *bytes) {
+    int sms = 0;
+    const cudaError_t e = current_device_sm_count(&sms);
+    if (e != cudaSuccess) return e;
+    *bytes = make_plan(m, n, k, adapters, rank, sms).bytes;
+    return cudaSuccess;
 }
 
 int hgemm_lora_launch(const GemmArgs &g, const LoraArgs &l, cudaStream_t stream, cudaError_t *cuda_err) {
-    float *v = static_cast<float *>(l.workspace);
-    const int64_t warps = g.m * l.rank, elements = g.m * g.n;
-    if ((warps + 7) / 8 > 2147483647 || (elements + 255) / 256 > 2147483647) return kLaunchBadConfig;
-    const unsigned gs = static_cast<unsigned>((warps + 7) / 8), ge = static_cast<unsigned>((elements + 255) / 256);
-    const int k8 = static_cast<int>(g.k / 8);
-    if (g.bf16) {
-        lora_shrink_kernel<true><<<gs, 256, 0, stream>>>(v, static_cast<const uint4 *>(g.a), g.lda / 8, l, g.m, k8);
-        lora_expand_kernel<true><<<ge, 256, 0, stream>>>(g, l, v);
-    } else {
-        lora_shrink_kernel<false><<<gs, 256, 0, stream>>>(v, static_cast<const uint4 *>(g.a), g.lda / 8, l, g.m, k8);
-        lora_expand_kernel<false><<<ge, 256, 0, stream>>>(g, l, v);
-    }
-    const cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) { *cuda_err = e; return kLaunchCuda; }
-    return kLaunchOk;
+    const auto failed = [cuda_err](cudaError_t e) { *cuda_err = e; return static_cast<int>(kLaunchCuda); };
+    int sms = 0, cc = 0, *status = nullptr;
+    cudaError_t e = gemm_device(&sms, &cc, &status);
+    if (e != cudaSuccess) return failed(e);
+    if (cc != 10) return kLaunchNotSm100;
+    const Plan p = make_plan(g.m, g.n, g.k, l.adapters, l.rank, sms);
+    if (p.v_rows > 2147483647) return kLaunchTooLarge;           // V's rows are counted in 32 bits
+    int32_t *table = static_cast<int32_t *>(l.workspace);
+    uint8_t *v = static_cast<uint8_t *>(l.workspace) + p.off_v;
+
+    Shrink s = {l.ids, l.scale, table, reinterpret_cast<uint4 *>(v), static_cast<uint32_t>(g.m), static_cast<uint32_t>(g.k),
+                static_cast<uint32_t>(l.adapters), static_cast<uint32_t>(l.rank), static_cast<uint32_t>(p.max_slots),
+                static_cast<uint32_t>(p.group_rows), static_cast<uint32_t>(p.table_stride), 8};
+    while (s.piece < kChunk && l.rank % (2 * s.piece) == 0) s.piece *= 2;
+    CUtensorMap tm_x, tm_a;
+    if (!gemm_operand_map(&tm_x, g.a, g.m, g.k, g.lda, kBM, g.bf16) ||
+        !gemm_operand_map(&tm_a, l.a, l.adapters * l.rank, g.k, g.k, s.piece, g.bf16))
+        return failed(cudaErrorInvalidValue);
+    // The largest cluster over k that keeps the tiles within one wave and leaves every CTA four k-blocks.
+    const int64_t tiles = (g.m + kBM - 1) / kBM, k_blocks = (g.k + kBK - 1) / kBK;
+    int64_t split = 1;
+    while (split < 8 && tiles * split * 2 <= sms && k_blocks >= 8 * split) split *= 2;
+    // Clusters for as many chunks as there can be, up to two waves of CTAs; those without a chunk leave at once.
+    int64_t chunks = (p.max_slots < g.m ? p.max_slots : g.m) * l.rank;
+    chunks = (chunks + kChunk - 1) / kChunk;
+    const int64_t most = 2 * sms / (tiles * split);
+    if (chunks > most) chunks = most < 1 ? 1 : most;
+
+    auto kernel = g.bf16 ? lora_shrink_kernel<true> : lora_shrink_kernel<false>;
+    static DeviceOnce once[2];
+    if ((e = allow_dynamic_smem(once[g.bf16 ? 1 : 0], kernel, kSmem)) != cudaSuccess) return failed(e);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * split), static_cast<unsigned>(chunks), 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if ((e = cudaLaunchKernelEx(&cfg, kernel, tm_x, tm_a, s, status)) != cudaSuccess) return failed(e);
+
+    const LoraGemm lg = {l.ids, table, v, l.b, l.adapters, l.rank, p.max_slots, p.group_rows, p.table_stride};
+    GemmArgs with = g;
+    with.lora = &lg;
+    return hgemm_launch_with_lora(with, stream, cuda_err);
 }
 
 }  // namespace pg

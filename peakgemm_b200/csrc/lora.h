@@ -16,7 +16,8 @@ struct LoraArgs {
     void *workspace;
 };
 
-size_t lora_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank);
+// Scratch for this shape on the current device.
+cudaError_t lora_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank, size_t *bytes);
 
 // g's product and epilogue terms plus the adapters' contribution; a LaunchResult.
 int hgemm_lora_launch(const GemmArgs &g, const LoraArgs &l, cudaStream_t stream, cudaError_t *cuda_err);

@@ -1,0 +1,139 @@
+// The adapters inside the GEMM kernels of gemm_sm100.cu.
+//
+// The up projection is more k: with v[t] = scale * x[t] A^T (lora.cu) a tile's accumulator gets, behind the k-blocks of
+// x W^T, one k-block of up to 64 rank elements for every adapter that occurs among the tile's rows:
+//     acc[t, j] += sum_r V[t, r] B_i[j, r],     V = v for the rows t that use adapter i, zeros for the others.
+// The contribution is added in fp32 before the one rounding, and the output is neither read again nor written twice.
+// A tile's rows form a group; lora.cu writes the group's adapters in the order of their first row ("slots") into a table
+// and the masked V of each slot, [group rows, rank], next to it.
+#pragma once
+
+#include <cuda.h>
+#include <stdint.h>
+
+#include "gemm_common.cuh"
+#include "rms_vec.cuh"
+
+namespace pg {
+namespace {
+
+struct LoraDev {
+    const int32_t *ids;         // [m]
+    const int32_t *table;       // per group table_stride words: the number of slots, 3 unused words, the slots' adapters
+    const uint16_t *v;          // [groups][max_slots][group_rows][rank]
+    const uint16_t *b;          // [adapters][n][rank]
+    const uint16_t *x, *w;      // the product's operands
+    int64_t ldx, ldw;
+    uint32_t k, n, rank, rank_blocks, max_slots, group_rows, table_stride;
+};
+
+template <bool LORA> struct LoraParam {};
+template <> struct LoraParam<true> {
+    CUtensorMap tm_v, tm_b;
+    LoraDev d;
+};
+
+// What a stage holds, written by the producer before it arms the stage: the number of 16-element steps of k, and
+// whether the tile ends with it.
+constexpr uint32_t kLoraLast = 8u;
+
+// The producer's walk over a tile's adapter blocks: `count` of them, slots first, first + step, ...
+struct LoraBlocks {
+    uint32_t count = 0, slot = 0, slot_step = 1, rb = 0, base = 0;
+    const int32_t *adapters = nullptr;
+    int32_t v_row = 0, b_row = 0;      // of the block that next() returned
+
+    __device__ __forceinline__ void open(const LoraDev &d, uint32_t group, uint32_t first = 0, uint32_t step = 1) {
+        const int32_t *t = d.table + static_cast<size_t>(group) * d.table_stride;
+        const uint32_t n = min(static_cast<uint32_t>(t[0]), d.max_slots);
+        adapters = t + 4;
+        slot = first;
+        slot_step = step;
+        rb = 0;
+        base = group * d.max_slots;
+        count = n > first ? (n - first + step - 1) / step * d.rank_blocks : 0u;
+    }
+    // The word of the stage that block kb goes to (block kb1 - 1 is the product's last).
+    __device__ __forceinline__ uint32_t info(const LoraDev &d, uint32_t kb, uint32_t kb1) const {
+        const uint32_t last = kb + 1 >= kb1 && kb + 1 - kb1 == count ? kLoraLast : 0u;
+        if (kb < kb1) return kBK / kUmmaK | last;
+        return min(kBK, d.rank - rb * kBK + kUmmaK - 1) / kUmmaK | last;
+    }
+    // Moves to the next block; returns its first rank element.
+    __device__ __forceinline__ int32_t next(const LoraDev &d) {
+        v_row = static_cast<int32_t>((base + slot) * d.group_rows);
+        b_row = adapters[slot] * static_cast<int32_t>(d.n);
+        const int32_t x = static_cast<int32_t>(rb * kBK);
+        if (++rb == d.rank_blocks) {
+            rb = 0;
+            slot += slot_step;
+        }
+        return x;
+    }
+};
+
+// A zero of V times an infinity or NaN in another row's adapter is NaN: such an element is computed again from its own
+// row's terms alone.  `acc` unless one of the group's other adapters holds such a value in this column.
+template <bool BF16>
+__device__ __noinline__ float lora_exact(const LoraDev &d, uint32_t group, uint32_t row, uint32_t col, float acc) {
+    const int32_t *t = d.table + static_cast<size_t>(group) * d.table_stride;
+    const int32_t slots = t[0], id = d.ids[row];
+    int32_t mine = -1;
+    bool other = false;
+    const uint32_t r8 = d.rank / 8;
+    float f[8], g[8];
+    for (int32_t s = 0; s < slots; ++s) {
+        const int32_t a = t[4 + s];
+        if (a == id) {
+            mine = s;
+            continue;
+        }
+        const uint4 *b = reinterpret_cast<const uint4 *>(d.b) + (static_cast<int64_t>(a) * d.n + col) * r8;
+        for (uint32_t r = 0; r < r8; ++r) {
+            vec_unpack<BF16>(b[r], f);
+            for (int e = 0; e < 8; ++e) other |= !(fabsf(f[e]) < __int_as_float(0x7f800000));     // infinity or NaN
+        }
+    }
+    if (!other) return acc;
+    float sum = 0.f;
+    const uint4 *x = reinterpret_cast<const uint4 *>(d.x + static_cast<int64_t>(row) * d.ldx);
+    const uint4 *w = reinterpret_cast<const uint4 *>(d.w + static_cast<int64_t>(col) * d.ldw);
+    for (uint32_t c = 0; c < d.k / 8; ++c) {
+        vec_unpack<BF16>(x[c], f);
+        vec_unpack<BF16>(w[c], g);
+        for (int e = 0; e < 8; ++e) sum = fmaf(f[e], g[e], sum);
+    }
+    if (mine >= 0) {
+        const uint32_t in_group = row - group * d.group_rows;
+        const uint4 *v = reinterpret_cast<const uint4 *>(d.v) +
+                         ((static_cast<int64_t>(group) * d.max_slots + mine) * d.group_rows + in_group) * r8;
+        const uint4 *b = reinterpret_cast<const uint4 *>(d.b) + (static_cast<int64_t>(id) * d.n + col) * r8;
+        for (uint32_t r = 0; r < r8; ++r) {
+            vec_unpack<BF16>(v[r], f);
+            vec_unpack<BF16>(b[r], g);
+            for (int e = 0; e < 8; ++e) sum = fmaf(f[e], g[e], sum);
+        }
+    }
+    return sum;
+}
+
+// N accumulators of row `row`, columns col, col + 1, ...
+template <bool BF16, int N>
+__device__ __forceinline__ void lora_repair(float (&f)[N], const LoraDev &d, uint32_t group, uint32_t row, uint32_t col,
+                                            uint32_t M) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) bad |= f[i] != f[i];
+    if (!bad || row >= M) return;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (f[i] != f[i] && col + i < d.n) f[i] = lora_exact<BF16>(d, group, row, col + i, f[i]);
+}
+template <bool BF16>
+__device__ __forceinline__ void lora_repair(uint32_t (&v)[32], const LoraDev &d, uint32_t group, uint32_t row, uint32_t col,
+                                            uint32_t M) {
+    lora_repair<BF16, 32>(reinterpret_cast<float(&)[32]>(v), d, group, row, col, M);
+}
+
+}  // namespace
+}  // namespace pg
