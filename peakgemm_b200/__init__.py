@@ -45,6 +45,10 @@ torch.ops.load_library(TORCH_LIB_PATH)
 _gemm_peak = torch.ops.PeakGemm.gemm_peak
 _rms_norm_fwd = torch.ops.PeakGemm.rms_norm_fwd
 _rms_norm_bwd = torch.ops.PeakGemm.rms_norm_bwd
+# the overloads themselves: a small call is bound by the host, and the lookup through the packet is part of it
+_gemm_peak_lora = torch.ops.PeakGemm.gemm_peak_lora.default
+_rms_norm_residual_fwd = torch.ops.PeakGemm.rms_norm_residual_fwd.default
+_rms_norm_residual_bwd = torch.ops.PeakGemm.rms_norm_residual_bwd.default
 
 
 def gemm_peak(c: torch.Tensor, a: torch.Tensor, b: torch.Tensor) -> None:
@@ -123,15 +127,11 @@ def gemm_peak_lora(d: torch.Tensor, a: torch.Tensor, b: torch.Tensor, lora_a: to
     into lora_a as into the weights: ``fold_gamma(lora_a.view(-1, k), gamma).view_as(lora_a)``.
     """
     assert a.dtype in [torch.half, torch.bfloat16]
-    k = a.shape[-1]
-    n = b.shape[0]
-    assert b.shape[1] == k and lora_a.shape[2] == k and lora_b.shape == (lora_a.shape[0], n, lora_a.shape[1])
-    a2 = a.view(-1, k)
-    d2 = d.view(-1, n)
-    assert d2.shape[0] == a2.shape[0] and ids.numel() == a2.shape[0]
-    rs = row_scale.view(-1) if row_scale is not None else None
-    res = residual.view(-1, n) if residual is not None else None
-    torch.ops.PeakGemm.gemm_peak_lora(d2, a2, b, lora_a, lora_b, ids.view(-1), scale, rs, bias, res)
+    if a.dim() != 2:
+        n = b.shape[0]
+        a, d, ids = a.view(-1, a.shape[-1]), d.view(-1, n), ids.view(-1)
+        residual = residual.view(-1, n) if residual is not None else None
+    _gemm_peak_lora(d, a, b, lora_a, lora_b, ids, scale, row_scale, bias, residual)     # checks the shapes
 
 
 def fold_gamma(w: torch.Tensor, gamma: torch.Tensor) -> torch.Tensor:
@@ -161,10 +161,6 @@ def rms_norm_linear(out: torch.Tensor, x: torch.Tensor, w_folded: torch.Tensor, 
     return rstd
 
 
-def _flat(t: torch.Tensor | None, h: int) -> torch.Tensor | None:
-    return t.view(-1, h) if t is not None else None
-
-
 def rms_norm_residual_fwd(s: torch.Tensor, y: torch.Tensor | None, u: torch.Tensor, residual: torch.Tensor, *,
                           gamma_post: torch.Tensor | None = None, gate: torch.Tensor | None = None,
                           res_scale: torch.Tensor | None = None, gamma_pre: torch.Tensor | None = None,
@@ -181,11 +177,8 @@ def rms_norm_residual_fwd(s: torch.Tensor, y: torch.Tensor | None, u: torch.Tens
     arithmetic; y comes from s before its rounding.  ``s`` may be ``residual`` itself and ``y`` may be ``u`` itself.
     """
     assert u.dtype in [torch.half, torch.bfloat16]
-    h = u.shape[-1]
-    assert s.shape == u.shape and residual.shape == u.shape and (y is None or y.shape == u.shape)
     assert (y is None) == (gamma_pre is None)
-    torch.ops.PeakGemm.rms_norm_residual_fwd(s.view(-1, h), _flat(y, h), u.view(-1, h), residual.view(-1, h), gamma_post,
-                                             _flat(gate, h), res_scale, gamma_pre, eps)
+    _rms_norm_residual_fwd(s, y, u, residual, gamma_post, gate, res_scale, gamma_pre, eps)     # checks the shapes
 
 
 def rms_norm_residual_bwd(du: torch.Tensor, dresidual: torch.Tensor, dy: torch.Tensor | None, ds: torch.Tensor | None,
@@ -205,14 +198,8 @@ def rms_norm_residual_bwd(du: torch.Tensor, dresidual: torch.Tensor, dy: torch.T
     ``du`` may be ``u`` or ``dy`` itself.
     """
     assert du.dtype in [torch.half, torch.bfloat16]
-    h = du.shape[-1]
-    for t in (dresidual, dy, ds, s, u, residual):
-        assert t is None or t.shape == du.shape
-    for d, t in ((dgamma_post, gamma_post), (dgate, gate), (dres_scale, res_scale), (dgamma_pre, gamma_pre)):
-        assert d is None or (t is not None and d.shape == t.shape)
-    torch.ops.PeakGemm.rms_norm_residual_bwd(du.view(-1, h), dresidual.view(-1, h), dgamma_post, _flat(dgate, h),
-                                             dres_scale, dgamma_pre, _flat(dy, h), _flat(ds, h), _flat(s, h), _flat(u, h),
-                                             _flat(residual, h), gamma_post, _flat(gate, h), res_scale, gamma_pre, eps)
+    _rms_norm_residual_bwd(du, dresidual, dgamma_post, dgate, dres_scale, dgamma_pre, dy, ds, s, u, residual, gamma_post,
+                           gate, res_scale, gamma_pre, eps)     # checks the shapes
 
 
 def _register_fakes() -> None:

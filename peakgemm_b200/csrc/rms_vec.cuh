@@ -1,4 +1,5 @@
-// 16-byte vectors of eight 16-bit elements <-> fp32, and the warp sum, for the kernels of rmsnorm_residual*.cu.
+// Pieces of the RMSNorm kernels: bulk row copies and the voting group barrier (rmsnorm_staged.cu, rmsnorm_residual_staged.cu),
+// 16-byte vectors of eight 16-bit elements <-> fp32, and the warp sum.
 #pragma once
 
 #include <stdint.h>
@@ -21,10 +22,21 @@ __device__ __forceinline__ uint4 vec_pack(const float (&f)[8]) {
                       ptx::pack2<BF16>(f[6], f[7]));
 }
 
+// First row of the c-th of n runs that share `rows` rows evenly.
+__host__ __device__ __forceinline__ uint32_t rms_run_begin(uint32_t c, uint32_t n, uint32_t rows) {
+    return static_cast<uint32_t>(static_cast<uint64_t>(c) * rows / n);
+}
+
 // Eight consecutive fp32 values, 16-byte aligned.
 __device__ __forceinline__ void vec_load_f32(const float *p, float (&f)[8]) {
     const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
     const float4 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
+    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+// The same from global or shared memory.
+__device__ __forceinline__ void vec_load_f32_any(const float *p, float (&f)[8]) {
+    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
     f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }
@@ -37,6 +49,32 @@ __device__ __forceinline__ float warp_sum_f32(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
+}
+
+// 1-D bulk copy global -> shared; both addresses 16-byte aligned, bytes % 16 == 0.
+__device__ __forceinline__ void bulk_load(uint32_t dst_smem, const void *src, uint32_t bytes, uint32_t bar,
+                                          uint64_t policy) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint "
+                 "[%0], [%1], %2, [%3], %4;"
+                 ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar), "l"(policy)
+                 : "memory");
+}
+
+// Named barrier `id` over `nthreads` consumer threads that also ORs a predicate across
+// them, so that "somebody abandoned a wait" is decided identically by the whole group.
+__device__ __forceinline__ bool group_barrier_or(uint32_t id, uint32_t nthreads, bool pred) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "bar.red.or.pred p, %2, %3, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "}\n"
+        : "=r"(r)
+        : "r"(static_cast<uint32_t>(pred)), "r"(id), "r"(nthreads)
+        : "memory");
+    return r != 0;
 }
 
 }  // namespace pg

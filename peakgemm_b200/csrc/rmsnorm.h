@@ -70,11 +70,26 @@ cudaError_t rmsnorm_residual_fwd_launch(const RmsResidualFwdArgs &a, cudaStream_
 cudaError_t rmsnorm_residual_bwd_bytes(int64_t rows, int64_t h, int64_t gate_rows, size_t *bytes);
 cudaError_t rmsnorm_residual_bwd_launch(const RmsResidualBwdArgs &a, cudaStream_t stream);
 
+// Backward, sums over rows: the rows are cut into `workers` consecutive runs; worker w's fp32 part of dgamma_post,
+// dgamma_pre and dres_scale is row w of its table.  A gate whose rows lie in one run gets its gradient from that worker;
+// one whose rows lie in several gets a part from each: a run holds at most two such gates, its first (row 2w of `gate`)
+// and its last (row 2w + 1).
+struct RmsResidualParts {
+    float *post, *pre, *scale, *gate;
+    double *scale_one;      // n_one of them, where res_scale has one element
+    uint32_t workers, n_one;
+};
+// Bulk-copy staged backward kernel (rmsnorm_residual_staged.cu), for the widths where `workers` is not 0.
+uint32_t rmsnorm_residual_staged_workers(int64_t rows, int64_t h, int sms);
+cudaError_t rmsnorm_residual_staged_bwd(const RmsResidualBwdArgs &a, const RmsResidualParts &parts, cudaStream_t stream);
+
 // Bulk-copy staged variants (rmsnorm_staged.cu), used for 2048 <= h <= 16384.
 bool rmsnorm_staged_supported(int64_t h, bool bwd);
 cudaError_t rmsnorm_staged_ctas(int64_t rows, int64_t h, bool bwd, int *ctas, int *partial_rows);
 cudaError_t rmsnorm_staged_fwd(const RmsFwdArgs &a, cudaStream_t stream);
 cudaError_t rmsnorm_staged_bwd(const RmsBwdArgs &a, cudaStream_t stream);   // writes the partial rows only
+// SM count of the current device and the staged kernels' status word there.
+cudaError_t rmsnorm_device(int *sms, int **status);
 // Synchronises the stream, returns and clears the staged kernels' device status word.
 cudaError_t rmsnorm_device_status(int *out, cudaStream_t stream);
 

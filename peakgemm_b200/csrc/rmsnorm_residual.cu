@@ -271,30 +271,16 @@ rms_residual_bwd_stats_kernel(const RmsResidualBwdArgs a, RowStats *stats, uint3
     }
 }
 
-// Where the parts of the column sums go.  The rows are cut into `chunks` consecutive chunks; chunk c's fp32 part of
-// dgamma_post, dgamma_pre and dres_scale is row c of its table.  A gate whose rows lie in one chunk gets its gradient
-// from that chunk; one whose rows lie in several gets a part from each: a chunk holds at most two such gates, its
-// first (row 2c of `gate`) and its last (row 2c + 1).
-struct Parts {
-    float *post, *pre, *scale, *gate;
-    double *scale_one;      // one per chunk and column block
-    uint32_t chunks;
-};
-
-__host__ __device__ __forceinline__ uint32_t chunk_begin(uint32_t c, uint32_t chunks, uint32_t rows) {
-    return static_cast<uint32_t>(static_cast<uint64_t>(c) * rows / chunks);
-}
-
 constexpr int kColThreads = 64;
 
 // Thread = one vector of eight columns over the rows of one chunk.
 template <bool BF16>
 __global__ void __launch_bounds__(kColThreads)
-rms_residual_bwd_cols_kernel(const RmsResidualBwdArgs a, const RowStats *stats, const Parts parts,
+rms_residual_bwd_cols_kernel(const RmsResidualBwdArgs a, const RowStats *stats, const RmsResidualParts parts,
                              uint32_t rows_per_gate) {
     const int h8 = static_cast<int>(a.t.h / 8), idx = blockIdx.x * kColThreads + threadIdx.x;
     const uint32_t rows = static_cast<uint32_t>(a.t.rows);
-    const uint32_t r0 = chunk_begin(blockIdx.y, parts.chunks, rows), r1 = chunk_begin(blockIdx.y + 1, parts.chunks, rows);
+    const uint32_t r0 = rms_run_begin(blockIdx.y, parts.workers, rows), r1 = rms_run_begin(blockIdx.y + 1, parts.workers, rows);
     float gp[8], sc[8], gate[8], q[8], post[8], pre[8], scale[8];
     double one = 0.0;
 #pragma unroll
@@ -371,12 +357,16 @@ rms_residual_bwd_cols_kernel(const RmsResidualBwdArgs a, const RowStats *stats, 
     }
 }
 
-// Adds the parts in a fixed order.  blockIdx.y: 0 dgamma_post, 1 dgamma_pre, 2 dres_scale, 3 + b the gate that has
-// rows on both sides of the end of chunk b (if there is one and b is its first chunk).  Block = 32 groups of four columns x 32 slices of the parts.
+// Adds the parts in a fixed order.  blockIdx.y: 0 dgamma_post, 1 dgamma_pre, 2 dres_scale; from 3 on the gates whose
+// rows lie in several runs, found through the gates (gates_by_run false: 3 + the gate) or through the runs' borders
+// (3 + the run: the gate that begins in it and reaches past its end).  Block = 32 groups of four columns x 32 slices.
 template <bool BF16>
 __global__ void __launch_bounds__(1024)
-rms_residual_bwd_reduce_kernel(const RmsResidualBwdArgs a, const Parts parts, uint32_t rows_per_gate, uint32_t n_one) {
+rms_residual_bwd_reduce_kernel(const RmsResidualBwdArgs a, const RmsResidualParts parts, uint32_t rows_per_gate, bool gates_by_run) {
     __shared__ float4 red[32][33];
+    // launched under programmatic stream serialisation, as the staged kernel in front of it
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int cx = threadIdx.x & 31, sl = threadIdx.x >> 5;
     const int64_t h4 = a.t.h / 4, col = static_cast<int64_t>(blockIdx.x) * 32 + cx;
     const uint32_t rows = static_cast<uint32_t>(a.t.rows);
@@ -384,7 +374,7 @@ rms_residual_bwd_reduce_kernel(const RmsResidualBwdArgs a, const Parts parts, ui
         if (blockIdx.x != 0) return;
         double *rd = reinterpret_cast<double *>(&red[0][0]);
         double v = 0.0;
-        for (uint32_t i = threadIdx.x; i < n_one; i += 1024) v += parts.scale_one[i];
+        for (uint32_t i = threadIdx.x; i < parts.n_one; i += 1024) v += __ldcg(parts.scale_one + i);
         rd[threadIdx.x] = v;
         __syncthreads();
         for (int s = 512; s > 0; s >>= 1) {
@@ -396,16 +386,19 @@ rms_residual_bwd_reduce_kernel(const RmsResidualBwdArgs a, const Parts parts, ui
     }
     const float *src = blockIdx.y == 0 ? parts.post : blockIdx.y == 1 ? parts.pre : parts.scale;
     float *dst = blockIdx.y == 0 ? a.dgamma_post : blockIdx.y == 1 ? a.dgamma_pre : a.dres_scale;
-    uint32_t c0 = 0, c1 = parts.chunks, gi = 0;
+    uint32_t c0 = 0, c1 = parts.workers, gi = 0;
     if (blockIdx.y >= 3) {
-        const uint32_t border = chunk_begin(blockIdx.y - 2, parts.chunks, rows);
-        if (border % rows_per_gate == 0) return;
-        gi = border / rows_per_gate;
-        // first and last chunk that hold rows of the gate: chunk c begins at floor(c * rows / chunks)
+        gi = blockIdx.y - 3;
+        if (gates_by_run) {
+            const uint32_t border = rms_run_begin(blockIdx.y - 2, parts.workers, rows);
+            if (border % rows_per_gate == 0) return;
+            gi = border / rows_per_gate;
+        }
+        // first and last run that hold rows of the gate: run c begins at floor(c * rows / workers)
         const uint64_t first = static_cast<uint64_t>(gi) * rows_per_gate, last = first + rows_per_gate - 1;
-        c0 = static_cast<uint32_t>(((first + 1) * parts.chunks - 1) / rows);
-        c1 = static_cast<uint32_t>(((last + 1) * parts.chunks - 1) / rows) + 1;
-        if (c0 != blockIdx.y - 3) return;
+        c0 = static_cast<uint32_t>(((first + 1) * parts.workers - 1) / rows);
+        c1 = static_cast<uint32_t>(((last + 1) * parts.workers - 1) / rows) + 1;
+        if (c1 - c0 < 2 || (gates_by_run && c0 != blockIdx.y - 3)) return;
     } else if (!dst) {
         return;
     }
@@ -414,10 +407,10 @@ rms_residual_bwd_reduce_kernel(const RmsResidualBwdArgs a, const Parts parts, ui
         for (uint32_t c = c0 + sl; c < c1; c += 32) {
             float4 p;
             if (blockIdx.y < 3) {
-                p = reinterpret_cast<const float4 *>(src)[c * h4 + col];
+                p = __ldcg(reinterpret_cast<const float4 *>(src) + c * h4 + col);
             } else {
-                const uint32_t slot = gi == chunk_begin(c, parts.chunks, rows) / rows_per_gate ? 0u : 1u;
-                p = reinterpret_cast<const float4 *>(parts.gate)[(2 * static_cast<int64_t>(c) + slot) * h4 + col];
+                const uint32_t slot = gi == rms_run_begin(c, parts.workers, rows) / rows_per_gate ? 0u : 1u;
+                p = __ldcg(reinterpret_cast<const float4 *>(parts.gate) + (2 * static_cast<int64_t>(c) + slot) * h4 + col);
             }
             v.x += p.x; v.y += p.y; v.z += p.z; v.w += p.w;
         }
@@ -441,29 +434,32 @@ rms_residual_bwd_reduce_kernel(const RmsResidualBwdArgs a, const Parts parts, ui
 
 uint32_t col_blocks(int64_t h) { return static_cast<uint32_t>((h / 8 + kColThreads - 1) / kColThreads); }
 
-// Chunks of rows: about 16 blocks of the column kernel per SM.
-uint32_t bwd_chunks(int64_t rows, int64_t h, int sms) {
-    int64_t c = (static_cast<int64_t>(sms) * 16 + col_blocks(h) - 1) / col_blocks(h);
-    if (c > rows) c = rows;
-    return static_cast<uint32_t>(c);
-}
-
-// Workspace: [stats of the rows][parts].
-struct Workspace {
-    size_t stats, post, pre, scale, gate, one, total;
+// How the backward pass of a shape runs: the staged kernel where it has the width, else the statistics and column
+// kernels with about 16 blocks of the latter per SM; and its workspace: [parts][statistics of the rows].
+struct BwdPlan {
+    bool staged;
+    uint32_t workers, n_one;
+    size_t post, pre, scale, one, gate, stats, total;
 };
-Workspace bwd_workspace(int64_t rows, int64_t h, int64_t gate_rows, uint32_t chunks) {
+BwdPlan bwd_plan(int64_t rows, int64_t h, int64_t gate_rows, int sms) {
     const auto up = [](size_t b) { return (b + 255) / 256 * 256; };
-    const size_t table = up(static_cast<size_t>(chunks) * h * sizeof(float));
-    Workspace w;
-    w.stats = 0;
-    w.post = up(static_cast<size_t>(rows) * sizeof(RowStats));
-    w.pre = w.post + table;
-    w.scale = w.pre + table;
-    w.one = w.scale + table;
-    w.gate = w.one + up(static_cast<size_t>(chunks) * col_blocks(h) * sizeof(double));
-    w.total = w.gate + (gate_rows ? 2 * table : 0);
-    return w;
+    BwdPlan p;
+    p.workers = rmsnorm_residual_staged_workers(rows, h, sms);
+    p.staged = p.workers > 0;
+    if (!p.staged) {
+        const int64_t c = (static_cast<int64_t>(sms) * 16 + col_blocks(h) - 1) / col_blocks(h);
+        p.workers = static_cast<uint32_t>(c < rows ? c : rows);
+    }
+    p.n_one = p.staged ? p.workers : p.workers * col_blocks(h);
+    const size_t table = up(static_cast<size_t>(p.workers) * h * sizeof(float));
+    p.post = 0;
+    p.pre = p.post + table;
+    p.scale = p.pre + table;
+    p.one = p.scale + table;
+    p.gate = p.one + up(p.n_one * sizeof(double));
+    p.stats = p.gate + (gate_rows ? 2 * table : 0);
+    p.total = p.stats + (p.staged ? 0 : up(static_cast<size_t>(rows) * sizeof(RowStats)));
+    return p;
 }
 
 uint32_t rows_per_gate(const RmsResidualTerms &t) {
@@ -502,7 +498,7 @@ cudaError_t rmsnorm_residual_bwd_bytes(int64_t rows, int64_t h, int64_t gate_row
     int sms = 0;
     const cudaError_t e = current_device_sm_count(&sms);
     if (e != cudaSuccess) return e;
-    *bytes = bwd_workspace(rows, h, gate_rows, bwd_chunks(rows, h, sms)).total;
+    *bytes = bwd_plan(rows, h, gate_rows, sms).total;
     return cudaSuccess;
 }
 
@@ -510,28 +506,49 @@ cudaError_t rmsnorm_residual_bwd_launch(const RmsResidualBwdArgs &a, cudaStream_
     int sms = 0;
     cudaError_t e = current_device_sm_count(&sms);
     if (e != cudaSuccess) return e;
-    const uint32_t chunks = bwd_chunks(a.t.rows, a.t.h, sms), rpg = rows_per_gate(a.t);
-    const Workspace w = bwd_workspace(a.t.rows, a.t.h, a.t.gate_rows, chunks);
+    const BwdPlan p = bwd_plan(a.t.rows, a.t.h, a.t.gate_rows, sms);
+    const uint32_t rpg = rows_per_gate(a.t);
     uint8_t *ws = static_cast<uint8_t *>(a.workspace);
-    RowStats *stats = reinterpret_cast<RowStats *>(ws + w.stats);
-    const Parts parts = {reinterpret_cast<float *>(ws + w.post), reinterpret_cast<float *>(ws + w.pre),
-                         reinterpret_cast<float *>(ws + w.scale), reinterpret_cast<float *>(ws + w.gate),
-                         reinterpret_cast<double *>(ws + w.one), chunks};
-    int64_t grid = static_cast<int64_t>(sms) * 8;
-    if (grid > a.t.rows) grid = a.t.rows;
-    const dim3 cols(col_blocks(a.t.h), chunks);
-    // gates whose rows lie in several chunks exist only where a gate has several rows
-    const dim3 red(static_cast<unsigned>((a.t.h / 4 + 31) / 32), 3 + (a.dgate && rpg > 1 ? chunks - 1 : 0u));
-    if (a.t.bf16) {
-        rms_residual_bwd_stats_kernel<true><<<static_cast<unsigned>(grid), 256, 0, stream>>>(a, stats, rpg);
-        rms_residual_bwd_cols_kernel<true><<<cols, kColThreads, 0, stream>>>(a, stats, parts, rpg);
-        rms_residual_bwd_reduce_kernel<true><<<red, 1024, 0, stream>>>(a, parts, rpg, chunks * cols.x);
+    RmsResidualParts parts = {reinterpret_cast<float *>(ws + p.post), reinterpret_cast<float *>(ws + p.pre),
+                              reinterpret_cast<float *>(ws + p.scale), reinterpret_cast<float *>(ws + p.gate),
+                              reinterpret_cast<double *>(ws + p.one), p.workers, p.n_one};
+    if (p.staged) {
+        e = rmsnorm_residual_staged_bwd(a, parts, stream);
+        if (e != cudaSuccess) return e;
     } else {
-        rms_residual_bwd_stats_kernel<false><<<static_cast<unsigned>(grid), 256, 0, stream>>>(a, stats, rpg);
-        rms_residual_bwd_cols_kernel<false><<<cols, kColThreads, 0, stream>>>(a, stats, parts, rpg);
-        rms_residual_bwd_reduce_kernel<false><<<red, 1024, 0, stream>>>(a, parts, rpg, chunks * cols.x);
+        RowStats *stats = reinterpret_cast<RowStats *>(ws + p.stats);
+        int64_t grid = static_cast<int64_t>(sms) * 8;
+        if (grid > a.t.rows) grid = a.t.rows;
+        const dim3 cols(col_blocks(a.t.h), p.workers);
+        if (a.t.bf16) {
+            rms_residual_bwd_stats_kernel<true><<<static_cast<unsigned>(grid), 256, 0, stream>>>(a, stats, rpg);
+            rms_residual_bwd_cols_kernel<true><<<cols, kColThreads, 0, stream>>>(a, stats, parts, rpg);
+        } else {
+            rms_residual_bwd_stats_kernel<false><<<static_cast<unsigned>(grid), 256, 0, stream>>>(a, stats, rpg);
+            rms_residual_bwd_cols_kernel<false><<<cols, kColThreads, 0, stream>>>(a, stats, parts, rpg);
+        }
+        if ((e = cudaGetLastError()) != cudaSuccess) return e;
     }
-    return cudaGetLastError();
+    // gates whose rows lie in several runs exist only where a gate has several rows; there are at most as many of them
+    // as gates, and as borders between runs
+    uint32_t shared = 0;
+    bool by_run = false;
+    if (a.dgate && rpg > 1) {
+        by_run = a.t.gate_rows > static_cast<int64_t>(p.workers) - 1;
+        shared = by_run ? p.workers - 1 : static_cast<uint32_t>(a.t.gate_rows);
+    }
+    if (!(a.dgamma_post || a.dgamma_pre || a.dres_scale || shared)) return cudaSuccess;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>((a.t.h / 4 + 31) / 32), 3 + shared, 1);
+    cfg.blockDim = dim3(1024, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, a.t.bf16 ? rms_residual_bwd_reduce_kernel<true> : rms_residual_bwd_reduce_kernel<false>,
+                              a, parts, rpg, by_run);
 }
 
 }  // namespace pg

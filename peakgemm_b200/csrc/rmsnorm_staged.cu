@@ -28,6 +28,7 @@
 
 #include "host_util.h"
 #include "ptx.cuh"
+#include "rms_vec.cuh"
 #include "rmsnorm.h"
 
 namespace pg {
@@ -88,32 +89,6 @@ __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, const Wa
             }
         }
     }
-}
-
-// 1-D bulk copy global -> shared; both addresses 16-byte aligned, bytes % 16 == 0.
-__device__ __forceinline__ void bulk_load(uint32_t dst_smem, const void *src, uint32_t bytes, uint32_t bar,
-                                          uint64_t policy) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint "
-                 "[%0], [%1], %2, [%3], %4;"
-                 ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar), "l"(policy)
-                 : "memory");
-}
-
-// Named barrier `id` over `nthreads` consumer threads that also ORs a predicate across
-// them, so that "somebody abandoned a wait" is decided identically by the whole group.
-__device__ __forceinline__ bool group_barrier_or(uint32_t id, uint32_t nthreads, bool pred) {
-    uint32_t r;
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p, q;\n\t"
-        "setp.ne.u32 q, %1, 0;\n\t"
-        "bar.red.or.pred p, %2, %3, q;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t"
-        "}\n"
-        : "=r"(r)
-        : "r"(static_cast<uint32_t>(pred)), "r"(id), "r"(nthreads)
-        : "memory");
-    return r != 0;
 }
 
 template <bool BF16>
@@ -548,6 +523,8 @@ cudaError_t launch_any(void *out, float *partial, const void *x, const void *dy,
 }
 
 }  // namespace
+
+cudaError_t rmsnorm_device(int *sms, int **status) { return device_setup(sms, status); }
 
 bool rmsnorm_staged_supported(int64_t h, bool bwd) {
     // Benchmark override (builds with PG_ENABLE_TUNING only), read once: PEAKGEMM_TUNE_RMS_STAGED=0 falls back to

@@ -251,12 +251,14 @@ void gemm_peak_lora(Tensor &d, const Tensor &a, const Tensor &b, const Tensor &l
 void *opt_ptr(const OptTensor &t) { return t ? t->data_ptr() : nullptr; }
 float *opt_f32(const OptTensor &t) { return t ? t->data_ptr<float>() : nullptr; }
 
-// `t`, where given, is a dense tensor of `type` with `numel` elements on like's device.
-void check_opt(const OptTensor &t, const Tensor &like, at::ScalarType type, int64_t numel, const char *op, const char *what) {
-    if (!t) return;
-    TORCH_CHECK(t->is_cuda() && t->device() == like.device(), op, ": ", what, " must be on the other tensors' CUDA device");
-    TORCH_CHECK(t->is_contiguous() && t->scalar_type() == type && t->numel() == numel, op, ": ", what,
-                " must be contiguous, of type ", type, " and have ", numel, " elements");
+// `t`, where given, is a dense tensor of `type` and shape `sizes` on like's device.
+void check_tensor(const Tensor &t, const Tensor &like, at::ScalarType type, at::IntArrayRef sizes, const char *op, const char *what) {
+    TORCH_CHECK(t.is_cuda() && t.device() == like.device(), op, ": ", what, " must be on the other tensors' CUDA device");
+    TORCH_CHECK(t.is_contiguous() && t.scalar_type() == type && t.sizes() == sizes, op, ": ", what,
+                " must be contiguous, of type ", type, " and shape ", sizes);
+}
+void check_opt(const OptTensor &t, const Tensor &like, at::ScalarType type, at::IntArrayRef sizes, const char *op, const char *what) {
+    if (t) check_tensor(*t, like, type, sizes, op, what);
 }
 
 struct ResidualTerms {
@@ -272,18 +274,18 @@ ResidualTerms check_residual_terms(const Tensor &u, const OptTensor &gamma_post,
     t.dtype = dtype_code(u, op);
     t.h = u.size(-1);
     t.rows = t.h > 0 ? u.numel() / t.h : 0;
-    check_opt(gamma_post, u, at::kFloat, t.h, op, "gamma_post");
-    check_opt(gamma_pre, u, at::kFloat, t.h, op, "gamma_pre");
+    check_opt(gamma_post, u, at::kFloat, {t.h}, op, "gamma_post");
+    check_opt(gamma_pre, u, at::kFloat, {t.h}, op, "gamma_pre");
     t.gate_rows = 0;
     if (gate) {
         TORCH_CHECK(gate->dim() >= 1 && gate->size(-1) == t.h, op, ": gate must be [..., h]");
         t.gate_rows = t.h > 0 ? gate->numel() / t.h : 0;
         TORCH_CHECK(t.gate_rows > 0 && t.rows % t.gate_rows == 0, op, ": the rows of gate must divide the rows of u");
-        check_opt(gate, u, u.scalar_type(), t.gate_rows * t.h, op, "gate");
+        check_tensor(*gate, u, u.scalar_type(), gate->sizes(), op, "gate");
     }
     t.res_scale_len = res_scale ? res_scale->numel() : 0;
     TORCH_CHECK(!res_scale || t.res_scale_len == 1 || t.res_scale_len == t.h, op, ": res_scale must have 1 or h elements");
-    check_opt(res_scale, u, at::kFloat, t.res_scale_len, op, "res_scale");
+    check_opt(res_scale, u, at::kFloat, {t.res_scale_len}, op, "res_scale");
     return t;
 }
 
@@ -293,9 +295,9 @@ void rms_norm_residual_fwd(Tensor &s, const OptTensor &y, const Tensor &u, const
     const char *op = "rms_norm_residual_fwd";
     const ResidualTerms t = check_residual_terms(u, gamma_post, gate, res_scale, gamma_pre, op);
     TORCH_CHECK(y.has_value() == gamma_pre.has_value(), op, ": y and gamma_pre come together");
-    check_opt(s, u, u.scalar_type(), u.numel(), op, "s");
-    check_opt(y, u, u.scalar_type(), u.numel(), op, "y");
-    check_opt(residual, u, u.scalar_type(), u.numel(), op, "residual");
+    check_tensor(s, u, u.scalar_type(), u.sizes(), op, "s");
+    check_opt(y, u, u.scalar_type(), u.sizes(), op, "y");
+    check_tensor(residual, u, u.scalar_type(), u.sizes(), op, "residual");
     c10::DeviceGuard device_guard(u.device());
     auto stream = at::cuda::getCurrentCUDAStream();
     check_status(pg_rmsnorm_residual_fwd(s.data_ptr(), opt_ptr(y), u.data_ptr(), residual.data_ptr(), opt_f32(gamma_post),
@@ -313,7 +315,7 @@ void rms_norm_residual_bwd(Tensor &du, Tensor &dresidual, const OptTensor &dgamm
     const char *op = "rms_norm_residual_bwd";
     const ResidualTerms t = check_residual_terms(du, gamma_post, gate, res_scale, gamma_pre, op);
     const at::ScalarType type = du.scalar_type();
-    const int64_t n = du.numel();
+    const at::IntArrayRef n = du.sizes();
     TORCH_CHECK(dy.has_value() == gamma_pre.has_value(), op, ": dy and gamma_pre come together");
     TORCH_CHECK(dy || ds, op, ": at least one of dy and ds is needed");
     TORCH_CHECK(s || !gamma_pre, op, ": gamma_pre needs s");
@@ -321,16 +323,16 @@ void rms_norm_residual_bwd(Tensor &du, Tensor &dresidual, const OptTensor &dgamm
     TORCH_CHECK(residual || !dres_scale, op, ": dres_scale needs residual");
     TORCH_CHECK((gamma_post || !dgamma_post) && (gate || !dgate) && (res_scale || !dres_scale) && (gamma_pre || !dgamma_pre),
                 op, ": a gradient needs the tensor it is the gradient of");
-    check_opt(dresidual, du, type, n, op, "dresidual");
+    check_tensor(dresidual, du, type, n, op, "dresidual");
     check_opt(dy, du, type, n, op, "dy");
     check_opt(ds, du, type, n, op, "ds");
     check_opt(s, du, type, n, op, "s");
     check_opt(u, du, type, n, op, "u");
     check_opt(residual, du, type, n, op, "residual");
-    check_opt(dgamma_post, du, at::kFloat, t.h, op, "dgamma_post");
-    check_opt(dgamma_pre, du, at::kFloat, t.h, op, "dgamma_pre");
-    check_opt(dgate, du, type, t.gate_rows * t.h, op, "dgate");
-    check_opt(dres_scale, du, at::kFloat, t.res_scale_len, op, "dres_scale");
+    check_opt(dgamma_post, du, at::kFloat, {t.h}, op, "dgamma_post");
+    check_opt(dgamma_pre, du, at::kFloat, {t.h}, op, "dgamma_pre");
+    if (dgate) check_tensor(*dgate, du, type, gate->sizes(), op, "dgate");
+    check_opt(dres_scale, du, at::kFloat, {t.res_scale_len}, op, "dres_scale");
     c10::DeviceGuard device_guard(du.device());
     auto stream = at::cuda::getCurrentCUDAStream();
     const size_t ws_bytes = pg_rmsnorm_residual_bwd_workspace_bytes(t.rows, t.h, t.gate_rows);

@@ -48,10 +48,8 @@ def test_operator_refuses_and_traces():
     good = [bf(4, 16), bf(4, 8), bf(16, 8), bf(2, 8, 8), bf(2, 16, 8), torch.zeros(4, dtype=torch.int32)]
     with pytest.raises((RuntimeError, NotImplementedError)):
         PeakGemm.gemm_peak_lora(*good)                                                   # no CPU path
-    for i, t in ((0, bf(5, 16)), (2, bf(16, 16)), (3, bf(2, 8, 16)), (4, bf(2, 16, 16)), (4, bf(3, 16, 8)),
-                 (5, torch.zeros(3, dtype=torch.int32)), (1, torch.zeros(4, 8))):
-        with pytest.raises(AssertionError):
-            PeakGemm.gemm_peak_lora(*good[:i], t, *good[i + 1:])
+    with pytest.raises(AssertionError):
+        PeakGemm.gemm_peak_lora(good[0], torch.zeros(4, 8), *good[2:])                   # float32
     with FakeTensorMode():
         e = lambda *s, **kw: torch.empty(*s, device="cuda", **kw)      # noqa: E731
         f = dict(dtype=torch.bfloat16)

@@ -161,6 +161,26 @@ def test_same_bits_on_every_call(cuda, m):
         assert torch.equal(call(x), first)
 
 
+def test_operator_refuses(cuda):
+    import PeakGemm
+
+    x = make(4, 16, 8, 2, 8, BF16, 130)
+    good = [torch.empty(4, 16, dtype=BF16, device="cuda"), *(x[key] for key in ("a", "b", "lora_a", "lora_b", "ids"))]
+    PeakGemm.gemm_peak_lora(*good)
+    bf = lambda *s: torch.zeros(*s, dtype=BF16, device="cuda")      # noqa: E731
+    for i, t in ((0, bf(5, 16)), (0, bf(4, 24)), (2, bf(16, 16)), (3, bf(2, 8, 16)), (3, x["lora_a"].half()), (4, bf(2, 16, 16)),
+                 (4, bf(3, 16, 8)), (4, x["lora_b"].cpu()), (4, bf(2, 8, 16).mT), (5, x["ids"][:3]), (5, x["ids"].long())):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            PeakGemm.gemm_peak_lora(*good[:i], t, *good[i + 1:])
+    for kw in (dict(scale=x["scale"][:1]), dict(scale=x["scale"].double()), dict(row_scale=x["scale"]), dict(bias=bf(8)),
+               dict(residual=bf(4, 8))):
+        with pytest.raises(RuntimeError):
+            PeakGemm.gemm_peak_lora(*good, **kw)
+    with pytest.raises(RuntimeError, match="UNSUPPORTED"):
+        PeakGemm.gemm_peak_lora(*good[:3], bf(2, 12, 8), bf(2, 16, 12), x["ids"])             # rank % 8
+    torch.cuda.synchronize()
+
+
 def test_no_rows_no_adapters(cuda):
     import PeakGemm
 

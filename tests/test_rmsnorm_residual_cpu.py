@@ -70,10 +70,6 @@ def test_operators_refuse_and_trace():
         PeakGemm.rms_norm_residual_fwd(x, None, x, x, gamma_pre=g)                   # gamma_pre without y
     with pytest.raises(AssertionError):
         PeakGemm.rms_norm_residual_fwd(x.float(), None, x.float(), x.float())
-    with pytest.raises(AssertionError):
-        PeakGemm.rms_norm_residual_fwd(x, None, x, x[:2])
-    with pytest.raises(AssertionError):
-        PeakGemm.rms_norm_residual_bwd(x, x, None, x, x, x, dgate=x)                 # a gradient of nothing
     with FakeTensorMode():
         x, g = torch.empty(4, 8, 64, dtype=torch.bfloat16, device="cuda"), torch.empty(64, device="cuda")
         PeakGemm.rms_norm_residual_fwd(x.clone(), x.clone(), x, x, gamma_post=g, gamma_pre=g)

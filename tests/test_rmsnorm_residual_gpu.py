@@ -190,6 +190,36 @@ def test_no_rows(cuda):
     assert (a == 0).all() and (b == 0).all() and (c == 0).all()
 
 
+def test_operators_refuse(cuda):
+    import PeakGemm
+
+    x = make(6, 64, BF16, 75, gates=3, res_scale=64)
+    u, p = x["u"], params(x)
+    new = lambda: torch.empty_like(u)      # noqa: E731
+    f = dict(s=new(), y=new(), u=u, residual=x["residual"])
+    PeakGemm.rms_norm_residual_fwd(**f, **p)
+    for key, t in (("s", u[:5]), ("s", u.half()), ("residual", u.view(2, 3, 64)), ("residual", u.cpu()), ("y", u[:, :32]),
+                   ("gamma_post", p["gamma_post"][:32]), ("gamma_post", p["gamma_post"].to(BF16)), ("gate", u[:4]),
+                   ("gate", x["gate"].half()), ("gate", x["gate"][:, :32]), ("res_scale", p["gamma_post"][:8]),
+                   ("res_scale", x["res_scale"].view(1, 64)), ("gamma_pre", p["gamma_pre"].cpu())):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            PeakGemm.rms_norm_residual_fwd(**{**f, **p, key: t})
+    with pytest.raises(AssertionError):
+        PeakGemm.rms_norm_residual_fwd(**{**f, **p, "y": None})
+    g = dict(du=new(), dresidual=new(), dy=x["dy"], ds=x["ds"], s=f["s"], u=u, residual=x["residual"], dgate=x["gate"].clone())
+    PeakGemm.rms_norm_residual_bwd(**g, **p)
+    for key, t in (("du", u.float()), ("dresidual", u[:5]), ("dy", None), ("s", None), ("u", None), ("dgate", u[:1]),
+                   ("gate", None), ("dgamma_post", p["gamma_post"][:8]), ("dres_scale", p["gamma_post"][:1]),
+                   ("dgamma_pre", p["gamma_pre"].to(BF16)), ("ds", u.t())):
+        with pytest.raises((RuntimeError, NotImplementedError, AssertionError)):
+            PeakGemm.rms_norm_residual_bwd(**{**g, **p, key: t})
+    with pytest.raises(RuntimeError):
+        PeakGemm.rms_norm_residual_bwd(new(), new(), None, None, f["s"], u)                  # nothing comes in
+    with pytest.raises(RuntimeError):
+        PeakGemm.rms_norm_residual_bwd(new(), new(), None, x["ds"], f["s"], u, dgate=u)      # the gradient of nothing
+    torch.cuda.synchronize()
+
+
 def test_only_the_wanted_gradients(cuda):
     """ds or dy missing, sums not asked for, inputs that are then not needed."""
     import PeakGemm
