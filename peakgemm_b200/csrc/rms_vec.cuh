@@ -27,16 +27,57 @@ __host__ __device__ __forceinline__ uint32_t rms_run_begin(uint32_t c, uint32_t 
     return static_cast<uint32_t>(static_cast<uint64_t>(c) * rows / n);
 }
 
+// Two fp32 values in one register pair: the packed instructions issue half as often, which is what bounds the kernels
+// that do much arithmetic per byte (rmsnorm_residual_staged.cu).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long &>(d))
+        : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)),
+          "l"(reinterpret_cast<const unsigned long long &>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long &>(d))
+        : "l"(reinterpret_cast<const unsigned long long &>(a)), "l"(reinterpret_cast<const unsigned long long &>(b)));
+    return d;
+}
+template <bool BF16>
+__device__ __forceinline__ void vec_unpack2(const uint4 &v, float2 (&f)[4]) {
+    ptx::unpack2<BF16>(v.x, f[0].x, f[0].y);
+    ptx::unpack2<BF16>(v.y, f[1].x, f[1].y);
+    ptx::unpack2<BF16>(v.z, f[2].x, f[2].y);
+    ptx::unpack2<BF16>(v.w, f[3].x, f[3].y);
+}
+template <bool BF16>
+__device__ __forceinline__ uint4 vec_pack2(const float2 (&f)[4]) {
+    return make_uint4(ptx::pack2<BF16>(f[0].x, f[0].y), ptx::pack2<BF16>(f[1].x, f[1].y),
+                      ptx::pack2<BF16>(f[2].x, f[2].y), ptx::pack2<BF16>(f[3].x, f[3].y));
+}
+// Eight fp32 values from shared memory (address `s`) or from global memory (`g`).
+__device__ __forceinline__ void vec_load2(bool shared, uint32_t s, const float *g, float2 (&f)[4]) {
+    if (shared) {
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0].x), "=f"(f[0].y), "=f"(f[1].x), "=f"(f[1].y) : "r"(s));
+        asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[2].x), "=f"(f[2].y), "=f"(f[3].x), "=f"(f[3].y) : "r"(s + 16));
+    } else {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(g)), b = __ldg(reinterpret_cast<const float4 *>(g) + 1);
+        f[0] = make_float2(a.x, a.y);
+        f[1] = make_float2(a.z, a.w);
+        f[2] = make_float2(b.x, b.y);
+        f[3] = make_float2(b.z, b.w);
+    }
+}
+__device__ __forceinline__ void vec_store2(float *p, const float2 (&f)[4]) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(f[2].x, f[2].y, f[3].x, f[3].y);
+}
+
 // Eight consecutive fp32 values, 16-byte aligned.
 __device__ __forceinline__ void vec_load_f32(const float *p, float (&f)[8]) {
     const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
     const float4 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-}
-// The same from global or shared memory.
-__device__ __forceinline__ void vec_load_f32_any(const float *p, float (&f)[8]) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
     f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
     f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
 }

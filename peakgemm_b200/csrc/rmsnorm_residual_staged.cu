@@ -64,7 +64,9 @@ Group make_group(int64_t rows, int64_t h, int sms) {
 
 template <int VPT> constexpr int max_threads() { return VPT == 1 ? 640 : 512; }
 
-template <int VPT, bool BF16, bool SCALE_COL>
+// Which terms a call has, where the kernel is compiled for them: gate 0 none, 1 one for several rows, 2 one for each row;
+// a res_scale per column or not; FULL: dy, ds and gamma_post are all there.  GATE 3: whatever the call has.
+template <int VPT, bool BF16, int GATE, bool SCALE_COL, bool FULL>
 __global__ void __launch_bounds__(max_threads<VPT>(), 1)
 rms_residual_bwd_staged_kernel(const RmsResidualBwdArgs a, const RmsResidualParts parts, const StagedPlan p,
                                uint32_t rows_per_gate, int *status) {
@@ -86,297 +88,296 @@ rms_residual_bwd_staged_kernel(const RmsResidualBwdArgs a, const RmsResidualPart
         fence_mbar_init();
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const float *gamma_pre = a.t.gamma_pre, *gamma_post = a.t.gamma_post;
+    const bool has_dy = FULL || a.dy, has_ds = FULL || a.ds, has_post = FULL || a.t.gamma_post;
     if (p.gamma_smem) {
         float *d = reinterpret_cast<float *>(smem);
         for (int i = threadIdx.x; i < h / 4; i += blockDim.x) {
-            if (gamma_pre) reinterpret_cast<float4 *>(d)[i] = __ldg(reinterpret_cast<const float4 *>(gamma_pre) + i);
-            if (gamma_post) reinterpret_cast<float4 *>(d + h)[i] = __ldg(reinterpret_cast<const float4 *>(gamma_post) + i);
+            if (has_dy) reinterpret_cast<float4 *>(d)[i] = __ldg(reinterpret_cast<const float4 *>(a.t.gamma_pre) + i);
+            if (has_post) reinterpret_cast<float4 *>(d + h)[i] = __ldg(reinterpret_cast<const float4 *>(a.t.gamma_post) + i);
         }
-        if (gamma_pre) gamma_pre = d;
-        if (gamma_post) gamma_post = d + h;
     }
     __syncthreads();
-    {
-        const int g = threadIdx.x / p.T, t = threadIdx.x - g * p.T;
-        const uint32_t worker = blockIdx.x * p.G + g;
-        const uint32_t r0 = rms_run_begin(worker, parts.workers, rows), r1 = rms_run_begin(worker + 1, parts.workers, rows);
-        float4 *red = reinterpret_cast<float4 *>(smem + p.off_red) + g * 4 * group_warps;       // [parity][A, B][warps]
-        // one thread: the copies of `row` into the group's ring place `at`
-        const auto issue = [&](uint32_t row, int at) {
-            const int slot = at * p.G + g;
-            const uint64_t pol = l2_policy_evict_first();              // every row is read once
-            const void *src[kOperands] = {a.dy, a.s, a.ds, a.u, a.residual, a.t.gate};
-            mbar_arrive_expect_tx(bar_full + slot * 8, p.slot_bytes);
-#pragma unroll
-            for (int o = 0; o < kOperands; ++o)
-                if (p.place[o] >= 0)
-                    bulk_load(sbase + p.off_slot + slot * p.slot_bytes + p.place[o] * p.row_bytes,
-                              static_cast<const uint4 *>(src[o]) + static_cast<int64_t>(row) * h8, p.row_bytes,
-                              bar_full + slot * 8, pol);
-        };
-        if (t == 0)
-            for (int i = 0; i < per_group && r0 + i < r1; ++i) issue(r0 + i, i);
-        const bool token_gate = p.place[kGate] >= 0, group_gate = a.t.gate && !token_gate;
-        const bool needs_u = a.t.gamma_post || a.dgate;
-        const float scale_one = a.t.res_scale && a.t.res_scale_one ? __ldg(a.t.res_scale) : 1.f;
+    const auto gamma_pre = [&](int idx, float2 (&f)[4]) {
+        vec_load2(p.gamma_smem, sbase + 32 * idx, a.t.gamma_pre + 8 * idx, f);
+    };
+    const auto gamma_post = [&](int idx, float2 (&f)[4]) {
+        vec_load2(p.gamma_smem, sbase + 4 * h + 32 * idx, a.t.gamma_post + 8 * idx, f);
+    };
 
-        float q[VPT][8], pre[VPT][8], scale[SCALE_COL ? VPT : 1][8];
-        uint4 gate[VPT];
-        double one = 0.0;
+    const int g = threadIdx.x / p.T, t = threadIdx.x - g * p.T;
+    const uint32_t worker = blockIdx.x * p.G + g;
+    const uint32_t r0 = rms_run_begin(worker, parts.workers, rows), r1 = rms_run_begin(worker + 1, parts.workers, rows);
+    float4 *red = reinterpret_cast<float4 *>(smem + p.off_red) + g * 4 * group_warps;       // [parity][A, B][warps]
+    // one thread: the copies of `row` into the group's ring place `at`
+    const auto issue = [&](uint32_t row, int at) {
+        const int slot = at * p.G + g;
+        const uint64_t pol = l2_policy_evict_first();              // every row is read once
+        const void *src[kOperands] = {a.dy, a.s, a.ds, a.u, a.residual, a.t.gate};
+        mbar_arrive_expect_tx(bar_full + slot * 8, p.slot_bytes);
+#pragma unroll
+        for (int o = 0; o < kOperands; ++o)
+            if (p.place[o] >= 0)
+                bulk_load(sbase + p.off_slot + slot * p.slot_bytes + p.place[o] * p.row_bytes,
+                          static_cast<const uint4 *>(src[o]) + static_cast<int64_t>(row) * h8, p.row_bytes,
+                          bar_full + slot * 8, pol);
+    };
+    if (t == 0)
+        for (int i = 0; i < per_group && r0 + i < r1; ++i) issue(r0 + i, i);
+
+    const bool token_gate = GATE == 2 || (GATE == 3 && p.place[kGate] >= 0);
+    const bool group_gate = GATE == 1 || (GATE == 3 && a.t.gate && !token_gate);
+    const bool needs_u = FULL || a.t.gamma_post || a.dgate;
+    const float one_scale = a.t.res_scale && a.t.res_scale_one ? __ldg(a.t.res_scale) : 1.f;
+    const float2 scale_one = make_float2(one_scale, one_scale), zero = make_float2(0.f, 0.f);
+
+    float2 q[VPT][4], pre[VPT][4], scale[SCALE_COL ? VPT : 1][4];
+    uint4 gate[VPT];
+    double one = 0.0;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        gate[j] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            q[j][e] = pre[j][e] = zero;
+            if constexpr (SCALE_COL) scale[j][e] = zero;
+        }
+    }
+    uint32_t gi = group_gate ? r0 / rows_per_gate : 0u;
+    uint32_t gate_end = group_gate ? (gi + 1) * rows_per_gate : rows;
+    bool fresh_gate = group_gate, first_flush = true;
+    int ring = 0;
+    uint32_t phase = 0, parity = 0;
+    for (uint32_t row = r0; row < r1; ++row, parity ^= 1u) {
+        if (fresh_gate) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int idx = t + p.T * j;
+                if (idx < h8) gate[j] = __ldg(static_cast<const uint4 *>(a.t.gate) + static_cast<int64_t>(gi) * h8 + idx);
+            }
+            fresh_gate = false;
+        }
+        const int slot = ring * p.G + g;
+        bool ok = wait_bar(bar_full + slot * 8, phase, ctx, kStRmsConsumer);
+        ok = __all_sync(0xffffffffu, ok);
+        const uint8_t *base = smem + p.off_slot + slot * p.slot_bytes;
+        const auto operand = [&](int o, int idx) {
+            return reinterpret_cast<const uint4 *>(base + p.place[o] * p.row_bytes)[idx];
+        };
+        // A: sums over the row
+        uint4 dyv[VPT], sv[VPT], uv[VPT];
+        float2 ss2 = zero, ws2 = zero, uu2 = zero;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            gate[j] = make_uint4(0, 0, 0, 0);
+            const int idx = t + p.T * j;
+            dyv[j] = sv[j] = uv[j] = make_uint4(0, 0, 0, 0);
+            if (ok && idx < h8) {
+                if (has_dy) {
+                    dyv[j] = operand(kDy, idx);
+                    sv[j] = operand(kS, idx);
+                    float2 s[4], d[4], gm[4];
+                    vec_unpack2<BF16>(sv[j], s);
+                    vec_unpack2<BF16>(dyv[j], d);
+                    gamma_pre(idx, gm);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                q[j][e] = pre[j][e] = 0.f;
-                if constexpr (SCALE_COL) scale[j][e] = 0.f;
+                    for (int e = 0; e < 4; ++e) {
+                        ss2 = fma2(s[e], s[e], ss2);
+                        ws2 = fma2(mul2(d[e], gm[e]), s[e], ws2);
+                    }
+                }
+                if (needs_u) {
+                    uv[j] = operand(kU, idx);
+                    float2 u[4];
+                    vec_unpack2<BF16>(uv[j], u);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) uu2 = fma2(u[e], u[e], uu2);
+                }
             }
         }
-        uint32_t gi = group_gate ? r0 / rows_per_gate : 0u;
-        uint32_t gate_end = group_gate ? (gi + 1) * rows_per_gate : rows;
-        bool fresh_gate = group_gate, first_flush = true;
-        int ring = 0;
-        uint32_t phase = 0, parity = 0;
-        for (uint32_t row = r0; row < r1; ++row, parity ^= 1u) {
-            if (fresh_gate) {
+        float ss = warp_sum_f32(ss2.x + ss2.y), ws = warp_sum_f32(ws2.x + ws2.y), uu = warp_sum_f32(uu2.x + uu2.y);
+        float4 *ra = red + parity * 2 * group_warps;
+        if (lane == 0) ra[warp - g * group_warps] = make_float4(ss, ws, uu, 0.f);
+        if (group_barrier_or(1 + g, p.T, !ok || *abort_flag != 0)) break;
+        ss = ws = uu = 0.f;
+        for (int w = 0; w < group_warps; ++w) {
+            const float4 v = ra[w];
+            ss += v.x;
+            ws += v.y;
+            uu += v.z;
+        }
+        // rsqrt.approx is within 2 ulp of fp32; the gradients are rounded to 16 bits or bounded by 2^-17
+        const float rs = rsqrtf(fmaf(ss, inv_h, a.t.eps)), ru = has_post ? rsqrtf(fmaf(uu, inv_h, a.t.eps)) : 1.f;
+        const float ms = -(ws * inv_h * rs * (rs * rs));
+        const float2 rs2 = make_float2(rs, rs), ms2 = make_float2(ms, ms), ru2 = make_float2(ru, ru);
+        // B: D and all that needs no further sum.  v = rstd(u) * e * gamma_post, so that du = v - rstd(u)^2 mean(v u) u.
+        float2 v[VPT][4], eu2 = zero, part = zero;
 #pragma unroll
-                for (int j = 0; j < VPT; ++j) {
-                    const int idx = t + p.T * j;
-                    if (idx < h8) gate[j] = __ldg(static_cast<const uint4 *>(a.t.gate) + static_cast<int64_t>(gi) * h8 + idx);
+        for (int j = 0; j < VPT; ++j) {
+            const int idx = t + p.T * j;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j][e] = zero;
+            if (idx < h8) {
+                float2 D[4], f[4], x[4];
+                const int64_t at = static_cast<int64_t>(row) * h8 + idx;
+                if (has_ds) {
+                    vec_unpack2<BF16>(operand(kDs, idx), D);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) D[e] = zero;
                 }
-                fresh_gate = false;
-            }
-            const int slot = ring * p.G + g;
-            bool ok = wait_bar(bar_full + slot * 8, phase, ctx, kStRmsConsumer);
-            ok = __all_sync(0xffffffffu, ok);
-            const uint8_t *base = smem + p.off_slot + slot * p.slot_bytes;
-            const auto operand = [&](int o, int idx) {
-                return reinterpret_cast<const uint4 *>(base + p.place[o] * p.row_bytes)[idx];
-            };
-            // A: sums over the row
-            uint4 dyv[VPT], sv[VPT], uv[VPT];
-            float ss = 0.f, ws = 0.f, uu = 0.f;
+                if (has_dy) {
+                    float2 gm[4];
+                    vec_unpack2<BF16>(dyv[j], x);
+                    vec_unpack2<BF16>(sv[j], f);
+                    gamma_pre(idx, gm);
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                const int idx = t + p.T * j;
-                dyv[j] = sv[j] = uv[j] = make_uint4(0, 0, 0, 0);
-                if (ok && idx < h8) {
-                    if (a.dy) {
-                        dyv[j] = operand(kDy, idx);
-                        sv[j] = operand(kS, idx);
-                        float s[8], d[8], gm[8];
-                        vec_unpack<BF16>(sv[j], s);
-                        vec_unpack<BF16>(dyv[j], d);
-                        vec_load_f32_any(gamma_pre + 8 * idx, gm);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            ss = fmaf(s[e], s[e], ss);
-                            ws = fmaf(d[e] * gm[e], s[e], ws);
-                        }
-                    }
-                    if (needs_u) {
-                        uv[j] = operand(kU, idx);
-                        float u[8];
-                        vec_unpack<BF16>(uv[j], u);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) uu = fmaf(u[e], u[e], uu);
+                    for (int e = 0; e < 4; ++e) {
+                        x[e] = mul2(x[e], rs2);
+                        pre[j][e] = fma2(x[e], f[e], pre[j][e]);
+                        D[e] = fma2(ms2, f[e], fma2(x[e], gm[e], D[e]));
                     }
                 }
-            }
-            float rstd_s = 0.f, ms = 0.f, rstd_u = 1.f;
-            {
-                ss = warp_sum_f32(ss);
-                ws = warp_sum_f32(ws);
-                uu = warp_sum_f32(uu);
-                float4 *ra = red + parity * 2 * group_warps;
-                if (lane == 0) ra[warp - g * group_warps] = make_float4(ss, ws, uu, 0.f);
-                if (group_barrier_or(1 + g, p.T, !ok || *abort_flag != 0)) break;
-                ss = ws = uu = 0.f;
-                for (int w = 0; w < group_warps; ++w) {
-                    const float4 v = ra[w];
-                    ss += v.x;
-                    ws += v.y;
-                    uu += v.z;
-                }
-                // rsqrt.approx is within 2 ulp of fp32; the gradients are rounded to 16 bits or bounded by 2^-17
-                rstd_s = rsqrtf(fmaf(ss, inv_h, a.t.eps));
-                ms = ws * inv_h * rstd_s * (rstd_s * rstd_s);
-                if (a.t.gamma_post) rstd_u = rsqrtf(fmaf(uu, inv_h, a.t.eps));
-            }
-            // B: D and all that needs no further sum
-            float v[VPT][8], eu = 0.f, part = 0.f;
+                if (a.dres_scale) {
+                    vec_unpack2<BF16>(operand(kRes, idx), f);
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                const int idx = t + p.T * j;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[j][e] = 0.f;
-                if (idx < h8) {
-                    float D[8], f[8], x[8];
-                    const int64_t at = static_cast<int64_t>(row) * h8 + idx;
-                    if (a.ds) {
-                        vec_unpack<BF16>(operand(kDs, idx), D);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) D[e] = 0.f;
-                    }
-                    if (a.dy) {
-                        float gm[8];
-                        vec_unpack<BF16>(dyv[j], x);
-                        vec_unpack<BF16>(sv[j], f);
-                        vec_load_f32_any(gamma_pre + 8 * idx, gm);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            D[e] += rstd_s * (x[e] * gm[e]) - ms * f[e];
-                            pre[j][e] = fmaf(x[e], f[e] * rstd_s, pre[j][e]);
-                        }
-                    }
-                    if (a.dres_scale) {
-                        vec_unpack<BF16>(operand(kRes, idx), f);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            if constexpr (SCALE_COL) scale[j][e] = fmaf(D[e], f[e], scale[j][e]);
-                            else part = fmaf(D[e], f[e], part);
-                        }
-                    }
-                    if constexpr (SCALE_COL) {
-                        vec_load_f32(a.t.res_scale + 8 * idx, x);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] *= D[e];
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = D[e] * scale_one;
-                    }
-                    __stcs(static_cast<uint4 *>(a.dresidual) + at, vec_pack<BF16>(x));
-                    vec_unpack<BF16>(uv[j], f);
-                    float gp[8];
-                    if (a.t.gamma_post) {
-                        vec_load_f32_any(gamma_post + 8 * idx, gp);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) gp[e] = 1.f;
-                    }
-                    if (token_gate) {
-                        vec_unpack<BF16>(operand(kGate, idx), x);
-                        if (a.dgate) {
-                            float dg[8];
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) dg[e] = D[e] * (f[e] * rstd_u) * gp[e];
-                            __stcs(static_cast<uint4 *>(a.dgate) + at, vec_pack<BF16>(dg));
-                        }
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            D[e] *= x[e];
-                            q[j][e] = fmaf(D[e], f[e] * rstd_u, q[j][e]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) q[j][e] = fmaf(D[e], f[e] * rstd_u, q[j][e]);
-                        if (group_gate) {
-                            vec_unpack<BF16>(gate[j], x);
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) D[e] *= x[e];
-                        }
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        v[j][e] = D[e] * gp[e];
-                        eu = fmaf(v[j][e], f[e], eu);
+                    for (int e = 0; e < 4; ++e) {
+                        if constexpr (SCALE_COL) scale[j][e] = fma2(D[e], f[e], scale[j][e]);
+                        else part = fma2(D[e], f[e], part);
                     }
                 }
-            }
-            if constexpr (!SCALE_COL) one += static_cast<double>(part);
-            // C: du
-            float mu = 0.f;
-            {
-                eu = warp_sum_f32(eu);
-                float *rb = reinterpret_cast<float *>(red + (parity * 2 + 1) * group_warps);
-                if (lane == 0) rb[warp - g * group_warps] = eu;
-                if (group_barrier_or(1 + g, p.T, *abort_flag != 0)) break;
-                // the whole group has the rest of the row in registers: its slot takes the next one
-                if (t == 0 && row + per_group < r1) issue(row + per_group, ring);
-                if (++ring == per_group) { ring = 0; phase ^= 1u; }
-                if (a.t.gamma_post) {
-                    eu = 0.f;
-                    for (int w = 0; w < group_warps; ++w) eu += rb[w];
-                    mu = eu * inv_h * rstd_u * (rstd_u * rstd_u);
+                if constexpr (SCALE_COL) {
+                    vec_load2(false, 0u, a.t.res_scale + 8 * idx, x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], D[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e] = mul2(D[e], scale_one);
                 }
-            }
+                __stcs(static_cast<uint4 *>(a.dresidual) + at, vec_pack2<BF16>(x));
+                vec_unpack2<BF16>(uv[j], f);
+                float2 gp[4];
+                if (has_post) gamma_post(idx, gp);
+                if (token_gate) {
+                    vec_unpack2<BF16>(operand(kGate, idx), x);
+                    if (a.dgate) {
+                        float2 dg[4];
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                const int idx = t + p.T * j;
-                if (idx < h8) {
-                    float u[8];
-                    vec_unpack<BF16>(uv[j], u);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) u[e] = rstd_u * v[j][e] - mu * u[e];
-                    __stcs(static_cast<uint4 *>(a.du) + static_cast<int64_t>(row) * h8 + idx, vec_pack<BF16>(u));
-                }
-            }
-            // the end of a gate's rows, or of the run
-            if (group_gate && (row + 1 == gate_end || row + 1 == r1)) {
-                const uint32_t g_first = gi * rows_per_gate;
-                const bool whole = g_first >= r0 && gate_end <= r1;
-#pragma unroll
-                for (int j = 0; j < VPT; ++j) {
-                    const int idx = t + p.T * j;
-                    if (idx < h8) {
-                        float x[8], o[8];
-                        vec_unpack<BF16>(gate[j], x);
-                        float *post = parts.post + static_cast<int64_t>(worker) * h + 8 * idx;
-                        if (a.dgamma_post) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) o[e] = (first_flush ? 0.f : post[e]) + x[e] * q[j][e];
-                            vec_store_f32(post, o);
+                        for (int e = 0; e < 4; ++e) {
+                            dg[e] = mul2(mul2(D[e], ru2), f[e]);
+                            if (has_post) dg[e] = mul2(dg[e], gp[e]);
                         }
-                        if (a.dgate) {
-#pragma unroll
-                            for (int e = 0; e < 8; ++e) o[e] = q[j][e];
-                            if (a.t.gamma_post) {
-                                vec_load_f32_any(gamma_post + 8 * idx, x);
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) o[e] *= x[e];
-                            }
-                            if (whole)
-                                static_cast<uint4 *>(a.dgate)[static_cast<int64_t>(gi) * h8 + idx] = vec_pack<BF16>(o);
-                            else
-                                vec_store_f32(parts.gate + (2 * static_cast<int64_t>(worker) + (g_first <= r0 ? 0 : 1)) * h + 8 * idx, o);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) q[j][e] = 0.f;
+                        __stcs(static_cast<uint4 *>(a.dgate) + at, vec_pack2<BF16>(dg));
                     }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) D[e] = mul2(D[e], x[e]);
                 }
-                first_flush = false;
-                ++gi;
-                gate_end += rows_per_gate;
-                fresh_gate = true;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    D[e] = mul2(D[e], ru2);
+                    q[j][e] = fma2(D[e], f[e], q[j][e]);
+                }
+                if (group_gate) {
+                    vec_unpack2<BF16>(gate[j], x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) D[e] = mul2(D[e], x[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[j][e] = has_post ? mul2(D[e], gp[e]) : D[e];
+                    eu2 = fma2(v[j][e], f[e], eu2);
+                }
             }
         }
-        const int64_t at = static_cast<int64_t>(worker) * h;
+        if constexpr (!SCALE_COL) one += static_cast<double>(part.x + part.y);
+        // C: du
+        float eu = warp_sum_f32(eu2.x + eu2.y);
+        float *rb = reinterpret_cast<float *>(red + (parity * 2 + 1) * group_warps);
+        if (lane == 0) rb[warp - g * group_warps] = eu;
+        if (group_barrier_or(1 + g, p.T, *abort_flag != 0)) break;
+        // the whole group has the rest of the row in registers: its slot takes the next one
+        if (t == 0 && row + per_group < r1) issue(row + per_group, ring);
+        if (++ring == per_group) { ring = 0; phase ^= 1u; }
+        float2 mu2 = zero;
+        if (has_post) {
+            eu = 0.f;
+            for (int w = 0; w < group_warps; ++w) eu += rb[w];
+            const float mu = -(eu * inv_h * ru * ru);
+            mu2 = make_float2(mu, mu);
+        }
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int idx = t + p.T * j;
             if (idx < h8) {
-                if (a.dgamma_post && !group_gate) vec_store_f32(parts.post + at + 8 * idx, q[j]);
-                if (a.dgamma_pre) vec_store_f32(parts.pre + at + 8 * idx, pre[j]);
-                if constexpr (SCALE_COL)
-                    if (a.dres_scale) vec_store_f32(parts.scale + at + 8 * idx, scale[j]);
+                float2 u[4];
+                vec_unpack2<BF16>(uv[j], u);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) u[e] = has_post ? fma2(mu2, u[e], v[j][e]) : v[j][e];
+                __stcs(static_cast<uint4 *>(a.du) + static_cast<int64_t>(row) * h8 + idx, vec_pack2<BF16>(u));
             }
         }
-        if constexpr (!SCALE_COL) {
-            if (a.dres_scale) {
+        // the end of a gate's rows, or of the run
+        if (group_gate && (row + 1 == gate_end || row + 1 == r1)) {
+            const uint32_t g_first = gi * rows_per_gate;
+            const bool whole = g_first >= r0 && gate_end <= r1;
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
-                // the row sums' buffers are free once the group has met again
-                group_barrier_or(1 + g, p.T, false);
-                double *rd = reinterpret_cast<double *>(red);
-                if (lane == 0) rd[warp - g * group_warps] = one;
-                group_barrier_or(1 + g, p.T, false);
-                if (t == 0) {
-                    double sum = 0.0;
-                    for (int w = 0; w < group_warps; ++w) sum += rd[w];
-                    parts.scale_one[worker] = sum;
+            for (int j = 0; j < VPT; ++j) {
+                const int idx = t + p.T * j;
+                if (idx < h8) {
+                    float2 x[4], o[4];
+                    float *post = parts.post + static_cast<int64_t>(worker) * h + 8 * idx;
+                    if (a.dgamma_post) {
+                        vec_unpack2<BF16>(gate[j], x);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            o[e] = fma2(x[e], q[j][e], first_flush ? zero : reinterpret_cast<const float2 *>(post)[e]);
+                        vec_store2(post, o);
+                    }
+                    if (a.dgate) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = q[j][e];
+                        if (has_post) {
+                            gamma_post(idx, x);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[e] = mul2(o[e], x[e]);
+                        }
+                        if (whole)
+                            static_cast<uint4 *>(a.dgate)[static_cast<int64_t>(gi) * h8 + idx] = vec_pack2<BF16>(o);
+                        else
+                            vec_store2(parts.gate + (2 * static_cast<int64_t>(worker) + (g_first <= r0 ? 0 : 1)) * h + 8 * idx, o);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) q[j][e] = zero;
                 }
+            }
+            first_flush = false;
+            ++gi;
+            gate_end += rows_per_gate;
+            fresh_gate = true;
+        }
+    }
+    const int64_t at = static_cast<int64_t>(worker) * h;
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int idx = t + p.T * j;
+        if (idx < h8) {
+            if (a.dgamma_post && !group_gate) vec_store2(parts.post + at + 8 * idx, q[j]);
+            if (a.dgamma_pre) vec_store2(parts.pre + at + 8 * idx, pre[j]);
+            if constexpr (SCALE_COL)
+                if (a.dres_scale) vec_store2(parts.scale + at + 8 * idx, scale[j]);
+        }
+    }
+    if constexpr (!SCALE_COL) {
+        if (a.dres_scale) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) one += __shfl_xor_sync(0xffffffffu, one, o);
+            // the row sums' buffers are free once the group has met again
+            group_barrier_or(1 + g, p.T, false);
+            double *rd = reinterpret_cast<double *>(red);
+            if (lane == 0) rd[warp - g * group_warps] = one;
+            group_barrier_or(1 + g, p.T, false);
+            if (t == 0) {
+                double sum = 0.0;
+                for (int w = 0; w < group_warps; ++w) sum += rd[w];
+                parts.scale_one[worker] = sum;
             }
         }
     }
@@ -413,10 +414,10 @@ StagedPlan make_staged_plan(const RmsResidualBwdArgs &a, int sms) {
     return p;
 }
 
-template <int VPT, bool BF16, bool SCALE_COL>
+template <int VPT, bool BF16, int GATE, bool SCALE_COL, bool FULL>
 cudaError_t launch_staged(const RmsResidualBwdArgs &a, const RmsResidualParts &parts, const StagedPlan &p, int *status,
                           cudaStream_t stream) {
-    auto kernel = rms_residual_bwd_staged_kernel<VPT, BF16, SCALE_COL>;
+    auto kernel = rms_residual_bwd_staged_kernel<VPT, BF16, GATE, SCALE_COL, FULL>;
     static DeviceOnce once;
     const cudaError_t e = allow_dynamic_smem(once, kernel, static_cast<int>(kSmemMost));
     if (e != cudaSuccess) return e;
@@ -432,6 +433,23 @@ cudaError_t launch_staged(const RmsResidualBwdArgs &a, const RmsResidualParts &p
     cfg.numAttrs = 1;
     const uint32_t rpg = static_cast<uint32_t>(a.t.gate_rows ? a.t.rows / a.t.gate_rows : a.t.rows);
     return cudaLaunchKernelEx(&cfg, kernel, a, parts, p, rpg, status);
+}
+
+// Kernels compiled for the terms a training step has (dy, ds and gamma_post there); one for all other combinations.
+template <int VPT, bool BF16>
+cudaError_t launch_terms(const RmsResidualBwdArgs &a, const RmsResidualParts &parts, const StagedPlan &p, int *status,
+                         cudaStream_t stream) {
+    const bool col = a.t.res_scale && !a.t.res_scale_one;
+    if (!(a.dy && a.ds && a.t.gamma_post))
+        return col ? launch_staged<VPT, BF16, 3, true, false>(a, parts, p, status, stream)
+                   : launch_staged<VPT, BF16, 3, false, false>(a, parts, p, status, stream);
+    const int gate = !a.t.gate ? 0 : p.place[kGate] >= 0 ? 2 : 1;
+    if (gate == 0) return col ? launch_staged<VPT, BF16, 0, true, true>(a, parts, p, status, stream)
+                              : launch_staged<VPT, BF16, 0, false, true>(a, parts, p, status, stream);
+    if (gate == 1) return col ? launch_staged<VPT, BF16, 1, true, true>(a, parts, p, status, stream)
+                              : launch_staged<VPT, BF16, 1, false, true>(a, parts, p, status, stream);
+    return col ? launch_staged<VPT, BF16, 2, true, true>(a, parts, p, status, stream)
+               : launch_staged<VPT, BF16, 2, false, true>(a, parts, p, status, stream);
 }
 
 }  // namespace
@@ -450,14 +468,9 @@ cudaError_t rmsnorm_residual_staged_bwd(const RmsResidualBwdArgs &a, const RmsRe
     if (e != cudaSuccess) return e;
     const StagedPlan p = make_staged_plan(a, sms);
     if (p.T == 0 || p.slots < p.G) return cudaErrorInvalidValue;
-    const bool col = a.t.res_scale && !a.t.res_scale_one;
-#define PG_STAGED(V)                                                                                   \
-    (a.t.bf16 ? (col ? launch_staged<V, true, true>(a, parts, p, status, stream)                        \
-                     : launch_staged<V, true, false>(a, parts, p, status, stream))                      \
-              : (col ? launch_staged<V, false, true>(a, parts, p, status, stream)                       \
-                     : launch_staged<V, false, false>(a, parts, p, status, stream)))
-    return p.vpt == 1 ? PG_STAGED(1) : PG_STAGED(2);
-#undef PG_STAGED
+    if (p.vpt == 1)
+        return a.t.bf16 ? launch_terms<1, true>(a, parts, p, status, stream) : launch_terms<1, false>(a, parts, p, status, stream);
+    return a.t.bf16 ? launch_terms<2, true>(a, parts, p, status, stream) : launch_terms<2, false>(a, parts, p, status, stream);
 }
 
 }  // namespace pg
