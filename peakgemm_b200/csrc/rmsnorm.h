@@ -79,8 +79,9 @@ struct RmsResidualParts {
     double *scale_one;      // n_one of them, where res_scale has one element
     uint32_t workers, n_one;
 };
-// Bulk-copy staged backward kernel (rmsnorm_residual_staged.cu), for the widths where `workers` is not 0.
-uint32_t rmsnorm_residual_staged_workers(int64_t rows, int64_t h, int sms);
+// Bulk-copy staged backward kernel (rmsnorm_residual_staged.cu), for the widths where `workers` is not 0; a row is
+// shared by ctas_per_row CTAs, each of which writes a scale_one of its own.
+uint32_t rmsnorm_residual_staged_workers(int64_t rows, int64_t h, int sms, uint32_t *ctas_per_row);
 cudaError_t rmsnorm_residual_staged_bwd(const RmsResidualBwdArgs &a, const RmsResidualParts &parts, cudaStream_t stream);
 
 // Bulk-copy staged variants (rmsnorm_staged.cu), used for 2048 <= h <= 16384.

@@ -444,13 +444,14 @@ struct BwdPlan {
 BwdPlan bwd_plan(int64_t rows, int64_t h, int64_t gate_rows, int sms) {
     const auto up = [](size_t b) { return (b + 255) / 256 * 256; };
     BwdPlan p;
-    p.workers = rmsnorm_residual_staged_workers(rows, h, sms);
+    uint32_t ctas_per_row = 1;
+    p.workers = rmsnorm_residual_staged_workers(rows, h, sms, &ctas_per_row);
     p.staged = p.workers > 0;
     if (!p.staged) {
         const int64_t c = (static_cast<int64_t>(sms) * 16 + col_blocks(h) - 1) / col_blocks(h);
         p.workers = static_cast<uint32_t>(c < rows ? c : rows);
     }
-    p.n_one = p.staged ? p.workers : p.workers * col_blocks(h);
+    p.n_one = p.staged ? p.workers * ctas_per_row : p.workers * col_blocks(h);
     const size_t table = up(static_cast<size_t>(p.workers) * h * sizeof(float));
     p.post = 0;
     p.pre = p.post + table;

@@ -80,7 +80,7 @@ def check_backward(x, s, out, eps=1e-6):
 
 # every width class (one warp per row, several vectors per thread, rows over 16384 elements), odd row counts
 SHAPES = [(1, 8), (5, 8), (7, 64), (33, 256), (100, 1000), (257, 4096), (64, 8192), (19, 5120), (301, 2048), (5, 16384),
-          (4, 16392), (3, 24576), (2, 65544)]
+          (4, 16392), (3, 24576), (2, 65544), (301, 4104), (150, 8200), (77, 12288), (40, 32768), (9, 32776)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
