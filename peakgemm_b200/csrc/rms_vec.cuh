@@ -56,10 +56,10 @@ __device__ __forceinline__ uint4 vec_pack2(const float2 (&f)[4]) {
     return make_uint4(ptx::pack2<BF16>(f[0].x, f[0].y), ptx::pack2<BF16>(f[1].x, f[1].y),
                       ptx::pack2<BF16>(f[2].x, f[2].y), ptx::pack2<BF16>(f[3].x, f[3].y));
 }
-// Eight fp32 values from shared memory.
-__device__ __forceinline__ void vec_load2(uint32_t s, float2 (&f)[4]) {
+// Eight fp32 values from shared memory, the upper four `half` bytes behind the lower ones.
+__device__ __forceinline__ void vec_load2(uint32_t s, uint32_t half, float2 (&f)[4]) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[0].x), "=f"(f[0].y), "=f"(f[1].x), "=f"(f[1].y) : "r"(s));
-    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[2].x), "=f"(f[2].y), "=f"(f[3].x), "=f"(f[3].y) : "r"(s + 16));
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f[2].x), "=f"(f[2].y), "=f"(f[3].x), "=f"(f[3].y) : "r"(s + half));
 }
 __device__ __forceinline__ void vec_store2(float *p, const float2 (&f)[4]) {
     reinterpret_cast<float4 *>(p)[0] = make_float4(f[0].x, f[0].y, f[1].x, f[1].y);

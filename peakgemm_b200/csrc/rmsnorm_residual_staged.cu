@@ -84,7 +84,7 @@ rms_residual_bwd_staged_kernel(const RmsResidualBwdArgs a, const RmsResidualPart
     const int row8 = static_cast<int>(a.t.h / 8);                   // a whole row, in vectors
     const uint32_t C = CLUSTER ? p.C : 1u, cta = CLUSTER ? cluster_ctarank() : 0u;
     const int col0 = static_cast<int>(cta) * p.cols8;               // this CTA's columns, in vectors
-    const int h8 = CLUSTER ? min(p.cols8, row8 - col0) : row8, h = 8 * p.cols8;
+    const int h8 = CLUSTER ? min(p.cols8, row8 - col0) : row8;
     const uint32_t row_bytes = h8 * 16;
     const float inv_h = 1.f / static_cast<float>(a.t.h);
     const uint32_t rows = static_cast<uint32_t>(a.t.rows);
@@ -112,15 +112,18 @@ rms_residual_bwd_staged_kernel(const RmsResidualBwdArgs a, const RmsResidualPart
         for (int k = 0; k < 3; ++k)
             if (src[k])
                 for (int i = threadIdx.x; i < 2 * h8; i += blockDim.x)
-                    reinterpret_cast<float4 *>(smem)[k * (h / 4) + i] = __ldg(reinterpret_cast<const float4 *>(src[k]) + 2 * col0 + i);
+                    reinterpret_cast<float4 *>(smem)[(2 * k + (i & 1)) * p.cols8 + (i >> 1)] =
+                        __ldg(reinterpret_cast<const float4 *>(src[k]) + 2 * col0 + i);
     }
     __syncthreads();
     if constexpr (CLUSTER) {                   // every CTA's barriers exist before anyone signals them
         cluster_arrive();
         cluster_wait();
     }
-    const auto gamma_pre = [&](int idx, float2 (&f)[4]) { vec_load2(sbase + 32 * idx, f); };
-    const auto gamma_post = [&](int idx, float2 (&f)[4]) { vec_load2(sbase + 4 * h + 32 * idx, f); };
+    // the lower and upper halves of the vectors apart: a warp's 16-byte loads are consecutive
+    const uint32_t half = 16 * p.cols8;
+    const auto gamma_pre = [&](int idx, float2 (&f)[4]) { vec_load2(sbase + 16 * idx, half, f); };
+    const auto gamma_post = [&](int idx, float2 (&f)[4]) { vec_load2(sbase + 2 * half + 16 * idx, half, f); };
 
     const int g = threadIdx.x / p.T, t = threadIdx.x - g * p.T;
     const uint32_t worker = blockIdx.x / C * p.G + g;
@@ -279,7 +282,7 @@ rms_residual_bwd_staged_kernel(const RmsResidualBwdArgs a, const RmsResidualPart
                     }
                 }
                 if constexpr (SCALE_COL) {
-                    vec_load2(sbase + 8 * h + 32 * idx, x);
+                    vec_load2(sbase + 4 * half + 16 * idx, half, x);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], D[e]);
                 } else {
