@@ -34,7 +34,8 @@ TORCH_LIB = os.path.join(PKG_DIR, "libPeakGemm.so")
 # signal go missing.  Loaded only by tests/test_wait_timeout_gpu.py; nothing in the package opens it.
 WAITTEST_LIB = os.path.join(PKG_DIR, "libPeakGemm_device_waittest.so")
 
-DEVICE_SOURCES = ["gemm_sm100.cu", "lora.cu", "rmsnorm.cu", "rmsnorm_staged.cu", "rmsnorm_static.cu", "rmsnorm_rstd.cu", "rmsnorm_residual.cu", "rmsnorm_residual_staged.cu", "peer.cu", "sgemm.cu", "probes.cu", "api.cu"]
+DEVICE_SOURCES = ["gemm_sm100.cu", "lora.cu", "rmsnorm.cu", "rmsnorm_staged.cu", "rmsnorm_static.cu", "rmsnorm_rstd.cu", "rmsnorm_residual.cu", "rmsnorm_residual_staged.cu",
+                  "rmsnorm_residual_staged_fwd.cu", "peer.cu", "sgemm.cu", "probes.cu", "api.cu"]
 DEVICE_HEADERS = ["ptx.cuh", "gemm_common.cuh", "lora_epilogue.cuh", "gemm_sm100.h", "host_util.h", "lora.h", "rms_vec.cuh", "rmsnorm.h", "sgemm.h", os.path.join(INCLUDE, "peakgemm.h")]
 
 NVCC_FLAGS = [

@@ -79,6 +79,9 @@ struct RmsResidualParts {
     double *scale_one;      // n_one of them, where res_scale has one element
     uint32_t workers, n_one;
 };
+// Bulk-copy staged forward kernel (rmsnorm_residual_staged_fwd.cu), where it has the width and every worker a row.
+bool rmsnorm_residual_staged_fwd_supported(const RmsResidualTerms &t, int sms);
+cudaError_t rmsnorm_residual_staged_fwd(const RmsResidualFwdArgs &a, cudaStream_t stream);
 // Bulk-copy staged backward kernel (rmsnorm_residual_staged.cu), for the widths where `workers` is not 0; a row is
 // shared by ctas_per_row CTAs, each of which writes a scale_one of its own.
 uint32_t rmsnorm_residual_staged_workers(int64_t rows, int64_t h, int sms, uint32_t *ctas_per_row);

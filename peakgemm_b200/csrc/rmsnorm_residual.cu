@@ -473,6 +473,7 @@ cudaError_t rmsnorm_residual_fwd_launch(const RmsResidualFwdArgs &a, cudaStream_
     int sms = 0;
     cudaError_t e = current_device_sm_count(&sms);
     if (e != cudaSuccess) return e;
+    if (rmsnorm_residual_staged_fwd_supported(a.t, sms)) return rmsnorm_residual_staged_fwd(a, stream);
     const int64_t h8 = a.t.h / 8;
     int64_t grid = static_cast<int64_t>(sms) * 16;
     if (grid > a.t.rows) grid = a.t.rows;

@@ -1,0 +1,271 @@
+// Forward pass of the norms around a gated residual (formulas: rmsnorm_residual.cu) for many rows of h <= 8192.
+// HBM-bound: two or three rows of 2h bytes come in and one or two go out for every row.
+//   * The threads of a CTA form G groups of T threads, each a worker that takes every W-th row; a thread owns two
+//     vectors of eight columns.  Operand rows (u, residual, the row's gate) arrive by cp.async.bulk in a ring of
+//     shared-memory slots per group, issued by the group's first thread for a slot that the group has just left.
+//   * A row needs the sum over u^2 (A) before s can be formed (B), and the sum over s^2 before y (C).  The second sum
+//     of a row is joined with the first of the next one: per row one barrier, behind it C of the row before, B, and A
+//     of the row after.
+//   * The gains are kept in shared memory, the lower and upper halves of the vectors apart (no bank conflicts).
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "gemm_common.cuh"
+#include "host_util.h"
+#include "ptx.cuh"
+#include "rms_vec.cuh"
+#include "rmsnorm.h"
+
+namespace pg {
+
+using namespace ptx;
+
+namespace {
+
+enum : int { kStRmsConsumer = 12 };      // status code: a consumer gave up waiting for its row
+
+constexpr int kVpt = 2;
+constexpr int kMaxThreads = 768;         // 80 registers a thread
+constexpr int kMaxGroups = 8, kMaxPerGroup = 3;
+constexpr uint32_t kSmemMost = 232448;
+
+struct FwdPlan {
+    int T, G, per_group;          // threads of a group, groups, slots of a group; T = 0: the width is not supported
+    uint32_t slot_bytes, off_slot, off_red, off_bar, smem;
+};
+
+// FULL: gamma_post and y are there.
+template <bool BF16, bool GATE, bool SCALE_COL, bool FULL>
+__global__ void __launch_bounds__(kMaxThreads, 1)
+rms_residual_fwd_staged_kernel(const RmsResidualFwdArgs a, const FwdPlan p, uint32_t workers, uint32_t rows_per_gate,
+                               int *status) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    constexpr int VPT = kVpt;
+    const uint32_t sbase = smem_u32(smem);
+    const int h8 = static_cast<int>(a.t.h / 8);
+    const uint32_t row_bytes = h8 * 16, half = h8 * 16;
+    const float inv_h = 1.f / static_cast<float>(a.t.h);
+    const uint32_t rows = static_cast<uint32_t>(a.t.rows);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int group_warps = p.T >> 5, g = threadIdx.x / p.T, t = threadIdx.x - g * p.T, gw = warp - g * group_warps;
+    const uint32_t bar_full = sbase + p.off_bar + g * p.per_group * 8;
+    volatile uint32_t *abort_flag = reinterpret_cast<volatile uint32_t *>(smem + p.off_bar + p.G * p.per_group * 8);
+    const WaitCtx ctx{abort_flag, status};
+    const bool has_post = FULL || a.t.gamma_post, has_y = FULL || a.y;
+    // the next launch orders itself with griddepcontrol.wait, as this one does
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < p.G * p.per_group; ++s) mbar_init(sbase + p.off_bar + s * 8, 1);
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    {
+        const float *src[3] = {has_post ? a.t.gamma_post : nullptr, has_y ? a.t.gamma_pre : nullptr,
+                               SCALE_COL ? a.t.res_scale : nullptr};
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (src[k])
+                for (int i = threadIdx.x; i < 2 * h8; i += blockDim.x)
+                    reinterpret_cast<float4 *>(smem)[(2 * k + (i & 1)) * h8 + (i >> 1)] =
+                        __ldg(reinterpret_cast<const float4 *>(src[k]) + i);
+    }
+    __syncthreads();
+    const uint32_t ring0 = p.off_slot + g * p.per_group * p.slot_bytes;
+    const uint32_t first = blockIdx.x * p.G + g;
+    const auto issue = [&](uint32_t row, int at) {
+        const uint64_t pol = l2_policy_evict_first();
+        const uint32_t dst = sbase + ring0 + at * p.slot_bytes, bar = bar_full + at * 8;
+        mbar_arrive_expect_tx(bar, p.slot_bytes);
+        bulk_load(dst, static_cast<const uint4 *>(a.u) + static_cast<int64_t>(row) * h8, row_bytes, bar, pol);
+        bulk_load(dst + row_bytes, static_cast<const uint4 *>(a.residual) + static_cast<int64_t>(row) * h8, row_bytes, bar, pol);
+        if constexpr (GATE)
+            bulk_load(dst + 2 * row_bytes, static_cast<const uint4 *>(a.t.gate) + static_cast<int64_t>(row / rows_per_gate) * h8,
+                      row_bytes, bar, rows_per_gate == 1 ? pol : l2_policy_evict_last());
+    };
+    // rows first, first + workers, ...; a thread that could overflow 32 bits leaves
+    if (t == 0)
+        for (int i = 0; i < p.per_group && first + static_cast<uint64_t>(i) * workers < rows; ++i) issue(first + i * workers, i);
+
+    float4 *red = reinterpret_cast<float4 *>(smem + p.off_red);
+    float2 *sums = reinterpret_cast<float2 *>(red) + g * 2 * group_warps;          // [parity][warps]
+    const float one_scale = a.t.res_scale && a.t.res_scale_one ? __ldg(a.t.res_scale) : 1.f;
+    const float2 scale_one = make_float2(one_scale, one_scale), zero = make_float2(0.f, 0.f);
+    float2 s[VPT][4];
+    float uu = 0.f, ss = 0.f;
+    int ring = 0, ring_prev = 0;
+    uint32_t phase = 0, parity = 0;
+    bool ok = true;
+    const auto operand = [&](int at, int o, int idx) {
+        return reinterpret_cast<const uint4 *>(smem + ring0 + at * p.slot_bytes + o * row_bytes)[idx];
+    };
+    // A: this thread's part of the sum over u^2 of the row at `at`
+    const auto sum_of = [&](int at) {
+        ok = __all_sync(0xffffffffu, wait_bar(bar_full + at * 8, phase, ctx, kStRmsConsumer));
+        float2 x = zero;
+        if (has_post) {
+#pragma unroll
+            for (int j = 0; j < VPT; ++j) {
+                const int idx = t + p.T * j;
+                if (ok && idx < h8) {
+                    float2 u[4];
+                    vec_unpack2<BF16>(operand(at, 0, idx), u);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x = fma2(u[e], u[e], x);
+                }
+            }
+        }
+        uu = x.x + x.y;
+    };
+    sum_of(0);
+    const uint64_t stride = workers;
+    for (uint64_t row = first;; row += stride, parity ^= 1u) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            uu += __shfl_xor_sync(0xffffffffu, uu, o);
+            ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        }
+        if (lane == 0) sums[parity * group_warps + gw] = make_float2(uu, ss);
+        if (group_barrier_or(1 + g, p.T, !ok || *abort_flag != 0)) break;
+        uu = ss = 0.f;
+        for (int w = 0; w < group_warps; ++w) {
+            const float2 x = sums[parity * group_warps + w];
+            uu += x.x;
+            ss += x.y;
+        }
+        if (row != first) {
+            const uint64_t before = row - stride;
+            // the group has left the slot of the row before
+            if (t == 0 && before + p.per_group * stride < rows) issue(static_cast<uint32_t>(before + p.per_group * stride), ring_prev);
+            if (has_y) {
+                // C (rsqrt.approx is within 2 ulp of fp32; y is rounded to 16 bits)
+                const float r = rsqrtf(fmaf(ss, inv_h, a.t.eps));
+                const float2 r2 = make_float2(r, r);
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) {
+                    const int idx = t + p.T * j;
+                    if (idx < h8) {
+                        float2 gm[4];
+                        vec_load2(sbase + 2 * half + 16 * idx, half, gm);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) gm[e] = mul2(mul2(s[j][e], r2), gm[e]);
+                        __stcs(static_cast<uint4 *>(a.y) + static_cast<int64_t>(before) * h8 + idx, vec_pack2<BF16>(gm));
+                    }
+                }
+            }
+        }
+        if (row >= rows) break;
+        // B: s, its sum of squares
+        const float r = has_post ? rsqrtf(fmaf(uu, inv_h, a.t.eps)) : 1.f;
+        const float2 r2 = make_float2(r, r);
+        float2 ss2 = zero;
+#pragma unroll
+        for (int j = 0; j < VPT; ++j) {
+            const int idx = t + p.T * j;
+            if (idx < h8) {
+                float2 u[4], x[4];
+                vec_unpack2<BF16>(operand(ring, 0, idx), u);
+                if (has_post) {
+                    vec_load2(sbase + 16 * idx, half, x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[e] = mul2(mul2(u[e], r2), x[e]);
+                }
+                if constexpr (GATE) {
+                    vec_unpack2<BF16>(operand(ring, 2, idx), x);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) u[e] = mul2(u[e], x[e]);
+                }
+                vec_unpack2<BF16>(operand(ring, 1, idx), x);
+                if constexpr (SCALE_COL) {
+                    float2 sc[4];
+                    vec_load2(sbase + 4 * half + 16 * idx, half, sc);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[j][e] = fma2(sc[e], x[e], u[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[j][e] = fma2(scale_one, x[e], u[e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) ss2 = fma2(s[j][e], s[j][e], ss2);
+                __stcs(static_cast<uint4 *>(a.s) + static_cast<int64_t>(row) * h8 + idx, vec_pack2<BF16>(s[j]));
+            }
+        }
+        ss = ss2.x + ss2.y;
+        uu = 0.f;
+        ring_prev = ring;
+        if (++ring == p.per_group) { ring = 0; phase ^= 1u; }
+        if (row + stride < rows) sum_of(ring);
+    }
+    __syncthreads();
+    if (*abort_flag) __nanosleep(50000);       // let bulk copies still in flight land
+}
+
+FwdPlan make_plan(const RmsResidualTerms &t) {
+    FwdPlan p = {};
+    const int64_t h8 = t.h / 8;
+    if (h8 > 1024) return p;
+    const int T = static_cast<int>(((h8 + kVpt - 1) / kVpt + 31) / 32 * 32);
+    p.G = kMaxThreads / T;
+    if (p.G > kMaxGroups) p.G = kMaxGroups;
+    p.slot_bytes = static_cast<uint32_t>(h8) * 16 * (t.gate ? 3 : 2);
+    p.off_slot = static_cast<uint32_t>(h8) * 32 * (t.res_scale && !t.res_scale_one ? 3 : 2);
+    const uint32_t fixed = p.G * (T / 32) * 2 * 8 + 16 + kMaxGroups * kMaxPerGroup * 8 + 16;
+    p.per_group = static_cast<int>((kSmemMost - p.off_slot - fixed) / p.slot_bytes) / p.G;
+    if (p.per_group > kMaxPerGroup) p.per_group = kMaxPerGroup;
+    if (p.per_group < 1) return p;
+    p.T = T;
+    p.off_red = p.off_slot + p.G * p.per_group * p.slot_bytes;
+    p.off_bar = (p.off_red + p.G * (T / 32) * 2 * 8 + 15) / 16 * 16;
+    p.smem = p.off_bar + kMaxGroups * kMaxPerGroup * 8 + 16;
+    return p;
+}
+
+template <bool BF16, bool GATE, bool SCALE_COL, bool FULL>
+cudaError_t launch_fwd(const RmsResidualFwdArgs &a, const FwdPlan &p, int sms, int *status, cudaStream_t stream) {
+    auto kernel = rms_residual_fwd_staged_kernel<BF16, GATE, SCALE_COL, FULL>;
+    static DeviceOnce once;
+    const cudaError_t e = allow_dynamic_smem(once, kernel, static_cast<int>(kSmemMost));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(sms), 1, 1);
+    cfg.blockDim = dim3(static_cast<unsigned>(p.T * p.G), 1, 1);
+    cfg.dynamicSmemBytes = p.smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const uint32_t rpg = static_cast<uint32_t>(a.t.gate_rows ? a.t.rows / a.t.gate_rows : a.t.rows);
+    return cudaLaunchKernelEx(&cfg, kernel, a, p, static_cast<uint32_t>(sms * p.G), rpg, status);
+}
+
+template <bool BF16>
+cudaError_t launch_terms(const RmsResidualFwdArgs &a, const FwdPlan &p, int sms, int *status, cudaStream_t stream) {
+    const bool col = a.t.res_scale && !a.t.res_scale_one, full = a.t.gamma_post && a.y;
+#define PG_FWD(GATE, COL)                                                             \
+    (full ? launch_fwd<BF16, GATE, COL, true>(a, p, sms, status, stream)              \
+          : launch_fwd<BF16, GATE, COL, false>(a, p, sms, status, stream))
+    if (a.t.gate) return col ? PG_FWD(true, true) : PG_FWD(true, false);
+    return col ? PG_FWD(false, true) : PG_FWD(false, false);
+#undef PG_FWD
+}
+
+}  // namespace
+
+bool rmsnorm_residual_staged_fwd_supported(const RmsResidualTerms &t, int sms) {
+    const FwdPlan p = make_plan(t);
+    // every worker has a row (a CTA's groups begin with one each)
+    return p.T != 0 && t.rows >= static_cast<int64_t>(sms) * p.G;
+}
+
+cudaError_t rmsnorm_residual_staged_fwd(const RmsResidualFwdArgs &a, cudaStream_t stream) {
+    int sms = 0, *status = nullptr;
+    const cudaError_t e = rmsnorm_device(&sms, &status);
+    if (e != cudaSuccess) return e;
+    const FwdPlan p = make_plan(a.t);
+    return a.t.bf16 ? launch_terms<true>(a, p, sms, status, stream) : launch_terms<false>(a, p, sms, status, stream);
+}
+
+}  // namespace pg
