@@ -27,7 +27,7 @@ enum : int { kStRmsConsumer = 12 };      // status code: a consumer gave up wait
 
 constexpr int kVpt = 2;
 constexpr int kMaxThreads = 768;         // 80 registers a thread
-constexpr int kMaxGroups = 8, kMaxPerGroup = 3;
+constexpr int kMaxGroups = 8, kMaxPerGroup = 4;
 constexpr uint32_t kSmemMost = 232448;
 
 struct FwdPlan {
@@ -212,7 +212,16 @@ FwdPlan make_plan(const RmsResidualTerms &t) {
     p.off_slot = static_cast<uint32_t>(h8) * 32 * (t.res_scale && !t.res_scale_one ? 3 : 2);
     const uint32_t fixed = p.G * (T / 32) * 2 * 8 + 16 + kMaxGroups * kMaxPerGroup * 8 + 16;
     p.per_group = static_cast<int>((kSmemMost - p.off_slot - fixed) / p.slot_bytes) / p.G;
-    if (p.per_group > kMaxPerGroup) p.per_group = kMaxPerGroup;
+    // About 112 KiB of rows in flight from HBM, at least two slots for a group and three for a lone one (whose next row
+    // has to be there while it works).  [rows, h] bf16, 134 M elements, us with 2 / 3 / 4 slots: h = 1024 (8 groups)
+    // 196 / 180 / 192, 2048 (6) 171 / 192 / 193, 5120 (2) 202 / 163-181 / 167-188, with a gate per row 224 / 236 / 234,
+    // 8192 (1) 281 / 174 / 166, with a gate per row 302 / 200 / 203.
+    const bool token_gate = t.gate && t.gate_rows == t.rows;
+    const int hbm_row = static_cast<int>(h8) * 16 * (token_gate ? 3 : 2) * p.G;
+    int want = (112 * 1024 + hbm_row / 2) / hbm_row;
+    if (want < (p.G == 1 ? 3 : 2)) want = p.G == 1 ? 3 : 2;
+    if (want > kMaxPerGroup) want = kMaxPerGroup;
+    if (p.per_group > want) p.per_group = want;
     if (p.per_group < 1) return p;
     p.T = T;
     p.off_red = p.off_slot + p.G * p.per_group * p.slot_bytes;
