@@ -463,15 +463,20 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                 tile_coords(group_m, u.tile, m_tiles, n_tiles, mi, ni, (flags & kFlagSerpentine) != 0);
                 const int32_t row_a = static_cast<int32_t>(mi * kTileM + rank * kBM);    // + mt * kBlockM
                 const int32_t row_b = static_cast<int32_t>(ni * BN + rank * C::kBRows);
-                LoraBlocks extra;                    // the adapters' k-blocks behind the product's own
+                LoraBlocks extra;                    // the adapters' blocks behind the product's own
+                if constexpr (LORA)
+                    if (it > 0) extra.load(lora.d, mi);
                 for (uint32_t kb = u.kb0; kb < u.kb1 + extra.count; ++kb) {
                     const bool own = !LORA || kb < u.kb1;
                     if constexpr (LORA) {
                         // The last block of the product has to know whether the tile ends with it: from here on the
                         // down projections must be there.
                         if (kb + 1 == u.kb1) {
-                            if (it == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
-                            extra.open(lora.d, mi);
+                            if (it == 0) {
+                                asm volatile("griddepcontrol.wait;" ::: "memory");
+                                extra.load(lora.d, mi);
+                            }
+                            extra.open(lora.d);
                         }
                     }
                     if (own && tail.wave_sync != nullptr && leader) {
@@ -495,12 +500,16 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                         // wait until the MMAs that read this stage have completed
                         ok = wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty);
                         if (!ok) break;
-                        if constexpr (LORA) stage_info[stage] = extra.info(lora.d, kb, u.kb1);
+                        uint32_t bytes = C::kStageBytes;             // of one CTA
+                        if constexpr (LORA) {
+                            stage_info[stage] = extra.info(lora.d, kb, u.kb1);
+                            if (!own) bytes = C::kStageBytes / kBK * lora.d.width * extra.parts(lora.d);
+                        }
                         if constexpr (CTA_GROUP == 2) {
                             mbar_arrive_cluster(peer_empty0 + stage * 8);   // relay to the peer
-                            mbar_arrive_expect_tx(bar_full + stage * 8, 2 * C::kStageBytes);
+                            mbar_arrive_expect_tx(bar_full + stage * 8, 2 * bytes);
                         } else {
-                            mbar_arrive_expect_tx(bar_full + stage * 8, C::kStageBytes);
+                            mbar_arrive_expect_tx(bar_full + stage * 8, bytes);
                         }
                     } else {
                         ok = wait_bar(bar_empty + stage * 8, phase, ctx, kStProducerEmpty);
@@ -512,16 +521,20 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     const uint32_t fb = (CTA_GROUP == 2) ? full0 + stage * 8 : bar_full + stage * 8;
                     if constexpr (LORA) {
                         if (!own) {
-                            const int32_t rx = extra.next(lora.d);
+                            const uint32_t parts = extra.parts(lora.d), width2 = lora.d.width * 2;
+                            for (uint32_t i = 0; i < parts; ++i) {
+                                const int32_t rx = extra.next(lora.d);
 #pragma unroll
-                            for (uint32_t mt = 0; mt < MT; ++mt) {
-                                const uint32_t da = dst_a + mt * C::kABox;
-                                const int32_t rv = extra.v_row + static_cast<int32_t>(mt * kBlockM + rank * kBM);
-                                if constexpr (CTA_GROUP == 2) tma_load_2d_pair(da, &lora.tm_v, fb, rx, rv);
-                                else tma_load_2d(da, &lora.tm_v, fb, rx, rv);
+                                for (uint32_t mt = 0; mt < MT; ++mt) {
+                                    const uint32_t da = dst_a + mt * C::kABox + i * kBM * width2;
+                                    const int32_t rv = extra.v_row + static_cast<int32_t>(mt * kBlockM + rank * kBM);
+                                    if constexpr (CTA_GROUP == 2) tma_load_2d_pair(da, &lora.tm_v, fb, rx, rv);
+                                    else tma_load_2d(da, &lora.tm_v, fb, rx, rv);
+                                }
+                                const uint32_t db = dst_b + i * C::kBRows * width2;
+                                if constexpr (CTA_GROUP == 2) tma_load_2d_pair(db, &lora.tm_b, fb, rx, extra.b_row + row_b);
+                                else tma_load_2d(db, &lora.tm_b, fb, rx, extra.b_row + row_b);
                             }
-                            if constexpr (CTA_GROUP == 2) tma_load_2d_pair(dst_b, &lora.tm_b, fb, rx, extra.b_row + row_b);
-                            else tma_load_2d(dst_b, &lora.tm_b, fb, rx, extra.b_row + row_b);
                             if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                             continue;
                         }
@@ -570,11 +583,20 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                     if (!ok) break;
                     tc_fence_after_sync();
-                    uint32_t steps = kBK / kUmmaK;
                     if constexpr (LORA) {
                         const uint32_t info = stage_info[stage];
-                        steps = info & 7u;
                         last = (info & kLoraLast) != 0;
+                        if (info >> 4) {
+#pragma unroll
+                            for (uint32_t mt = 0; mt < MT; ++mt)
+                                lora_stage_mma<CTA_GROUP>(tmem_base + (MT == 2 ? mt : acc) * BN,
+                                                          smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox,
+                                                          smem_base + C::kOffB + stage * C::kBBytes, kBM, C::kBRows, idesc,
+                                                          info, lora.d.width);
+                            umma_commit<CTA_GROUP>(bar_empty + stage * 8);
+                            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                            continue;
+                        }
                     }
                     const uint64_t db = smem_desc_k_sw128(smem_base + C::kOffB + stage * C::kBBytes);
 #pragma unroll
@@ -593,7 +615,6 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
 #pragma unroll
                         for (uint32_t k = 0; k < kBK / kUmmaK; ++k) {
                             // 16 elements of k = 32 bytes inside the 128-byte swizzle row = +2 in the >>4 address field
-                            if (LORA && k >= steps) break;
                             umma_f16<CTA_GROUP>(tmem_d, da + 2 * k, db + 2 * k, idesc,
                                                 (kb != u.kb0 || k != 0u) ? 1u : 0u);
                         }
@@ -1056,23 +1077,28 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 if constexpr (LORA) {
                     if (kb + 1 == kb1) {
                         asm volatile("griddepcontrol.wait;" ::: "memory");
-                        extra.open(lora.d, mi, rank, (k_blocks + per - 1) / per);
+                        extra.load(lora.d, mi);
+                        extra.open(lora.d, rank, (k_blocks + per - 1) / per);
                     }
                 }
                 if (!wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty)) break;
-                if constexpr (LORA) stage_info[stage] = extra.info(lora.d, kb, kb1);
-                mbar_arrive_expect_tx(bar_full + stage * 8, C::kStageBytes);
                 if constexpr (LORA) {
+                    stage_info[stage] = extra.info(lora.d, kb, kb1);
                     if (kb >= kb1) {
-                        const int32_t rx = extra.next(lora.d);
-                        tma_load_2d(smem_base + C::kOffA + stage * C::kABytes, &lora.tm_v, bar_full + stage * 8, rx,
-                                    extra.v_row);
-                        tma_load_2d(smem_base + C::kOffB + stage * C::kBBytes, &lora.tm_b, bar_full + stage * 8, rx,
-                                    extra.b_row + static_cast<int32_t>(ni * BN));
+                        const uint32_t parts = extra.parts(lora.d), width2 = lora.d.width * 2;
+                        mbar_arrive_expect_tx(bar_full + stage * 8, parts * width2 * (kBM + BN));
+                        for (uint32_t i = 0; i < parts; ++i) {
+                            const int32_t rx = extra.next(lora.d);
+                            tma_load_2d(smem_base + C::kOffA + stage * C::kABytes + i * kBM * width2, &lora.tm_v,
+                                        bar_full + stage * 8, rx, extra.v_row);
+                            tma_load_2d(smem_base + C::kOffB + stage * C::kBBytes + i * BN * width2, &lora.tm_b,
+                                        bar_full + stage * 8, rx, extra.b_row + static_cast<int32_t>(ni * BN));
+                        }
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                         continue;
                     }
                 }
+                mbar_arrive_expect_tx(bar_full + stage * 8, C::kStageBytes);
                 const int32_t kx = static_cast<int32_t>(kb * kBK);
                 tma_load_2d_hint(smem_base + C::kOffA + stage * C::kABytes, &tm_a, bar_full + stage * 8, kx,
                                  static_cast<int32_t>(mi * kBM), pol_keep);
@@ -1092,19 +1118,22 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                 if (!ok) break;
                 tc_fence_after_sync();
-                uint32_t steps = kBK / kUmmaK;
                 if constexpr (LORA) {
                     const uint32_t info = stage_info[stage];
-                    steps = info & 7u;
                     last = (info & kLoraLast) != 0;
+                    if (info >> 4) {
+                        lora_stage_mma<1>(tmem_base, smem_base + C::kOffA + stage * C::kABytes,
+                                          smem_base + C::kOffB + stage * C::kBBytes, kBM, BN, idesc, info, lora.d.width);
+                        umma_commit<1>(bar_empty + stage * 8);
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                        continue;
+                    }
                 }
                 const uint64_t da = smem_desc_k_sw128(smem_base + C::kOffA + stage * C::kABytes);
                 const uint64_t db = smem_desc_k_sw128(smem_base + C::kOffB + stage * C::kBBytes);
 #pragma unroll
-                for (uint32_t k = 0; k < kBK / kUmmaK; ++k) {
-                    if (LORA && k >= steps) break;
+                for (uint32_t k = 0; k < kBK / kUmmaK; ++k)
                     umma_f16<1>(tmem_base, da + 2 * k, db + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
-                }
                 umma_commit<1>(bar_empty + stage * 8);
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
@@ -1588,23 +1617,28 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                 if constexpr (LORA) {
                     if (kb + 1 == kb1) {
                         asm volatile("griddepcontrol.wait;" ::: "memory");
-                        extra.open(lora.d, 0, rank, (k_blocks + per - 1) / per);
+                        extra.load(lora.d, 0);
+                        extra.open(lora.d, rank, (k_blocks + per - 1) / per);
                     }
                 }
                 if (!wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty)) break;
-                if constexpr (LORA) stage_info[stage] = extra.info(lora.d, kb, kb1);
-                mbar_arrive_expect_tx(bar_full + stage * 8, C::kStageBytes);
                 if constexpr (LORA) {
+                    stage_info[stage] = extra.info(lora.d, kb, kb1);
                     if (kb >= kb1) {
-                        const int32_t rx = extra.next(lora.d);
-                        tma_load_2d(smem_base + C::kOffW + stage * C::kWBytes, &lora.tm_b, bar_full + stage * 8, rx,
-                                    extra.b_row + static_cast<int32_t>(ni * kBM));
-                        tma_load_2d(smem_base + C::kOffT + stage * C::kTBytes, &lora.tm_v, bar_full + stage * 8, rx,
-                                    extra.v_row);
+                        const uint32_t parts = extra.parts(lora.d), width2 = lora.d.width * 2;
+                        mbar_arrive_expect_tx(bar_full + stage * 8, parts * width2 * (kBM + TOK));
+                        for (uint32_t i = 0; i < parts; ++i) {
+                            const int32_t rx = extra.next(lora.d);
+                            tma_load_2d(smem_base + C::kOffW + stage * C::kWBytes + i * kBM * width2, &lora.tm_b,
+                                        bar_full + stage * 8, rx, extra.b_row + static_cast<int32_t>(ni * kBM));
+                            tma_load_2d(smem_base + C::kOffT + stage * C::kTBytes + i * TOK * width2, &lora.tm_v,
+                                        bar_full + stage * 8, rx, extra.v_row);
+                        }
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                         continue;
                     }
                 }
+                mbar_arrive_expect_tx(bar_full + stage * 8, C::kStageBytes);
                 const int32_t kx = static_cast<int32_t>(kb * kBK);
                 tma_load_2d_hint(smem_base + C::kOffW + stage * C::kWBytes, &tm_w, bar_full + stage * 8, kx,
                                  static_cast<int32_t>(ni * kBM), pol_stream);
@@ -1624,19 +1658,22 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                 ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                 if (!ok) break;
                 tc_fence_after_sync();
-                uint32_t steps = kBK / kUmmaK;
                 if constexpr (LORA) {
                     const uint32_t info = stage_info[stage];
-                    steps = info & 7u;
                     last = (info & kLoraLast) != 0;
+                    if (info >> 4) {
+                        lora_stage_mma<1>(tmem_base, smem_base + C::kOffW + stage * C::kWBytes,
+                                          smem_base + C::kOffT + stage * C::kTBytes, kBM, TOK, idesc, info, lora.d.width);
+                        umma_commit<1>(bar_empty + stage * 8);
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                        continue;
+                    }
                 }
                 const uint64_t dw = smem_desc_k_sw128(smem_base + C::kOffW + stage * C::kWBytes);
                 const uint64_t dt = smem_desc_k_sw128(smem_base + C::kOffT + stage * C::kTBytes);
 #pragma unroll
-                for (uint32_t k = 0; k < kBK / kUmmaK; ++k) {
-                    if (LORA && k >= steps) break;
+                for (uint32_t k = 0; k < kBK / kUmmaK; ++k)
                     umma_f16<1>(tmem_base, dw + 2 * k, dt + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
-                }
                 umma_commit<1>(bar_empty + stage * 8);
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
@@ -1785,11 +1822,13 @@ bool encode_tmap(CUtensorMap *tm, const void *base, int64_t rows, int64_t cols, 
     if (!enc) return false;
     cuuint64_t gdim[2] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows)};
     cuuint64_t gstride[1] = {static_cast<cuuint64_t>(ld) * 2};
-    cuuint32_t box[2] = {box_cols, box_rows};     // 64 columns: 128-byte swizzle; 32 columns: 64-byte swizzle
+    cuuint32_t box[2] = {box_cols, box_rows};     // 64, 32 or 16 columns: 128-, 64- or 32-byte swizzle
     cuuint32_t estr[2] = {1, 1};
     CUresult r = enc(tm, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
                      const_cast<void *>(base), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                     box_cols == 16   ? CU_TENSOR_MAP_SWIZZLE_32B
+                     : box_cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                      : CU_TENSOR_MAP_SWIZZLE_128B,
                      is_output ? CU_TENSOR_MAP_L2_PROMOTION_NONE : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS;
@@ -1803,7 +1842,7 @@ struct TmapKey {
     const void *base;
     int64_t rows, cols, ld;
     uint32_t box_rows;
-    uint32_t kind;   // bit 0: bf16, bit 1: output, bit 2: 32-column box
+    uint32_t kind;   // bit 0: bf16, bit 1: output, bit 2: 32-column box, bit 3: 16-column box
     bool operator==(const TmapKey &o) const {
         return base == o.base && rows == o.rows && cols == o.cols && ld == o.ld && box_rows == o.box_rows &&
                kind == o.kind;
@@ -1820,7 +1859,7 @@ bool make_tmap(CUtensorMap *tm, const void *base, int64_t rows, int64_t cols, in
                uint32_t box_rows, bool bf16, bool is_output, uint32_t box_cols = kBK) {
     thread_local TmapSlot cache[kTmapSlots] = {};
     const TmapKey key{base, rows, cols, ld, box_rows,
-                      (bf16 ? 1u : 0u) | (is_output ? 2u : 0u) | (box_cols == 32 ? 4u : 0u)};
+                      (bf16 ? 1u : 0u) | (is_output ? 2u : 0u) | (box_cols == 32 ? 4u : 0u) | (box_cols == 16 ? 8u : 0u)};
     uint64_t h = reinterpret_cast<uint64_t>(base) >> 8;
     h ^= static_cast<uint64_t>(rows) * 0x9E3779B97F4A7C15ull + static_cast<uint64_t>(cols) * 31 + box_rows + key.kind;
     TmapSlot &slot = cache[(h ^ (h >> 17)) % kTmapSlots];
@@ -1905,10 +1944,11 @@ bool fill_lora(LoraParam<true> *p, const GemmArgs &g, uint32_t v_rows, uint32_t 
     p->d = {l.ids, l.table, static_cast<const uint16_t *>(l.v), static_cast<const uint16_t *>(l.b),
             static_cast<const uint16_t *>(g.a), static_cast<const uint16_t *>(g.b), g.lda, g.ldb,
             static_cast<uint32_t>(g.k), static_cast<uint32_t>(g.n), static_cast<uint32_t>(l.rank),
-            static_cast<uint32_t>((l.rank + kBK - 1) / kBK), static_cast<uint32_t>(l.max_slots),
+            static_cast<uint32_t>((l.rank + kBK - 1) / kBK), l.rank <= 16 ? 16u : l.rank <= 32 ? 32u : 64u,
+            static_cast<uint32_t>(l.max_slots),
             static_cast<uint32_t>(l.group_rows), static_cast<uint32_t>(l.table_stride)};
-    return make_tmap(&p->tm_v, l.v, groups * l.max_slots * l.group_rows, l.rank, l.rank, v_rows, g.bf16, false) &&
-           make_tmap(&p->tm_b, l.b, l.adapters * g.n, l.rank, l.rank, b_rows, g.bf16, false);
+    return make_tmap(&p->tm_v, l.v, groups * l.max_slots * l.group_rows, l.rank, l.rank, v_rows, g.bf16, false, p->d.width) &&
+           make_tmap(&p->tm_b, l.b, l.adapters * g.n, l.rank, l.rank, b_rows, g.bf16, false, p->d.width);
 }
 
 // Launch attributes common to the three kernels: the cluster shape, and for a caller that chained this

@@ -6,6 +6,9 @@
 // launched under programmatic stream serialisation: it streams the shared weights while this kernel runs and waits for
 // it only in front of the tile's last block.
 //
+// Few tokens (at most 64) of small ranks take plain fp32 dot products (lora_dot_kernel): a handful of blocks without
+// set-up, a few microseconds, beside which the GEMM's CTAs fit on the same SMs.  Otherwise the tensor cores:
+//
 // Down projection, per 128 rows of a (one tile): the adapters that occur in the tile's group of rows are listed in the
 // order of their first row; their A_i, `rank` rows of k elements each, stand below one another as the second operand,
 // cut into chunks of 64 rows.  One cluster per tile and chunk computes 128 x 64 with tcgen05 (every row of a against
@@ -22,6 +25,7 @@
 #include "host_util.h"
 #include "lora.h"
 #include "ptx.cuh"
+#include "rms_vec.cuh"
 
 namespace pg {
 
@@ -124,7 +128,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     if (rank == 0 && blockIdx.y == 0 && row0 == group0) {
         int32_t *t = p.table + static_cast<size_t>(group) * p.table_stride;
         if (threadIdx.x == 0) t[0] = static_cast<int32_t>(n_slots);
-        for (uint32_t i = threadIdx.x; i < n_slots; i += kThreads) t[4 + i] = slots[i];
+        for (uint32_t i = threadIdx.x; i < n_slots; i += kThreads) t[1 + i] = slots[i];
     }
     __syncwarp();              // the cluster barrier wants whole warps
     cluster_arrive();          // every CTA of the cluster is running before anyone writes into its shared memory
@@ -250,6 +254,84 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     }
 }
 
+constexpr uint32_t kDotRanks = 4;        // rank elements of a block: its loads of a token's row serve all of them
+constexpr uint32_t kDotWarps = 8;
+
+// v of one token and kDotRanks rank elements; one group of at most 64 rows.  Bound by latency: every load of a thread is
+// in flight at once for k up to 2048, the row's adapter is read in parallel with the group's list.
+template <bool BF16>
+__global__ void __launch_bounds__(kDotWarps * 32)
+lora_dot_kernel(const uint4 *x, int64_t ldx8, const uint4 *a, const Shrink p) {
+    __shared__ int32_t slots[64];
+    __shared__ uint32_t s_count;
+    __shared__ float red[kDotWarps][kDotRanks];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t t = blockIdx.y, r0 = blockIdx.x * kDotRanks;
+    const auto checked = [&](int32_t id) { return id >= 0 && static_cast<uint32_t>(id) < p.adapters ? id : -1; };
+    const int32_t id = checked(p.ids[t]);
+    if (warp == 0) {                     // the distinct ids in the order of their first row
+        uint32_t n = 0;
+        for (uint32_t r = 0; r < p.m; r += 32) {
+            const int32_t mine = r + lane < p.m ? checked(p.ids[r + lane]) : -1;
+            const uint32_t same = __match_any_sync(0xffffffffu, mine);       // every lane takes part
+            bool fresh = mine >= 0 && __ffs(same) - 1 == static_cast<int>(lane);
+            for (uint32_t e = 0; e < n; ++e) fresh = fresh && slots[e] != mine;
+            const uint32_t who = __ballot_sync(0xffffffffu, fresh);
+            if (fresh) slots[n + __popc(who & ((1u << lane) - 1u))] = mine;
+            n += __popc(who);
+            __syncwarp();
+        }
+        if (lane == 0) s_count = n;
+    }
+    float sum[kDotRanks] = {};
+    if (id >= 0) {
+        const uint32_t k8 = p.k / 8;
+        const uint4 *xr = x + t * ldx8, *ar = a + (static_cast<int64_t>(id) * p.rank + r0) * k8;
+#pragma unroll 2
+        for (uint32_t i = threadIdx.x; i < k8; i += kDotWarps * 32) {
+            const uint4 xv = __ldg(xr + i);
+            uint4 av[kDotRanks];
+#pragma unroll
+            for (uint32_t r = 0; r < kDotRanks; ++r) av[r] = __ldg(ar + static_cast<int64_t>(r) * k8 + i);
+            float f[8], g[8];
+            vec_unpack<BF16>(xv, f);
+#pragma unroll
+            for (uint32_t r = 0; r < kDotRanks; ++r) {
+                vec_unpack<BF16>(av[r], g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[r] = fmaf(f[e], g[e], sum[r]);
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t r = 0; r < kDotRanks; ++r) sum[r] = warp_sum_f32(sum[r]);
+    if (lane == 0)
+#pragma unroll
+        for (uint32_t r = 0; r < kDotRanks; ++r) red[warp][r] = sum[r];
+    __syncthreads();
+    const uint32_t n = s_count;
+    if (blockIdx.x == 0 && t == 0) {
+        if (threadIdx.x == 0) p.table[0] = static_cast<int32_t>(n);
+        for (uint32_t i = threadIdx.x; i < n; i += kDotWarps * 32) p.table[1 + i] = slots[i];
+    }
+    // the row of every slot: the scaled value, rounded once, in the slot of the row's adapter, zeros in the others
+    if (threadIdx.x < n) {
+        uint2 out = make_uint2(0, 0);
+        if (slots[threadIdx.x] == id) {
+            const float scale = p.scale ? p.scale[id] : 1.f;
+            float v[kDotRanks] = {};
+#pragma unroll
+            for (uint32_t w = 0; w < kDotWarps; ++w)
+#pragma unroll
+                for (uint32_t r = 0; r < kDotRanks; ++r) v[r] += red[w][r];
+            out = make_uint2(pack2<BF16>(v[0] * scale, v[1] * scale), pack2<BF16>(v[2] * scale, v[3] * scale));
+        }
+        reinterpret_cast<uint2 *>(p.v)[((static_cast<int64_t>(threadIdx.x) * p.group_rows + t) * p.rank + r0) / 4] = out;
+    }
+}
+
 struct Plan {
     int64_t group_rows, groups, max_slots, table_stride, v_rows;
     size_t off_v, bytes;
@@ -260,11 +342,31 @@ Plan make_plan(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank, 
     p.group_rows = lora_group_rows(m, n, k, sms);
     p.groups = (m + p.group_rows - 1) / p.group_rows;
     p.max_slots = adapters < p.group_rows ? adapters : p.group_rows;
-    p.table_stride = 4 + p.max_slots;
+    p.table_stride = (1 + p.max_slots + 3) / 4 * 4;
     p.v_rows = p.groups * p.max_slots * p.group_rows;
     p.off_v = (static_cast<size_t>(p.groups) * p.table_stride * 4 + 255) / 256 * 256;
     p.bytes = p.off_v + static_cast<size_t>(p.v_rows) * rank * 2;
     return p;
+}
+
+// Dot products read an adapter's rows once for every token: up to 32 MiB of them.
+bool dot_pays(int64_t m, int64_t k, int64_t rank) {
+    static const int env = tune_env_int("PEAKGEMM_TUNE_LORA_DOT_MB", 32);
+    return m * k * rank * 2 <= static_cast<int64_t>(env) << 20;
+}
+
+// CTAs of a cluster over k.  Beside the persistent GEMM kernels (which need whole SMs) as few as will do: the down
+// projection has the time of a tile's own k-blocks, about 0.38 us each, and every SM it occupies starts its tiles late;
+// a CTA takes about 5 us and 0.27 us a k-block.  Beside the others, whose CTAs are done soon, as many as fit.
+int64_t choose_split(int64_t tiles, int64_t k_blocks, int64_t group_rows, int sms) {
+    static const int env = tune_env_int("PEAKGEMM_TUNE_LORA_SPLIT", 0);
+    if (env > 0) return env;
+    int64_t split = 1;
+    while (split < 8 && tiles * split * 2 <= sms && k_blocks >= 8 * split) {
+        if (group_rows >= 256 && 5.0 + 0.27 * static_cast<double>(k_blocks) / split <= 0.38 * static_cast<double>(k_blocks)) break;
+        split *= 2;
+    }
+    return split;
 }
 
 }  // namespace
@@ -291,39 +393,46 @@ int hgemm_lora_launch(const GemmArgs &g, const LoraArgs &l, cudaStream_t stream,
     Shrink s = {l.ids, l.scale, table, reinterpret_cast<uint4 *>(v), static_cast<uint32_t>(g.m), static_cast<uint32_t>(g.k),
                 static_cast<uint32_t>(l.adapters), static_cast<uint32_t>(l.rank), static_cast<uint32_t>(p.max_slots),
                 static_cast<uint32_t>(p.group_rows), static_cast<uint32_t>(p.table_stride), 8};
-    while (s.piece < kChunk && l.rank % (2 * s.piece) == 0) s.piece *= 2;
-    CUtensorMap tm_x, tm_a;
-    if (!gemm_operand_map(&tm_x, g.a, g.m, g.k, g.lda, kBM, g.bf16) ||
-        !gemm_operand_map(&tm_a, l.a, l.adapters * l.rank, g.k, g.k, s.piece, g.bf16))
-        return failed(cudaErrorInvalidValue);
-    // The largest cluster over k that keeps the tiles within one wave and leaves every CTA four k-blocks.
-    const int64_t tiles = (g.m + kBM - 1) / kBM, k_blocks = (g.k + kBK - 1) / kBK;
-    int64_t split = 1;
-    while (split < 8 && tiles * split * 2 <= sms && k_blocks >= 8 * split) split *= 2;
-    // Clusters for as many chunks as there can be, up to two waves of CTAs; those without a chunk leave at once.
-    int64_t chunks = (p.max_slots < g.m ? p.max_slots : g.m) * l.rank;
-    chunks = (chunks + kChunk - 1) / kChunk;
-    const int64_t most = 2 * sms / (tiles * split);
-    if (chunks > most) chunks = most < 1 ? 1 : most;
-
-    auto kernel = g.bf16 ? lora_shrink_kernel<true> : lora_shrink_kernel<false>;
-    static DeviceOnce once[2];
-    if ((e = allow_dynamic_smem(once[g.bf16 ? 1 : 0], kernel, kSmem)) != cudaSuccess) return failed(e);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * split), static_cast<unsigned>(chunks), 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = kSmem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    if ((e = cudaLaunchKernelEx(&cfg, kernel, tm_x, tm_a, s, status)) != cudaSuccess) return failed(e);
+    cfg.numAttrs = 1;
+    if (p.group_rows <= 64 && dot_pays(g.m, g.k, l.rank)) {
+        cfg.gridDim = dim3(static_cast<unsigned>(l.rank / kDotRanks), static_cast<unsigned>(g.m), 1);
+        cfg.blockDim = dim3(kDotWarps * 32, 1, 1);
+        if ((e = cudaLaunchKernelEx(&cfg, g.bf16 ? lora_dot_kernel<true> : lora_dot_kernel<false>,
+                                    static_cast<const uint4 *>(g.a), g.lda / 8, static_cast<const uint4 *>(l.a), s)) != cudaSuccess)
+            return failed(e);
+    } else {
+        while (s.piece < kChunk && l.rank % (2 * s.piece) == 0) s.piece *= 2;
+        CUtensorMap tm_x, tm_a;
+        if (!gemm_operand_map(&tm_x, g.a, g.m, g.k, g.lda, kBM, g.bf16) ||
+            !gemm_operand_map(&tm_a, l.a, l.adapters * l.rank, g.k, g.k, s.piece, g.bf16))
+            return failed(cudaErrorInvalidValue);
+        const int64_t tiles = (g.m + kBM - 1) / kBM;
+        const int64_t split = choose_split(tiles, (g.k + kBK - 1) / kBK, p.group_rows, sms);
+        // Clusters for as many chunks as there can be, up to two waves of CTAs; those without a chunk leave at once.
+        int64_t chunks = (p.max_slots < g.m ? p.max_slots : g.m) * l.rank;
+        chunks = (chunks + kChunk - 1) / kChunk;
+        const int64_t most = 2 * sms / (tiles * split);
+        if (chunks > most) chunks = most < 1 ? 1 : most;
+
+        auto kernel = g.bf16 ? lora_shrink_kernel<true> : lora_shrink_kernel<false>;
+        static DeviceOnce once[2];
+        if ((e = allow_dynamic_smem(once[g.bf16 ? 1 : 0], kernel, kSmem)) != cudaSuccess) return failed(e);
+        cfg.gridDim = dim3(static_cast<unsigned>(tiles * split), static_cast<unsigned>(chunks), 1);
+        cfg.blockDim = dim3(kThreads, 1, 1);
+        cfg.dynamicSmemBytes = kSmem;
+        attr[1].id = cudaLaunchAttributeClusterDimension;
+        attr[1].val.clusterDim.x = static_cast<unsigned>(split);
+        attr[1].val.clusterDim.y = 1;
+        attr[1].val.clusterDim.z = 1;
+        cfg.numAttrs = 2;
+        if ((e = cudaLaunchKernelEx(&cfg, kernel, tm_x, tm_a, s, status)) != cudaSuccess) return failed(e);
+    }
 
     const LoraGemm lg = {l.ids, table, v, l.b, l.adapters, l.rank, p.max_slots, p.group_rows, p.table_stride};
     GemmArgs with = g;

@@ -1,11 +1,15 @@
 // The adapters inside the GEMM kernels of gemm_sm100.cu.
 //
 // The up projection is more k: with v[t] = scale * x[t] A^T (lora.cu) a tile's accumulator gets, behind the k-blocks of
-// x W^T, one k-block of up to 64 rank elements for every adapter that occurs among the tile's rows:
+// x W^T, the rank elements of every adapter that occurs among the tile's rows:
 //     acc[t, j] += sum_r V[t, r] B_i[j, r],     V = v for the rows t that use adapter i, zeros for the others.
 // The contribution is added in fp32 before the one rounding, and the output is neither read again nor written twice.
 // A tile's rows form a group; lora.cu writes the group's adapters in the order of their first row ("slots") into a table
 // and the masked V of each slot, [group rows, rank], next to it.
+// A stage of the operand ring takes 64 elements of k: one block of a rank over 32, two adapters of a rank up to 32, four
+// of a rank up to 16.  Each is a part of its own in the stage, 64, 32 or 16 elements wide, with the swizzle of that
+// width (128, 64 or 32 bytes).  With one adapter per stage the ring held 6 KiB where it holds 24: 64 x 14336 x 4096, rank
+// 16, 32 adapters in the batch, 44.6 us.
 #pragma once
 
 #include <cuda.h>
@@ -19,12 +23,12 @@ namespace {
 
 struct LoraDev {
     const int32_t *ids;         // [m]
-    const int32_t *table;       // per group table_stride words: the number of slots, 3 unused words, the slots' adapters
+    const int32_t *table;       // per group table_stride words: the number of slots, then the slots' adapters
     const uint16_t *v;          // [groups][max_slots][group_rows][rank]
     const uint16_t *b;          // [adapters][n][rank]
     const uint16_t *x, *w;      // the product's operands
     int64_t ldx, ldw;
-    uint32_t k, n, rank, rank_blocks, max_slots, group_rows, table_stride;
+    uint32_t k, n, rank, rank_blocks, width, max_slots, group_rows, table_stride;     // width: of a part, 16, 32 or 64
 };
 
 template <bool LORA> struct LoraParam {};
@@ -33,36 +37,46 @@ template <> struct LoraParam<true> {
     LoraDev d;
 };
 
-// What a stage holds, written by the producer before it arms the stage: the number of 16-element steps of k, and
-// whether the tile ends with it.
+// What a stage holds, written by the producer before it arms the stage: bits 0-2 the 16-element steps of k in a part,
+// bit 3 whether the tile ends with the stage, bits 4-6 the number of adapter parts (0: a block of the product).
 constexpr uint32_t kLoraLast = 8u;
 
-// The producer's walk over a tile's adapter blocks: `count` of them, slots first, first + step, ...
+// The producer's walk over a tile's adapters: slots first, first + step, ..., in `count` stages.
 struct LoraBlocks {
-    uint32_t count = 0, slot = 0, slot_step = 1, rb = 0, base = 0;
+    uint32_t count = 0, slot = 0, slot_step = 1, slots = 0, rb = 0, base = 0;
+    int4 head = {0, 0, 0, 0};          // the table's first words: the number of slots and three adapters
     const int32_t *adapters = nullptr;
-    int32_t v_row = 0, b_row = 0;      // of the block that next() returned
+    int32_t v_row = 0, b_row = 0;      // of the part that next() returned
 
-    __device__ __forceinline__ void open(const LoraDev &d, uint32_t group, uint32_t first = 0, uint32_t step = 1) {
+    __device__ __forceinline__ void load(const LoraDev &d, uint32_t group) {
         const int32_t *t = d.table + static_cast<size_t>(group) * d.table_stride;
-        const uint32_t n = min(static_cast<uint32_t>(t[0]), d.max_slots);
-        adapters = t + 4;
+        head = *reinterpret_cast<const int4 *>(t);
+        adapters = t + 1;
+        base = group * d.max_slots;
+    }
+    __device__ __forceinline__ void open(const LoraDev &d, uint32_t first = 0, uint32_t step = 1) {
+        slots = min(static_cast<uint32_t>(head.x), d.max_slots);
         slot = first;
         slot_step = step;
         rb = 0;
-        base = group * d.max_slots;
-        count = n > first ? (n - first + step - 1) / step * d.rank_blocks : 0u;
+        const uint32_t mine = slots > first ? (slots - first + step - 1) / step : 0u, pack = kBK / d.width;
+        count = pack > 1 ? (mine + pack - 1) / pack : mine * d.rank_blocks;
+    }
+    // Parts of the stage that next() will fill.
+    __device__ __forceinline__ uint32_t parts(const LoraDev &d) const {
+        return min(kBK / d.width, (slots - slot + slot_step - 1) / slot_step);
     }
     // The word of the stage that block kb goes to (block kb1 - 1 is the product's last).
     __device__ __forceinline__ uint32_t info(const LoraDev &d, uint32_t kb, uint32_t kb1) const {
         const uint32_t last = kb + 1 >= kb1 && kb + 1 - kb1 == count ? kLoraLast : 0u;
         if (kb < kb1) return kBK / kUmmaK | last;
-        return min(kBK, d.rank - rb * kBK + kUmmaK - 1) / kUmmaK | last;
+        return min(d.width, d.rank - rb * kBK + kUmmaK - 1) / kUmmaK | last | parts(d) << 4;
     }
-    // Moves to the next block; returns its first rank element.
+    // Moves to the next part; returns its first rank element.
     __device__ __forceinline__ int32_t next(const LoraDev &d) {
         v_row = static_cast<int32_t>((base + slot) * d.group_rows);
-        b_row = adapters[slot] * static_cast<int32_t>(d.n);
+        const int32_t adapter = slot == 0 ? head.y : slot == 1 ? head.z : slot == 2 ? head.w : adapters[slot];
+        b_row = adapter * static_cast<int32_t>(d.n);
         const int32_t x = static_cast<int32_t>(rb * kBK);
         if (++rb == d.rank_blocks) {
             rb = 0;
@@ -71,6 +85,18 @@ struct LoraBlocks {
         return x;
     }
 };
+
+// The MMAs of a stage of adapter parts: A's parts from smem_a, a_rows rows each, B's from smem_b, b_rows rows each.
+template <int CTA_GROUP>
+__device__ __forceinline__ void lora_stage_mma(uint32_t tmem_d, uint32_t smem_a, uint32_t smem_b, uint32_t a_rows,
+                                               uint32_t b_rows, uint32_t idesc, uint32_t info, uint32_t width) {
+    const uint32_t parts = info >> 4, steps = info & 7u;
+    for (uint32_t i = 0; i < parts; ++i) {
+        const uint64_t da = ptx::smem_desc_k(smem_a + i * a_rows * width * 2, width * 2);
+        const uint64_t db = ptx::smem_desc_k(smem_b + i * b_rows * width * 2, width * 2);
+        for (uint32_t k = 0; k < steps; ++k) ptx::umma_f16<CTA_GROUP>(tmem_d, da + 2 * k, db + 2 * k, idesc, 1u);
+    }
+}
 
 // A zero of V times an infinity or NaN in another row's adapter is NaN: such an element is computed again from its own
 // row's terms alone.  `acc` unless one of the group's other adapters holds such a value in this column.
@@ -83,7 +109,7 @@ __device__ __noinline__ float lora_exact(const LoraDev &d, uint32_t group, uint3
     const uint32_t r8 = d.rank / 8;
     float f[8], g[8];
     for (int32_t s = 0; s < slots; ++s) {
-        const int32_t a = t[4 + s];
+        const int32_t a = t[1 + s];
         if (a == id) {
             mine = s;
             continue;

@@ -281,6 +281,18 @@ __device__ __forceinline__ uint64_t smem_desc_k_sw128(uint32_t smem_addr) {
     return d;
 }
 
+// The same for rows of `bytes` = 32, 64 or 128 bytes with the swizzle of that width: 8-row groups 8 * bytes apart, layout
+// 6, 4 or 2.
+__device__ __forceinline__ uint64_t smem_desc_k(uint32_t smem_addr, uint32_t bytes) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
+    d |= static_cast<uint64_t>(1) << 16;
+    d |= static_cast<uint64_t>(bytes / 2) << 32;            // 8 * bytes >> 4
+    d |= static_cast<uint64_t>(1) << 46;
+    d |= static_cast<uint64_t>(bytes == 32 ? 6 : bytes == 64 ? 4 : 2) << 61;
+    return d;
+}
+
 // Instruction descriptor for tcgen05.mma.kind::f16 with fp32 accumulation:
 //   [4,6) D format: 1 = f32     [7,10) A format, [10,13) B format: 0 = f16, 1 = bf16
 //   bit 15 / bit 16: A / B major, 0 = K-major
