@@ -463,48 +463,13 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                 tile_coords(group_m, u.tile, m_tiles, n_tiles, mi, ni, (flags & kFlagSerpentine) != 0);
                 const int32_t row_a = static_cast<int32_t>(mi * kTileM + rank * kBM);    // + mt * kBlockM
                 const int32_t row_b = static_cast<int32_t>(ni * BN + rank * C::kBRows);
-                LoraBlocks extra;                    // the adapters' blocks behind the product's own
-                if constexpr (LORA)
-                    if (it > 0) extra.load(lora.d, mi);
-                for (uint32_t kb = u.kb0; kb < u.kb1 + extra.count; ++kb) {
-                    const bool own = !LORA || kb < u.kb1;
-                    if constexpr (LORA) {
-                        // The last block of the product has to know whether the tile ends with it: from here on the
-                        // down projections must be there.
-                        if (kb + 1 == u.kb1) {
-                            if (it == 0) {
-                                asm volatile("griddepcontrol.wait;" ::: "memory");
-                                extra.load(lora.d, mi);
-                            }
-                            extra.open(lora.d);
-                        }
-                    }
-                    if (own && tail.wave_sync != nullptr && leader) {
-                        // Synchronisation points of the producers (the first k-block of every tile and every
-                        // sync_kb-th after it): a worker announces that it has reached the point, and sync_lag
-                        // k-blocks later waits until every worker of this wave of tiles has.  Workers that share an
-                        // A or a B panel therefore ask for the same k-block within a few k-block times of each
-                        // other: one's fetch from DRAM is the others' L2 hit, or is merged with theirs on the way to
-                        // L2.  The lag hides the counter's round trip behind loads that are already allowed.  (The
-                        // peer CTA's producer is paced by the relayed empty[s].)
-                        const uint32_t rel = kb - u.kb0;
-                        if (rel == 0 || (tail.sync_kb != 0 && rel % tail.sync_kb == 0)) {
-                            red_relaxed_gpu_add(tail.wave_sync, 1u);
-                            sync_target += min(workers, total_tiles - it * workers);
-                            sync_wait_at = kb + tail.sync_lag;
-                        }
-                        // (letting a wait end when all but 4-37 workers had arrived was measured: no gain)
-                        if (kb == sync_wait_at && sync_waits) sync_waits = wait_count_patiently(tail.wave_sync, sync_target);
-                    }
+                // The stage's MMAs have completed: hand the stage to the peer too and arm it with `bytes` of each CTA.
+                const auto take_stage = [&](uint32_t bytes, uint32_t info) {
                     if (leader) {
                         // wait until the MMAs that read this stage have completed
                         ok = wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty);
-                        if (!ok) break;
-                        uint32_t bytes = C::kStageBytes;             // of one CTA
-                        if constexpr (LORA) {
-                            stage_info[stage] = extra.info(lora.d, kb, u.kb1);
-                            if (!own) bytes = C::kStageBytes / kBK * lora.d.width * extra.parts(lora.d);
-                        }
+                        if (!ok) return;
+                        if (info) stage_info[stage] = info;
                         if constexpr (CTA_GROUP == 2) {
                             mbar_arrive_cluster(peer_empty0 + stage * 8);   // relay to the peer
                             mbar_arrive_expect_tx(bar_full + stage * 8, 2 * bytes);
@@ -513,32 +478,13 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                         }
                     } else {
                         ok = wait_bar(bar_empty + stage * 8, phase, ctx, kStProducerEmpty);
-                        if (!ok) break;
                     }
+                };
+                const auto load_block = [&](uint32_t kb) {
                     const uint32_t dst_a = smem_base + C::kOffA + stage * C::kABytes;
                     const uint32_t dst_b = smem_base + C::kOffB + stage * C::kBBytes;
                     const int32_t kx = static_cast<int32_t>(kb * kBK);
                     const uint32_t fb = (CTA_GROUP == 2) ? full0 + stage * 8 : bar_full + stage * 8;
-                    if constexpr (LORA) {
-                        if (!own) {
-                            const uint32_t parts = extra.parts(lora.d), width2 = lora.d.width * 2;
-                            for (uint32_t i = 0; i < parts; ++i) {
-                                const int32_t rx = extra.next(lora.d);
-#pragma unroll
-                                for (uint32_t mt = 0; mt < MT; ++mt) {
-                                    const uint32_t da = dst_a + mt * C::kABox + i * kBM * width2;
-                                    const int32_t rv = extra.v_row + static_cast<int32_t>(mt * kBlockM + rank * kBM);
-                                    if constexpr (CTA_GROUP == 2) tma_load_2d_pair(da, &lora.tm_v, fb, rx, rv);
-                                    else tma_load_2d(da, &lora.tm_v, fb, rx, rv);
-                                }
-                                const uint32_t db = dst_b + i * C::kBRows * width2;
-                                if constexpr (CTA_GROUP == 2) tma_load_2d_pair(db, &lora.tm_b, fb, rx, extra.b_row + row_b);
-                                else tma_load_2d(db, &lora.tm_b, fb, rx, extra.b_row + row_b);
-                            }
-                            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-                            continue;
-                        }
-                    }
 #pragma unroll
                     for (uint32_t mt = 0; mt < MT; ++mt) {
                         const uint32_t da = dst_a + mt * C::kABox;
@@ -559,6 +505,67 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                         else tma_load_2d(dst_b, &tm_b, fb, kx, row_b);
                     }
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                };
+                LoraBlocks extra;                    // the adapters' blocks behind the product's own
+                if constexpr (LORA)
+                    if (it > 0) extra.load(lora.d, mi);
+                // With adapters the last block is taken apart below: in the loop, the few instructions that ask for it
+                // took the one producing thread longer than the tensor cores take for the block.
+                const uint32_t plain_end = LORA ? u.kb1 - 1 : u.kb1;
+                for (uint32_t kb = u.kb0; kb < plain_end; ++kb) {
+                    if (tail.wave_sync != nullptr && leader) {
+                        // Synchronisation points of the producers (the first k-block of every tile and every
+                        // sync_kb-th after it): a worker announces that it has reached the point, and sync_lag
+                        // k-blocks later waits until every worker of this wave of tiles has.  Workers that share an
+                        // A or a B panel therefore ask for the same k-block within a few k-block times of each
+                        // other: one's fetch from DRAM is the others' L2 hit, or is merged with theirs on the way to
+                        // L2.  The lag hides the counter's round trip behind loads that are already allowed.  (The
+                        // peer CTA's producer is paced by the relayed empty[s].)
+                        const uint32_t rel = kb - u.kb0;
+                        if (rel == 0 || (tail.sync_kb != 0 && rel % tail.sync_kb == 0)) {
+                            red_relaxed_gpu_add(tail.wave_sync, 1u);
+                            sync_target += min(workers, total_tiles - it * workers);
+                            sync_wait_at = kb + tail.sync_lag;
+                        }
+                        // (letting a wait end when all but 4-37 workers had arrived was measured: no gain)
+                        if (kb == sync_wait_at && sync_waits) sync_waits = wait_count_patiently(tail.wave_sync, sync_target);
+                    }
+                    take_stage(C::kStageBytes, 0u);
+                    if (!ok) break;
+                    load_block(kb);
+                }
+                if constexpr (LORA) {
+                    if (!ok) break;
+                    // The product's last block has to say whether the tile ends with it: here the down projections
+                    // must be there.
+                    if (it == 0) {
+                        asm volatile("griddepcontrol.wait;" ::: "memory");
+                        extra.load(lora.d, mi);
+                    }
+                    extra.open(lora.d);
+                    take_stage(C::kStageBytes, extra.info(lora.d, u.kb1 - 1, u.kb1));
+                    if (!ok) break;
+                    load_block(u.kb1 - 1);
+                    for (uint32_t kb = u.kb1; kb < u.kb1 + extra.count; ++kb) {
+                        const uint32_t parts = extra.parts(lora.d), width2 = lora.d.width * 2;
+                        take_stage(C::kStageBytes / (2 * kBK) * width2 * parts, extra.info(lora.d, kb, u.kb1));
+                        if (!ok) break;
+                        const uint32_t fb = (CTA_GROUP == 2) ? full0 + stage * 8 : bar_full + stage * 8;
+                        for (uint32_t i = 0; i < parts; ++i) {
+                            const int32_t rx = extra.next(lora.d);
+#pragma unroll
+                            for (uint32_t mt = 0; mt < MT; ++mt) {
+                                const uint32_t da = smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox + i * kBM * width2;
+                                const int32_t rv = extra.v_row + static_cast<int32_t>(mt * kBlockM + rank * kBM);
+                                if constexpr (CTA_GROUP == 2) tma_load_2d_pair(da, &lora.tm_v, fb, rx, rv);
+                                else tma_load_2d(da, &lora.tm_v, fb, rx, rv);
+                            }
+                            const uint32_t db = smem_base + C::kOffB + stage * C::kBBytes + i * C::kBRows * width2;
+                            if constexpr (CTA_GROUP == 2) tma_load_2d_pair(db, &lora.tm_b, fb, rx, extra.b_row + row_b);
+                            else tma_load_2d(db, &lora.tm_b, fb, rx, extra.b_row + row_b);
+                        }
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    }
                 }
             }
         }
@@ -578,26 +585,13 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     if (!ok) break;
                     tc_fence_after_sync();
                 }
-                bool last = false;
-                for (uint32_t kb = u.kb0; LORA ? !last : kb < u.kb1; ++kb) {
+                bool last = !LORA;
+                for (uint32_t kb = u.kb0; kb < u.kb1; ++kb) {
                     ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                     if (!ok) break;
                     tc_fence_after_sync();
-                    if constexpr (LORA) {
-                        const uint32_t info = stage_info[stage];
-                        last = (info & kLoraLast) != 0;
-                        if (info >> 4) {
-#pragma unroll
-                            for (uint32_t mt = 0; mt < MT; ++mt)
-                                lora_stage_mma<CTA_GROUP>(tmem_base + (MT == 2 ? mt : acc) * BN,
-                                                          smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox,
-                                                          smem_base + C::kOffB + stage * C::kBBytes, kBM, C::kBRows, idesc,
-                                                          info, lora.d.width);
-                            umma_commit<CTA_GROUP>(bar_empty + stage * 8);
-                            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-                            continue;
-                        }
-                    }
+                    if constexpr (LORA)
+                        if (kb + 1 == u.kb1) last = (stage_info[stage] & kLoraLast) != 0;
                     const uint64_t db = smem_desc_k_sw128(smem_base + C::kOffB + stage * C::kBBytes);
 #pragma unroll
                     for (uint32_t mt = 0; mt < MT; ++mt) {
@@ -622,6 +616,23 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     if (!ok) break;
                     umma_commit<CTA_GROUP>(bar_empty + stage * 8);   // stage free once these MMAs are done
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+                if constexpr (LORA) {
+                    while (ok && !last) {            // the adapters' stages
+                        ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        const uint32_t info = stage_info[stage];
+                        last = (info & kLoraLast) != 0;
+#pragma unroll
+                        for (uint32_t mt = 0; mt < MT; ++mt)
+                            lora_stage_mma<CTA_GROUP>(tmem_base + (MT == 2 ? mt : acc) * BN,
+                                                      smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox,
+                                                      smem_base + C::kOffB + stage * C::kBBytes, kBM, C::kBRows, idesc,
+                                                      info & 0x77u, lora.d.width);
+                        umma_commit<CTA_GROUP>(bar_empty + stage * 8);
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    }
                 }
                 if (!ok) break;
 #ifdef PG_TEST_SHORT_WAIT
@@ -1083,7 +1094,7 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 }
                 if (!wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty)) break;
                 if constexpr (LORA) {
-                    stage_info[stage] = extra.info(lora.d, kb, kb1);
+                    if (kb + 1 >= kb1) stage_info[stage] = extra.info(lora.d, kb, kb1);
                     if (kb >= kb1) {
                         const uint32_t parts = extra.parts(lora.d), width2 = lora.d.width * 2;
                         mbar_arrive_expect_tx(bar_full + stage * 8, parts * width2 * (kBM + BN));
@@ -1113,22 +1124,13 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             constexpr uint32_t idesc = instr_desc_f16(BF16, kBM, BN);
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            bool last = false;
-            for (uint32_t kb = kb0; LORA ? !last : kb < kb1; ++kb) {
+            bool last = !LORA;
+            for (uint32_t kb = kb0; kb < kb1; ++kb) {
                 ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                 if (!ok) break;
                 tc_fence_after_sync();
-                if constexpr (LORA) {
-                    const uint32_t info = stage_info[stage];
-                    last = (info & kLoraLast) != 0;
-                    if (info >> 4) {
-                        lora_stage_mma<1>(tmem_base, smem_base + C::kOffA + stage * C::kABytes,
-                                          smem_base + C::kOffB + stage * C::kBBytes, kBM, BN, idesc, info, lora.d.width);
-                        umma_commit<1>(bar_empty + stage * 8);
-                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-                        continue;
-                    }
-                }
+                if constexpr (LORA)
+                    if (kb + 1 == kb1) last = (stage_info[stage] & kLoraLast) != 0;
                 const uint64_t da = smem_desc_k_sw128(smem_base + C::kOffA + stage * C::kABytes);
                 const uint64_t db = smem_desc_k_sw128(smem_base + C::kOffB + stage * C::kBBytes);
 #pragma unroll
@@ -1136,6 +1138,19 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     umma_f16<1>(tmem_base, da + 2 * k, db + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
                 umma_commit<1>(bar_empty + stage * 8);
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+            if constexpr (LORA) {
+                while (ok && !last) {                // the adapters' stages
+                    ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const uint32_t info = stage_info[stage];
+                    last = (info & kLoraLast) != 0;
+                    lora_stage_mma<1>(tmem_base, smem_base + C::kOffA + stage * C::kABytes,
+                                      smem_base + C::kOffB + stage * C::kBBytes, kBM, BN, idesc, info & 0x77u, lora.d.width);
+                    umma_commit<1>(bar_empty + stage * 8);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
             }
             if (ok) umma_commit<1>(bar_acc_full);
         }
@@ -1623,7 +1638,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                 }
                 if (!wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty)) break;
                 if constexpr (LORA) {
-                    stage_info[stage] = extra.info(lora.d, kb, kb1);
+                    if (kb + 1 >= kb1) stage_info[stage] = extra.info(lora.d, kb, kb1);
                     if (kb >= kb1) {
                         const uint32_t parts = extra.parts(lora.d), width2 = lora.d.width * 2;
                         mbar_arrive_expect_tx(bar_full + stage * 8, parts * width2 * (kBM + TOK));
@@ -1653,22 +1668,13 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
             constexpr uint32_t idesc = instr_desc_f16(BF16, kBM, TOK);
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            bool last = false;
-            for (uint32_t kb = kb0; LORA ? !last : kb < kb1; ++kb) {
+            bool last = !LORA;
+            for (uint32_t kb = kb0; kb < kb1; ++kb) {
                 ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                 if (!ok) break;
                 tc_fence_after_sync();
-                if constexpr (LORA) {
-                    const uint32_t info = stage_info[stage];
-                    last = (info & kLoraLast) != 0;
-                    if (info >> 4) {
-                        lora_stage_mma<1>(tmem_base, smem_base + C::kOffW + stage * C::kWBytes,
-                                          smem_base + C::kOffT + stage * C::kTBytes, kBM, TOK, idesc, info, lora.d.width);
-                        umma_commit<1>(bar_empty + stage * 8);
-                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-                        continue;
-                    }
-                }
+                if constexpr (LORA)
+                    if (kb + 1 == kb1) last = (stage_info[stage] & kLoraLast) != 0;
                 const uint64_t dw = smem_desc_k_sw128(smem_base + C::kOffW + stage * C::kWBytes);
                 const uint64_t dt = smem_desc_k_sw128(smem_base + C::kOffT + stage * C::kTBytes);
 #pragma unroll
@@ -1676,6 +1682,19 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                     umma_f16<1>(tmem_base, dw + 2 * k, dt + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
                 umma_commit<1>(bar_empty + stage * 8);
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+            if constexpr (LORA) {
+                while (ok && !last) {                // the adapters' stages
+                    ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const uint32_t info = stage_info[stage];
+                    last = (info & kLoraLast) != 0;
+                    lora_stage_mma<1>(tmem_base, smem_base + C::kOffW + stage * C::kWBytes,
+                                      smem_base + C::kOffT + stage * C::kTBytes, kBM, TOK, idesc, info & 0x77u, lora.d.width);
+                    umma_commit<1>(bar_empty + stage * 8);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
             }
             if (ok) umma_commit<1>(bar_acc_full);
         }
