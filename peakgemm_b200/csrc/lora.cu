@@ -34,19 +34,24 @@ using namespace ptx;
 namespace {
 
 constexpr uint32_t kChunk = 64;              // columns (adapter rows) of a tile
-constexpr uint32_t kStages = 4;
 constexpr uint32_t kXBytes = kBM * kBK * 2;
 constexpr uint32_t kWBytes = kChunk * kBK * 2;
 constexpr uint32_t kMaxGroup = 512;
-constexpr uint32_t kOffX = 0;
-constexpr uint32_t kOffW = kOffX + kStages * kXBytes;
-constexpr uint32_t kOffRecv = kOffW + kStages * kWBytes;        // [S slots][64/S/4][128 rows][4] fp32
-constexpr uint32_t kOffBar = kOffRecv + kBM * kChunk * 4;       // full[], empty[], acc_full
-constexpr uint32_t kOffMisc = kOffBar + (2 * kStages + 1) * 8;  // tensor-memory slot, abort flag, slot count
-constexpr uint32_t kOffPiece = kOffMisc + 16;                   // first row of A of each piece of the chunk
-constexpr uint32_t kOffIds = kOffPiece + 8 * 4;                 // the group's adapter ids, -1: none
-constexpr uint32_t kOffSlots = kOffIds + kMaxGroup * 4;         // the adapters that occur
-constexpr uint32_t kSmem = kOffSlots + kMaxGroup * 4 + 1024;
+
+// STAGES 3: two CTAs fit on an SM; 7: one, with twice the bytes in flight of its own.
+template <int STAGES>
+struct ShrinkSmem {
+    static constexpr uint32_t kX = 0;
+    static constexpr uint32_t kW = kX + STAGES * kXBytes;
+    static constexpr uint32_t kRecv = kW + STAGES * kWBytes;        // [S slots][64/S/4][128 rows][4] fp32
+    static constexpr uint32_t kBar = kRecv + kBM * kChunk * 4;      // full[], empty[], acc_full
+    static constexpr uint32_t kMisc = kBar + (2 * STAGES + 1) * 8;  // tensor-memory slot, abort flag, slot count
+    static constexpr uint32_t kPiece = kMisc + 16;                  // first row of A of each piece of the chunk
+    static constexpr uint32_t kIds = kPiece + 8 * 4;                // the group's adapter ids, -1: none
+    static constexpr uint32_t kSlots = kIds + kMaxGroup * 4;        // the adapters that occur
+    static constexpr uint32_t kBytes = kSlots + kMaxGroup * 4 + 1024;
+    static_assert(kBytes <= (STAGES == 3 ? 115712u : 232448u), "shared memory");
+};
 
 struct Shrink {
     const int32_t *ids;
@@ -57,10 +62,12 @@ struct Shrink {
     uint32_t piece;                // rows of A per load: 8 .. 64, divides rank and 64
 };
 
-template <bool BF16>
+template <int STAGES, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
 lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a, const Shrink p,
                    int *status) {
+    using L = ShrinkSmem<STAGES>;
+    constexpr uint32_t kStages = STAGES;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -68,12 +75,12 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t S = cluster_nctarank(), rank = cluster_ctarank();
     const uint32_t cols = kChunk / S;                                  // columns this CTA finally owns
-    const uint32_t bar_full = smem_base + kOffBar, bar_empty = bar_full + kStages * 8, bar_acc = bar_empty + kStages * 8;
-    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + kOffMisc);
+    const uint32_t bar_full = smem_base + L::kBar, bar_empty = bar_full + kStages * 8, bar_acc = bar_empty + kStages * 8;
+    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + L::kMisc);
     volatile uint32_t *abort_flag = misc + 1;
     const WaitCtx ctx{abort_flag, status};
-    int32_t *piece_row = reinterpret_cast<int32_t *>(smem + kOffPiece);
-    int32_t *ids = reinterpret_cast<int32_t *>(smem + kOffIds), *slots = reinterpret_cast<int32_t *>(smem + kOffSlots);
+    int32_t *piece_row = reinterpret_cast<int32_t *>(smem + L::kPiece);
+    int32_t *ids = reinterpret_cast<int32_t *>(smem + L::kIds), *slots = reinterpret_cast<int32_t *>(smem + L::kSlots);
 
     const uint32_t row0 = blockIdx.x / S * kBM;                        // the tile's first row
     const uint32_t group = row0 / p.group_rows, group0 = group * p.group_rows;
@@ -93,12 +100,21 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         prefetch_tensormap(&tm_a);
     }
     if (warp == 1) {
-        tmem_alloc<1>(smem_base + kOffMisc, kChunk);
+        tmem_alloc<1>(smem_base + L::kMisc, kChunk);
         tmem_relinquish<1>();
     }
     // Everything before this launch has completed: the next launch, the GEMM, may read what they wrote at once.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // The rows of a do not depend on the list: the first of them are on their way while it is made.
+    const uint32_t early = blockIdx.y == 0 ? min(kStages, kb1 - kb0) : 0u;
+    if (threadIdx.x == 0) {
+        for (uint32_t i = 0; i < early; ++i) {
+            mbar_expect_tx(bar_full + i * 8, kXBytes);
+            tma_load_2d_hint(smem_base + L::kX + i * kXBytes, &tm_x, bar_full + i * 8, static_cast<int32_t>((kb0 + i) * kBK),
+                             static_cast<int32_t>(row0), l2_policy_evict_last());
+        }
+    }
     for (uint32_t i = threadIdx.x; i < p.group_rows; i += kThreads) {
         const int32_t id = group0 + i < p.m ? p.ids[group0 + i] : -1;
         ids[i] = id >= 0 && static_cast<uint32_t>(id) < p.adapters ? id : -1;
@@ -134,6 +150,11 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     cluster_arrive();          // every CTA of the cluster is running before anyone writes into its shared memory
     cluster_wait();
 
+    if (chunks == 0 && threadIdx.x == 0) {             // no row of the group has an adapter: let the early loads land
+        for (uint32_t i = 0; i < early; ++i) mbar_arrive(bar_full + i * 8);
+        for (uint32_t i = 0; i < early; ++i)
+            if (!wait_bar(bar_full + i * 8, 0, ctx, kStProducerEmpty)) break;
+    }
     uint32_t stage = 0, phase = 0, acc_phase = 0;
     for (uint32_t c = blockIdx.y; c < chunks; c += gridDim.y, acc_phase ^= 1u) {
         const uint32_t live = min(kChunk, a_rows - c * kChunk);       // columns of this chunk that exist
@@ -148,11 +169,13 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 for (uint32_t kb = kb0; kb < kb1; ++kb) {
                     if (!wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty)) break;
                     const uint32_t full = bar_full + stage * 8;
-                    mbar_arrive_expect_tx(full, kXBytes + live * kBK * 2);
+                    const bool there = c == 0 && kb - kb0 < early;
+                    mbar_arrive_expect_tx(full, (there ? 0u : kXBytes) + live * kBK * 2);
                     const int32_t kx = static_cast<int32_t>(kb * kBK);
-                    tma_load_2d_hint(smem_base + kOffX + stage * kXBytes, &tm_x, full, kx, static_cast<int32_t>(row0), keep);
+                    if (!there)
+                        tma_load_2d_hint(smem_base + L::kX + stage * kXBytes, &tm_x, full, kx, static_cast<int32_t>(row0), keep);
                     for (uint32_t i = 0; i < pieces; ++i)
-                        tma_load_2d_hint(smem_base + kOffW + stage * kWBytes + i * p.piece * kBK * 2, &tm_a, full, kx,
+                        tma_load_2d_hint(smem_base + L::kW + stage * kWBytes + i * p.piece * kBK * 2, &tm_a, full, kx,
                                          piece_row[i], stream);
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
@@ -167,8 +190,8 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                     ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                     if (!ok) break;
                     tc_fence_after_sync();
-                    const uint64_t dx = smem_desc_k_sw128(smem_base + kOffX + stage * kXBytes);
-                    const uint64_t dw = smem_desc_k_sw128(smem_base + kOffW + stage * kWBytes);
+                    const uint64_t dx = smem_desc_k_sw128(smem_base + L::kX + stage * kXBytes);
+                    const uint64_t dw = smem_desc_k_sw128(smem_base + L::kW + stage * kWBytes);
 #pragma unroll
                     for (uint32_t k = 0; k < kBK / kUmmaK; ++k)
                         umma_f16<1>(tmem, dx + 2 * k, dw + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
@@ -199,7 +222,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 for (int i = 0; i < 32; ++i) f[h * 32 + i] = ok ? __uint_as_float(v[i]) : 0.f;
             }
             tc_fence_before_sync();
-            const uint32_t recv = smem_base + kOffRecv;
+            const uint32_t recv = smem_base + L::kRecv;
 #pragma unroll
             for (uint32_t j = 0; j < kChunk / 4; ++j) {
                 const uint32_t owner = 4 * j / cols;
@@ -214,7 +237,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
             const uint32_t row = (warp & 3u) * 32u + lane, in_group = row0 + row - group0;
             if (in_group < p.group_rows && row0 + row < p.m) {
                 const int32_t id = ids[in_group];
-                const float4 *recv = reinterpret_cast<const float4 *>(smem + kOffRecv);
+                const float4 *recv = reinterpret_cast<const float4 *>(smem + L::kRecv);
                 for (uint32_t g = 0; g < cols / 8; ++g) {
                     const uint32_t local = rank * cols + 8 * g, at = c * kChunk + local;
                     if (local >= live) break;
@@ -420,12 +443,19 @@ int hgemm_lora_launch(const GemmArgs &g, const LoraArgs &l, cudaStream_t stream,
         const int64_t most = 2 * sms / (tiles * split);
         if (chunks > most) chunks = most < 1 ? 1 : most;
 
-        auto kernel = g.bf16 ? lora_shrink_kernel<true> : lora_shrink_kernel<false>;
-        static DeviceOnce once[2];
-        if ((e = allow_dynamic_smem(once[g.bf16 ? 1 : 0], kernel, kSmem)) != cudaSuccess) return failed(e);
+        // CTAs that will have work, with four adapters in a group of prompts, one for every other token otherwise
+        int64_t usual = p.group_rows > 128 ? 4 : g.m / 2;
+        if (usual > p.max_slots) usual = p.max_slots;
+        const bool deep = tiles * split * ((usual * l.rank + kChunk - 1) / kChunk) <= sms;
+        auto kernel = deep ? (g.bf16 ? lora_shrink_kernel<7, true> : lora_shrink_kernel<7, false>)
+                           : (g.bf16 ? lora_shrink_kernel<3, true> : lora_shrink_kernel<3, false>);
+        const uint32_t smem_bytes = deep ? ShrinkSmem<7>::kBytes : ShrinkSmem<3>::kBytes;
+        static DeviceOnce once[4];
+        if ((e = allow_dynamic_smem(once[(deep ? 2 : 0) + (g.bf16 ? 1 : 0)], kernel, static_cast<int>(smem_bytes))) != cudaSuccess)
+            return failed(e);
         cfg.gridDim = dim3(static_cast<unsigned>(tiles * split), static_cast<unsigned>(chunks), 1);
         cfg.blockDim = dim3(kThreads, 1, 1);
-        cfg.dynamicSmemBytes = kSmem;
+        cfg.dynamicSmemBytes = smem_bytes;
         attr[1].id = cudaLaunchAttributeClusterDimension;
         attr[1].val.clusterDim.x = static_cast<unsigned>(split);
         attr[1].val.clusterDim.y = 1;

@@ -88,6 +88,11 @@ __device__ __forceinline__ void mbar_arrive_expect_tx(uint32_t bar, uint32_t byt
                  : "memory");
 }
 
+// Adds to the bytes the barrier's current phase waits for, without an arrival.
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
 // Arrive on a barrier that lives in another CTA of the cluster (address from mapa()).
 // Default semantics (release at CTA scope): a cluster-scope release here costs a
 // full memory fence per call (measured: ~0.75 us on the issuing thread), and the
