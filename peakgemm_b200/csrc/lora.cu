@@ -378,17 +378,12 @@ bool dot_pays(int64_t m, int64_t k, int64_t rank) {
     return m * k * rank * 2 <= static_cast<int64_t>(env) << 20;
 }
 
-// CTAs of a cluster over k.  Beside the persistent GEMM kernels (which need whole SMs) as few as will do: the down
-// projection has the time of a tile's own k-blocks, about 0.38 us each, and every SM it occupies starts its tiles late;
-// a CTA takes about 5 us and 0.27 us a k-block.  Beside the others, whose CTAs are done soon, as many as fit.
-int64_t choose_split(int64_t tiles, int64_t k_blocks, int64_t group_rows, int sms) {
-    static const int env = tune_env_int("PEAKGEMM_TUNE_LORA_SPLIT", 0);
-    if (env > 0) return env;
+// CTAs of a cluster over k: as many as keep the tiles within one wave and leave every CTA four k-blocks.  Fewer, beside
+// which the persistent GEMM kernels could begin, cost more: each occupies half an SM pair, and the tiles of the pairs
+// that come free late end late (1003 x 4104 x 5128, us with 1 / 2 / 4 / 8: 83 / 73 / 58 / 57).
+int64_t choose_split(int64_t tiles, int64_t k_blocks, int sms) {
     int64_t split = 1;
-    while (split < 8 && tiles * split * 2 <= sms && k_blocks >= 8 * split) {
-        if (group_rows >= 256 && 5.0 + 0.27 * static_cast<double>(k_blocks) / split <= 0.38 * static_cast<double>(k_blocks)) break;
-        split *= 2;
-    }
+    while (split < 8 && tiles * split * 2 <= sms && k_blocks >= 8 * split) split *= 2;
     return split;
 }
 
@@ -436,7 +431,7 @@ int hgemm_lora_launch(const GemmArgs &g, const LoraArgs &l, cudaStream_t stream,
             !gemm_operand_map(&tm_a, l.a, l.adapters * l.rank, g.k, g.k, s.piece, g.bf16))
             return failed(cudaErrorInvalidValue);
         const int64_t tiles = (g.m + kBM - 1) / kBM;
-        const int64_t split = choose_split(tiles, (g.k + kBK - 1) / kBK, p.group_rows, sms);
+        const int64_t split = choose_split(tiles, (g.k + kBK - 1) / kBK, sms);
         // Clusters for as many chunks as there can be, up to two waves of CTAs; those without a chunk leave at once.
         int64_t chunks = (p.max_slots < g.m ? p.max_slots : g.m) * l.rank;
         chunks = (chunks + kChunk - 1) / kChunk;

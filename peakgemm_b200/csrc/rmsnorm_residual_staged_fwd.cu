@@ -60,18 +60,8 @@ rms_residual_fwd_staged_kernel(const RmsResidualFwdArgs a, const FwdPlan p, uint
         *abort_flag = 0;
         fence_mbar_init();
     }
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    {
-        const float *src[3] = {has_post ? a.t.gamma_post : nullptr, has_y ? a.t.gamma_pre : nullptr,
-                               SCALE_COL ? a.t.res_scale : nullptr};
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-            if (src[k])
-                for (int i = threadIdx.x; i < 2 * h8; i += blockDim.x)
-                    reinterpret_cast<float4 *>(smem)[(2 * k + (i & 1)) * h8 + (i >> 1)] =
-                        __ldg(reinterpret_cast<const float4 *>(src[k]) + i);
-    }
     __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const uint32_t ring0 = p.off_slot + g * p.per_group * p.slot_bytes;
     const uint32_t first = blockIdx.x * p.G + g;
     const auto issue = [&](uint32_t row, int at) {
@@ -84,9 +74,20 @@ rms_residual_fwd_staged_kernel(const RmsResidualFwdArgs a, const FwdPlan p, uint
             bulk_load(dst + 2 * row_bytes, static_cast<const uint4 *>(a.t.gate) + static_cast<int64_t>(row / rows_per_gate) * h8,
                       row_bytes, bar, rows_per_gate == 1 ? pol : l2_policy_evict_last());
     };
-    // rows first, first + workers, ...; a thread that could overflow 32 bits leaves
+    // rows first, first + workers, ...; the first of them are on their way while the gains are copied
     if (t == 0)
         for (int i = 0; i < p.per_group && first + static_cast<uint64_t>(i) * workers < rows; ++i) issue(first + i * workers, i);
+    {
+        const float *src[3] = {has_post ? a.t.gamma_post : nullptr, has_y ? a.t.gamma_pre : nullptr,
+                               SCALE_COL ? a.t.res_scale : nullptr};
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (src[k])
+                for (int i = threadIdx.x; i < 2 * h8; i += blockDim.x)
+                    reinterpret_cast<float4 *>(smem)[(2 * k + (i & 1)) * h8 + (i >> 1)] =
+                        __ldg(reinterpret_cast<const float4 *>(src[k]) + i);
+    }
+    __syncthreads();
 
     float4 *red = reinterpret_cast<float4 *>(smem + p.off_red);
     float2 *sums = reinterpret_cast<float2 *>(red) + g * 2 * group_warps;          // [parity][warps]
