@@ -11,7 +11,7 @@
 //
 // Down projection, per 128 rows of a (one tile): the adapters that occur in the tile's group of rows are listed in the
 // order of their first row; their A_i, `rank` rows of k elements each, stand below one another as the second operand,
-// cut into chunks of 64 rows.  One cluster per tile and chunk computes 128 x 64 with tcgen05 (every row of a against
+// cut into chunks of 64 or 128 rows.  One cluster per tile and chunk computes 128 x 64 (128) with tcgen05 (every row of a against
 // every listed adapter: the tensor pipe has time to spare, a and A_i are what costs), each CTA of the cluster a slice
 // of k; the partial sums meet through distributed shared memory in rank order.  Each CTA then writes its columns of V:
 // the scaled value, rounded once to the 16-bit type (the next product's operand type), for the rows that use the
@@ -33,24 +33,24 @@ using namespace ptx;
 
 namespace {
 
-constexpr uint32_t kChunk = 64;              // columns (adapter rows) of a tile
 constexpr uint32_t kXBytes = kBM * kBK * 2;
-constexpr uint32_t kWBytes = kChunk * kBK * 2;
 constexpr uint32_t kMaxGroup = 512;
 
-// STAGES 3: two CTAs fit on an SM; 7: one, with twice the bytes in flight of its own.
-template <int STAGES>
+// CHUNK columns (adapter rows) of a tile: 64 with 7 stages; 128 with 4, which reads the rows of a half as often.
+template <int CHUNK>
 struct ShrinkSmem {
+    static constexpr int STAGES = CHUNK == 64 ? 7 : 4;
+    static constexpr uint32_t kWBytes = CHUNK * kBK * 2;
     static constexpr uint32_t kX = 0;
     static constexpr uint32_t kW = kX + STAGES * kXBytes;
-    static constexpr uint32_t kRecv = kW + STAGES * kWBytes;        // [S slots][64/S/4][128 rows][4] fp32
-    static constexpr uint32_t kBar = kRecv + kBM * kChunk * 4;      // full[], empty[], acc_full
+    static constexpr uint32_t kRecv = kW + STAGES * kWBytes;        // [S slots][CHUNK/S/4][128 rows][4] fp32
+    static constexpr uint32_t kBar = kRecv + kBM * CHUNK * 4;      // full[], empty[], acc_full
     static constexpr uint32_t kMisc = kBar + (2 * STAGES + 1) * 8;  // tensor-memory slot, abort flag, slot count
     static constexpr uint32_t kPiece = kMisc + 16;                  // first row of A of each piece of the chunk
-    static constexpr uint32_t kIds = kPiece + 8 * 4;                // the group's adapter ids, -1: none
+    static constexpr uint32_t kIds = kPiece + 16 * 4;               // the group's adapter ids, -1: none
     static constexpr uint32_t kSlots = kIds + kMaxGroup * 4;        // the adapters that occur
     static constexpr uint32_t kBytes = kSlots + kMaxGroup * 4 + 1024;
-    static_assert(kBytes <= (STAGES == 3 ? 115712u : 232448u), "shared memory");
+    static_assert(kBytes <= 232448u, "shared memory");
 };
 
 struct Shrink {
@@ -59,15 +59,15 @@ struct Shrink {
     int32_t *table;
     uint4 *v;
     uint32_t m, k, adapters, rank, max_slots, group_rows, table_stride;
-    uint32_t piece;                // rows of A per load: 8 .. 64, divides rank and 64
+    uint32_t piece;                // rows of A per load: 8 .. 64, divides rank
 };
 
-template <int STAGES, bool BF16>
+template <int CHUNK, bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
 lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a, const Shrink p,
                    int *status) {
-    using L = ShrinkSmem<STAGES>;
-    constexpr uint32_t kStages = STAGES;
+    using L = ShrinkSmem<CHUNK>;
+    constexpr uint32_t kStages = L::STAGES, kChunk = CHUNK, kWBytes = L::kWBytes;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -210,25 +210,26 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after_sync();
             }
-            float f[kChunk];
-#pragma unroll
-            for (uint32_t h = 0; h < 2; ++h) {
+            const uint32_t recv = smem_base + L::kRecv;
+#pragma unroll 1
+            for (uint32_t h = 0; h < kChunk / 32; ++h) {
                 uint32_t v[32];
                 if (ok) {
                     tmem_ld_32x32b_x32(tmem + ((q * 32u) << 16) + h * 32u, v);
                     tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = 0u;
                 }
 #pragma unroll
-                for (int i = 0; i < 32; ++i) f[h * 32 + i] = ok ? __uint_as_float(v[i]) : 0.f;
+                for (uint32_t j = 0; j < 8; ++j) {
+                    const uint32_t col = h * 32u + 4u * j, owner = col / cols;
+                    const uint32_t dst = recv + ((rank * (cols / 4) + (col - owner * cols) / 4) * kBM + row) * 16u;
+                    st_cluster_v4(mapa(dst, owner), __uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
+                                  __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
+                }
             }
             tc_fence_before_sync();
-            const uint32_t recv = smem_base + L::kRecv;
-#pragma unroll
-            for (uint32_t j = 0; j < kChunk / 4; ++j) {
-                const uint32_t owner = 4 * j / cols;
-                const uint32_t dst = recv + ((rank * (cols / 4) + (4 * j - owner * cols) / 4) * kBM + row) * 16u;
-                st_cluster_v4(mapa(dst, owner), f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-            }
         }
         __syncwarp();
         cluster_arrive();          // all parts delivered
@@ -280,12 +281,12 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
 constexpr uint32_t kDotRanks = 4;        // rank elements of a block: its loads of a token's row serve all of them
 constexpr uint32_t kDotWarps = 8;
 
-// v of one token and kDotRanks rank elements; one group of at most 64 rows.  Bound by latency: every load of a thread is
-// in flight at once for k up to 2048, the row's adapter is read in parallel with the group's list.
+// v of one token and kDotRanks rank elements.  Bound by latency: every load of a thread is in flight at once for k up to
+// 2048, and the row's adapter is read in parallel with the listing of its group's.
 template <bool BF16>
 __global__ void __launch_bounds__(kDotWarps * 32)
 lora_dot_kernel(const uint4 *x, int64_t ldx8, const uint4 *a, const Shrink p) {
-    __shared__ int32_t slots[64];
+    __shared__ int32_t slots[kMaxGroup];
     __shared__ uint32_t s_count;
     __shared__ float red[kDotWarps][kDotRanks];
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -294,10 +295,11 @@ lora_dot_kernel(const uint4 *x, int64_t ldx8, const uint4 *a, const Shrink p) {
     const uint32_t t = blockIdx.y, r0 = blockIdx.x * kDotRanks;
     const auto checked = [&](int32_t id) { return id >= 0 && static_cast<uint32_t>(id) < p.adapters ? id : -1; };
     const int32_t id = checked(p.ids[t]);
+    const uint32_t group = t / p.group_rows, group0 = group * p.group_rows, group_end = min(p.m, group0 + p.group_rows);
     if (warp == 0) {                     // the distinct ids in the order of their first row
         uint32_t n = 0;
-        for (uint32_t r = 0; r < p.m; r += 32) {
-            const int32_t mine = r + lane < p.m ? checked(p.ids[r + lane]) : -1;
+        for (uint32_t r = group0; r < group_end; r += 32) {
+            const int32_t mine = r + lane < group_end ? checked(p.ids[r + lane]) : -1;
             const uint32_t same = __match_any_sync(0xffffffffu, mine);       // every lane takes part
             bool fresh = mine >= 0 && __ffs(same) - 1 == static_cast<int>(lane);
             for (uint32_t e = 0; e < n; ++e) fresh = fresh && slots[e] != mine;
@@ -335,14 +337,15 @@ lora_dot_kernel(const uint4 *x, int64_t ldx8, const uint4 *a, const Shrink p) {
         for (uint32_t r = 0; r < kDotRanks; ++r) red[warp][r] = sum[r];
     __syncthreads();
     const uint32_t n = s_count;
-    if (blockIdx.x == 0 && t == 0) {
-        if (threadIdx.x == 0) p.table[0] = static_cast<int32_t>(n);
-        for (uint32_t i = threadIdx.x; i < n; i += kDotWarps * 32) p.table[1 + i] = slots[i];
+    if (blockIdx.x == 0 && t == group0) {
+        int32_t *table = p.table + static_cast<size_t>(group) * p.table_stride;
+        if (threadIdx.x == 0) table[0] = static_cast<int32_t>(n);
+        for (uint32_t i = threadIdx.x; i < n; i += kDotWarps * 32) table[1 + i] = slots[i];
     }
     // the row of every slot: the scaled value, rounded once, in the slot of the row's adapter, zeros in the others
-    if (threadIdx.x < n) {
+    for (uint32_t slot = threadIdx.x; slot < n; slot += kDotWarps * 32) {
         uint2 out = make_uint2(0, 0);
-        if (slots[threadIdx.x] == id) {
+        if (slots[slot] == id) {
             const float scale = p.scale ? p.scale[id] : 1.f;
             float v[kDotRanks] = {};
 #pragma unroll
@@ -351,7 +354,8 @@ lora_dot_kernel(const uint4 *x, int64_t ldx8, const uint4 *a, const Shrink p) {
                 for (uint32_t r = 0; r < kDotRanks; ++r) v[r] += red[w][r];
             out = make_uint2(pack2<BF16>(v[0] * scale, v[1] * scale), pack2<BF16>(v[2] * scale, v[3] * scale));
         }
-        reinterpret_cast<uint2 *>(p.v)[((static_cast<int64_t>(threadIdx.x) * p.group_rows + t) * p.rank + r0) / 4] = out;
+        const int64_t row = (static_cast<int64_t>(group) * p.max_slots + slot) * p.group_rows + (t - group0);
+        reinterpret_cast<uint2 *>(p.v)[(row * p.rank + r0) / 4] = out;
     }
 }
 
@@ -372,7 +376,8 @@ Plan make_plan(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank, 
     return p;
 }
 
-// Dot products read an adapter's rows once for every token: up to 32 MiB of them.
+// Dot products read an adapter's rows once for every token: up to 32 MiB of them they are done sooner than a tcgen05
+// launch (9 us and more).
 bool dot_pays(int64_t m, int64_t k, int64_t rank) {
     static const int env = tune_env_int("PEAKGEMM_TUNE_LORA_DOT_MB", 32);
     return m * k * rank * 2 <= static_cast<int64_t>(env) << 20;
@@ -418,35 +423,37 @@ int hgemm_lora_launch(const GemmArgs &g, const LoraArgs &l, cudaStream_t stream,
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (p.group_rows <= 64 && dot_pays(g.m, g.k, l.rank)) {
+    if (g.m <= 65535 && dot_pays(g.m, g.k, l.rank)) {
         cfg.gridDim = dim3(static_cast<unsigned>(l.rank / kDotRanks), static_cast<unsigned>(g.m), 1);
         cfg.blockDim = dim3(kDotWarps * 32, 1, 1);
         if ((e = cudaLaunchKernelEx(&cfg, g.bf16 ? lora_dot_kernel<true> : lora_dot_kernel<false>,
                                     static_cast<const uint4 *>(g.a), g.lda / 8, static_cast<const uint4 *>(l.a), s)) != cudaSuccess)
             return failed(e);
     } else {
-        while (s.piece < kChunk && l.rank % (2 * s.piece) == 0) s.piece *= 2;
+        while (s.piece < 64 && l.rank % (2 * s.piece) == 0) s.piece *= 2;
         CUtensorMap tm_x, tm_a;
         if (!gemm_operand_map(&tm_x, g.a, g.m, g.k, g.lda, kBM, g.bf16) ||
             !gemm_operand_map(&tm_a, l.a, l.adapters * l.rank, g.k, g.k, s.piece, g.bf16))
             return failed(cudaErrorInvalidValue);
         const int64_t tiles = (g.m + kBM - 1) / kBM;
         const int64_t split = choose_split(tiles, (g.k + kBK - 1) / kBK, sms);
+        // Chunks of 64 where their CTAs (for four adapters in a group of prompts, one for every other token otherwise) fit
+        // on the SMs at once; else of 128 (128 x 4096 x 14336, 20 adapters of rank 64: 160 CTAs, 51 us).
+        int64_t usual = p.group_rows > 128 ? 4 : g.m / 2;
+        if (usual > p.max_slots) usual = p.max_slots;
+        const bool narrow = tiles * split * ((usual * l.rank + 63) / 64) <= sms;
+        const int64_t chunk = narrow ? 64 : 128;
         // Clusters for as many chunks as there can be, up to two waves of CTAs; those without a chunk leave at once.
         int64_t chunks = (p.max_slots < g.m ? p.max_slots : g.m) * l.rank;
-        chunks = (chunks + kChunk - 1) / kChunk;
+        chunks = (chunks + chunk - 1) / chunk;
         const int64_t most = 2 * sms / (tiles * split);
         if (chunks > most) chunks = most < 1 ? 1 : most;
 
-        // CTAs that will have work, with four adapters in a group of prompts, one for every other token otherwise
-        int64_t usual = p.group_rows > 128 ? 4 : g.m / 2;
-        if (usual > p.max_slots) usual = p.max_slots;
-        const bool deep = tiles * split * ((usual * l.rank + kChunk - 1) / kChunk) <= sms;
-        auto kernel = deep ? (g.bf16 ? lora_shrink_kernel<7, true> : lora_shrink_kernel<7, false>)
-                           : (g.bf16 ? lora_shrink_kernel<3, true> : lora_shrink_kernel<3, false>);
-        const uint32_t smem_bytes = deep ? ShrinkSmem<7>::kBytes : ShrinkSmem<3>::kBytes;
+        auto kernel = narrow ? (g.bf16 ? lora_shrink_kernel<64, true> : lora_shrink_kernel<64, false>)
+                             : (g.bf16 ? lora_shrink_kernel<128, true> : lora_shrink_kernel<128, false>);
+        const uint32_t smem_bytes = narrow ? ShrinkSmem<64>::kBytes : ShrinkSmem<128>::kBytes;
         static DeviceOnce once[4];
-        if ((e = allow_dynamic_smem(once[(deep ? 2 : 0) + (g.bf16 ? 1 : 0)], kernel, static_cast<int>(smem_bytes))) != cudaSuccess)
+        if ((e = allow_dynamic_smem(once[(narrow ? 2 : 0) + (g.bf16 ? 1 : 0)], kernel, static_cast<int>(smem_bytes))) != cudaSuccess)
             return failed(e);
         cfg.gridDim = dim3(static_cast<unsigned>(tiles * split), static_cast<unsigned>(chunks), 1);
         cfg.blockDim = dim3(kThreads, 1, 1);
