@@ -11,9 +11,9 @@
 //
 // Down projection, per 128 rows of a (one tile): the adapters that occur in the tile's group of rows are listed in the
 // order of their first row; their A_i, `rank` rows of k elements each, stand below one another as the second operand,
-// cut into chunks of 64 or 128 rows.  One cluster per tile and chunk computes 128 x 64 (128) with tcgen05 (every row of a against
+// cut into chunks of 64 to 128 rows, as many as the grid has clusters.  A cluster computes 128 rows x a chunk with tcgen05 (every row of a against
 // every listed adapter: the tensor pipe has time to spare, a and A_i are what costs), each CTA of the cluster a slice
-// of k; the partial sums meet through distributed shared memory in rank order.  Each CTA then writes its columns of V:
+// of k; the partial sums meet through distributed shared memory in rank order.  Each CTA then writes its rows of V:
 // the scaled value, rounded once to the 16-bit type (the next product's operand type), for the rows that use the
 // adapter, zeros for the others (selected, not multiplied: a row's NaN stays its own).
 
@@ -36,22 +36,19 @@ namespace {
 constexpr uint32_t kXBytes = kBM * kBK * 2;
 constexpr uint32_t kMaxGroup = 512;
 
-// CHUNK columns (adapter rows) of a tile: 64 with 7 stages; 128 with 4, which reads the rows of a half as often.
-template <int CHUNK>
-struct ShrinkSmem {
-    static constexpr int STAGES = CHUNK == 64 ? 7 : 4;
-    static constexpr uint32_t kWBytes = CHUNK * kBK * 2;
-    static constexpr uint32_t kX = 0;
-    static constexpr uint32_t kW = kX + STAGES * kXBytes;
-    static constexpr uint32_t kRecv = kW + STAGES * kWBytes;        // [S slots][CHUNK/S/4][128 rows][4] fp32
-    static constexpr uint32_t kBar = kRecv + kBM * CHUNK * 4;      // full[], empty[], acc_full
-    static constexpr uint32_t kMisc = kBar + (2 * STAGES + 1) * 8;  // tensor-memory slot, abort flag, slot count
-    static constexpr uint32_t kPiece = kMisc + 16;                  // first row of A of each piece of the chunk
-    static constexpr uint32_t kIds = kPiece + 16 * 4;               // the group's adapter ids, -1: none
-    static constexpr uint32_t kSlots = kIds + kMaxGroup * 4;        // the adapters that occur
-    static constexpr uint32_t kBytes = kSlots + kMaxGroup * 4 + 1024;
-    static_assert(kBytes <= 232448u, "shared memory");
-};
+constexpr uint32_t kStages = 4;
+constexpr uint32_t kMinChunk = 64, kMaxChunk = 128;             // columns (adapter rows) of a cluster's tile
+constexpr uint32_t kWBytes = kMaxChunk * kBK * 2;
+constexpr uint32_t kOffX = 0;
+constexpr uint32_t kOffW = kOffX + kStages * kXBytes;
+constexpr uint32_t kOffRecv = kOffW + kStages * kWBytes;        // [S senders][columns / 4][128 / S rows][4] fp32
+constexpr uint32_t kOffBar = kOffRecv + kBM * kMaxChunk * 4;    // full[], empty[], acc_full
+constexpr uint32_t kOffMisc = kOffBar + (2 * kStages + 1) * 8;  // tensor-memory slot, abort flag, slot count
+constexpr uint32_t kOffPiece = kOffMisc + 16;                   // first row of A of each piece of the chunk
+constexpr uint32_t kOffIds = kOffPiece + 16 * 4;                // the group's adapter ids, -1: none
+constexpr uint32_t kOffSlots = kOffIds + kMaxGroup * 4;         // the adapters that occur
+constexpr uint32_t kSmem = kOffSlots + kMaxGroup * 4 + 1024;
+static_assert(kSmem <= 232448, "exceeds 227 KiB of shared memory");
 
 struct Shrink {
     const int32_t *ids;
@@ -62,25 +59,23 @@ struct Shrink {
     uint32_t piece;                // rows of A per load: 8 .. 64, divides rank
 };
 
-template <int CHUNK, bool BF16>
+template <bool BF16>
 __global__ void __launch_bounds__(kThreads, 1)
 lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a, const Shrink p,
                    int *status) {
-    using L = ShrinkSmem<CHUNK>;
-    constexpr uint32_t kStages = L::STAGES, kChunk = CHUNK, kWBytes = L::kWBytes;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
     uint8_t *smem = smem_raw + (smem_base - smem_u32(smem_raw));
     const uint32_t warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
     const uint32_t lane = threadIdx.x & 31u;
     const uint32_t S = cluster_nctarank(), rank = cluster_ctarank();
-    const uint32_t cols = kChunk / S;                                  // columns this CTA finally owns
-    const uint32_t bar_full = smem_base + L::kBar, bar_empty = bar_full + kStages * 8, bar_acc = bar_empty + kStages * 8;
-    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + L::kMisc);
+    const uint32_t own_rows = kBM / S;                                 // rows of the tile this CTA finally owns
+    const uint32_t bar_full = smem_base + kOffBar, bar_empty = bar_full + kStages * 8, bar_acc = bar_empty + kStages * 8;
+    volatile uint32_t *misc = reinterpret_cast<volatile uint32_t *>(smem + kOffMisc);
     volatile uint32_t *abort_flag = misc + 1;
     const WaitCtx ctx{abort_flag, status};
-    int32_t *piece_row = reinterpret_cast<int32_t *>(smem + L::kPiece);
-    int32_t *ids = reinterpret_cast<int32_t *>(smem + L::kIds), *slots = reinterpret_cast<int32_t *>(smem + L::kSlots);
+    int32_t *piece_row = reinterpret_cast<int32_t *>(smem + kOffPiece);
+    int32_t *ids = reinterpret_cast<int32_t *>(smem + kOffIds), *slots = reinterpret_cast<int32_t *>(smem + kOffSlots);
 
     const uint32_t row0 = blockIdx.x / S * kBM;                        // the tile's first row
     const uint32_t group = row0 / p.group_rows, group0 = group * p.group_rows;
@@ -100,7 +95,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         prefetch_tensormap(&tm_a);
     }
     if (warp == 1) {
-        tmem_alloc<1>(smem_base + L::kMisc, kChunk);
+        tmem_alloc<1>(smem_base + kOffMisc, kMaxChunk);
         tmem_relinquish<1>();
     }
     // Everything before this launch has completed: the next launch, the GEMM, may read what they wrote at once.
@@ -111,7 +106,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     if (threadIdx.x == 0) {
         for (uint32_t i = 0; i < early; ++i) {
             mbar_expect_tx(bar_full + i * 8, kXBytes);
-            tma_load_2d_hint(smem_base + L::kX + i * kXBytes, &tm_x, bar_full + i * 8, static_cast<int32_t>((kb0 + i) * kBK),
+            tma_load_2d_hint(smem_base + kOffX + i * kXBytes, &tm_x, bar_full + i * 8, static_cast<int32_t>((kb0 + i) * kBK),
                              static_cast<int32_t>(row0), l2_policy_evict_last());
         }
     }
@@ -140,7 +135,12 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         if (lane == 0) misc[2] = n;
     }
     __syncthreads();
-    const uint32_t n_slots = misc[2], a_rows = n_slots * p.rank, chunks = (a_rows + kChunk - 1) / kChunk;
+    const uint32_t n_slots = misc[2], a_rows = n_slots * p.rank;
+    // The narrowest chunk (a multiple of 16, and of the pieces A comes in) with which the grid's clusters take one each:
+    // 128 x 4096 x 14336 with 20 adapters of rank 64, 16 chunks of 80 on 128 CTAs instead of 20 of 64 on 160.
+    const uint32_t step = max(16u, p.piece);
+    const uint32_t chunk = min(kMaxChunk, max(kMinChunk, ((a_rows + gridDim.y - 1) / gridDim.y + step - 1) / step * step));
+    const uint32_t chunks = (a_rows + chunk - 1) / chunk;
     if (rank == 0 && blockIdx.y == 0 && row0 == group0) {
         int32_t *t = p.table + static_cast<size_t>(group) * p.table_stride;
         if (threadIdx.x == 0) t[0] = static_cast<int32_t>(n_slots);
@@ -157,12 +157,12 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     }
     uint32_t stage = 0, phase = 0, acc_phase = 0;
     for (uint32_t c = blockIdx.y; c < chunks; c += gridDim.y, acc_phase ^= 1u) {
-        const uint32_t live = min(kChunk, a_rows - c * kChunk);       // columns of this chunk that exist
+        const uint32_t live = min(chunk, a_rows - c * chunk);       // columns of this chunk that exist
         if (warp == 0) {
             if (lane == 0) {
                 const uint32_t pieces = live / p.piece;
                 for (uint32_t i = 0; i < pieces; ++i) {
-                    const uint32_t at = c * kChunk + i * p.piece, slot = at / p.rank;
+                    const uint32_t at = c * chunk + i * p.piece, slot = at / p.rank;
                     piece_row[i] = slots[slot] * static_cast<int32_t>(p.rank) + static_cast<int32_t>(at - slot * p.rank);
                 }
                 const uint64_t keep = l2_policy_evict_last(), stream = l2_policy_evict_first();
@@ -173,9 +173,9 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                     mbar_arrive_expect_tx(full, (there ? 0u : kXBytes) + live * kBK * 2);
                     const int32_t kx = static_cast<int32_t>(kb * kBK);
                     if (!there)
-                        tma_load_2d_hint(smem_base + L::kX + stage * kXBytes, &tm_x, full, kx, static_cast<int32_t>(row0), keep);
+                        tma_load_2d_hint(smem_base + kOffX + stage * kXBytes, &tm_x, full, kx, static_cast<int32_t>(row0), keep);
                     for (uint32_t i = 0; i < pieces; ++i)
-                        tma_load_2d_hint(smem_base + L::kW + stage * kWBytes + i * p.piece * kBK * 2, &tm_a, full, kx,
+                        tma_load_2d_hint(smem_base + kOffW + stage * kWBytes + i * p.piece * kBK * 2, &tm_a, full, kx,
                                          piece_row[i], stream);
                     if (++stage == kStages) { stage = 0; phase ^= 1u; }
                 }
@@ -184,14 +184,14 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         } else if (warp == 1) {
             if (lane == 0 && has_k) {
                 // columns that do not exist hold what was in shared memory; they are not stored
-                constexpr uint32_t idesc = instr_desc_f16(BF16, kBM, kChunk);
+                const uint32_t idesc = instr_desc_f16(BF16, kBM, chunk);
                 bool ok = true;
                 for (uint32_t kb = kb0; kb < kb1; ++kb) {
                     ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                     if (!ok) break;
                     tc_fence_after_sync();
-                    const uint64_t dx = smem_desc_k_sw128(smem_base + L::kX + stage * kXBytes);
-                    const uint64_t dw = smem_desc_k_sw128(smem_base + L::kW + stage * kWBytes);
+                    const uint64_t dx = smem_desc_k_sw128(smem_base + kOffX + stage * kXBytes);
+                    const uint64_t dw = smem_desc_k_sw128(smem_base + kOffW + stage * kWBytes);
 #pragma unroll
                     for (uint32_t k = 0; k < kBK / kUmmaK; ++k)
                         umma_f16<1>(tmem, dx + 2 * k, dw + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
@@ -202,7 +202,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
             }
             __syncwarp();
         } else {
-            // my partial sums of the columns each peer owns go to that peer
+            // my partial sums of a row go to the CTA that owns it
             const uint32_t q = warp & 3u, row = q * 32u + lane;
             bool ok = has_k;
             if (has_k) {
@@ -210,9 +210,10 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after_sync();
             }
-            const uint32_t recv = smem_base + L::kRecv;
+            const uint32_t owner = row / own_rows;
+            const uint32_t recv = mapa(smem_base + kOffRecv + (rank * (chunk / 4) * own_rows + row - owner * own_rows) * 16u, owner);
 #pragma unroll 1
-            for (uint32_t h = 0; h < kChunk / 32; ++h) {
+            for (uint32_t h = 0; h < (live + 31) / 32; ++h) {
                 uint32_t v[32];
                 if (ok) {
                     tmem_ld_32x32b_x32(tmem + ((q * 32u) << 16) + h * 32u, v);
@@ -222,12 +223,10 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                     for (int i = 0; i < 32; ++i) v[i] = 0u;
                 }
 #pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    const uint32_t col = h * 32u + 4u * j, owner = col / cols;
-                    const uint32_t dst = recv + ((rank * (cols / 4) + (col - owner * cols) / 4) * kBM + row) * 16u;
-                    st_cluster_v4(mapa(dst, owner), __uint_as_float(v[4 * j]), __uint_as_float(v[4 * j + 1]),
-                                  __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
-                }
+                for (uint32_t j = 0; j < 8; ++j)
+                    if (h * 32u + 4u * j < live)
+                        st_cluster_v4(recv + (h * 8u + j) * own_rows * 16u, __uint_as_float(v[4 * j]),
+                                      __uint_as_float(v[4 * j + 1]), __uint_as_float(v[4 * j + 2]), __uint_as_float(v[4 * j + 3]));
             }
             tc_fence_before_sync();
         }
@@ -235,32 +234,30 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         cluster_arrive();          // all parts delivered
         cluster_wait();
         if (warp >= 2) {
-            const uint32_t row = (warp & 3u) * 32u + lane, in_group = row0 + row - group0;
-            if (in_group < p.group_rows && row0 + row < p.m) {
+            const float4 *recv = reinterpret_cast<const float4 *>(smem + kOffRecv);
+            for (uint32_t i = threadIdx.x - 64; i < own_rows * (live / 8); i += 128) {
+                const uint32_t g = i / own_rows, r_own = i - g * own_rows, row = row0 + rank * own_rows + r_own;
+                const uint32_t in_group = row - group0;
+                if (in_group >= p.group_rows || row >= p.m) continue;
                 const int32_t id = ids[in_group];
-                const float4 *recv = reinterpret_cast<const float4 *>(smem + L::kRecv);
-                for (uint32_t g = 0; g < cols / 8; ++g) {
-                    const uint32_t local = rank * cols + 8 * g, at = c * kChunk + local;
-                    if (local >= live) break;
-                    const uint32_t slot = at / p.rank, r = at - slot * p.rank;
-                    uint4 out = make_uint4(0, 0, 0, 0);
-                    if (slots[slot] == id) {
-                        float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                        for (uint32_t s = 0; s < S; ++s) {
-                            const float4 *src = recv + (s * (cols / 4) + 2 * g) * kBM + row;
-                            const float4 a = src[0], b = src[kBM];
-                            f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
-                            f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
-                        }
-                        const float scale = p.scale ? p.scale[id] : 1.f;
-                        out.x = pack2<BF16>(f[0] * scale, f[1] * scale);
-                        out.y = pack2<BF16>(f[2] * scale, f[3] * scale);
-                        out.z = pack2<BF16>(f[4] * scale, f[5] * scale);
-                        out.w = pack2<BF16>(f[6] * scale, f[7] * scale);
+                const uint32_t at = c * chunk + 8 * g, slot = at / p.rank, r = at - slot * p.rank;
+                uint4 out = make_uint4(0, 0, 0, 0);
+                if (slots[slot] == id) {
+                    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    for (uint32_t s = 0; s < S; ++s) {
+                        const float4 *src = recv + (s * (chunk / 4) + 2 * g) * own_rows + r_own;
+                        const float4 a = src[0], b = src[own_rows];
+                        f[0] += a.x; f[1] += a.y; f[2] += a.z; f[3] += a.w;
+                        f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
                     }
-                    const int64_t v_row = (static_cast<int64_t>(group) * p.max_slots + slot) * p.group_rows + in_group;
-                    p.v[(v_row * p.rank + r) / 8] = out;
+                    const float scale = p.scale ? p.scale[id] : 1.f;
+                    out.x = pack2<BF16>(f[0] * scale, f[1] * scale);
+                    out.y = pack2<BF16>(f[2] * scale, f[3] * scale);
+                    out.z = pack2<BF16>(f[4] * scale, f[5] * scale);
+                    out.w = pack2<BF16>(f[6] * scale, f[7] * scale);
                 }
+                const int64_t v_row = (static_cast<int64_t>(group) * p.max_slots + slot) * p.group_rows + in_group;
+                p.v[(v_row * p.rank + r) / 8] = out;
             }
         }
         if (c + gridDim.y < chunks) {      // the receive buffer and the accumulator are free again everywhere
@@ -274,7 +271,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     if (*abort_flag) __nanosleep(50000);
     if (warp == 1) {
         tc_fence_after_sync();
-        tmem_dealloc<1>(tmem, kChunk);
+        tmem_dealloc<1>(tmem, kMaxChunk);
     }
 }
 
@@ -437,27 +434,18 @@ int hgemm_lora_launch(const GemmArgs &g, const LoraArgs &l, cudaStream_t stream,
             return failed(cudaErrorInvalidValue);
         const int64_t tiles = (g.m + kBM - 1) / kBM;
         const int64_t split = choose_split(tiles, (g.k + kBK - 1) / kBK, sms);
-        // Chunks of 64 where their CTAs (for four adapters in a group of prompts, one for every other token otherwise) fit
-        // on the SMs at once; else of 128 (128 x 4096 x 14336, 20 adapters of rank 64: 160 CTAs, 51 us).
-        int64_t usual = p.group_rows > 128 ? 4 : g.m / 2;
-        if (usual > p.max_slots) usual = p.max_slots;
-        const bool narrow = tiles * split * ((usual * l.rank + 63) / 64) <= sms;
-        const int64_t chunk = narrow ? 64 : 128;
-        // Clusters for as many chunks as there can be, up to two waves of CTAs; those without a chunk leave at once.
+        // Clusters for as many chunks as there can be, up to one wave of CTAs; those without a chunk leave at once.
         int64_t chunks = (p.max_slots < g.m ? p.max_slots : g.m) * l.rank;
-        chunks = (chunks + chunk - 1) / chunk;
-        const int64_t most = 2 * sms / (tiles * split);
+        chunks = (chunks + kMinChunk - 1) / kMinChunk;
+        const int64_t most = sms / (tiles * split);
         if (chunks > most) chunks = most < 1 ? 1 : most;
 
-        auto kernel = narrow ? (g.bf16 ? lora_shrink_kernel<64, true> : lora_shrink_kernel<64, false>)
-                             : (g.bf16 ? lora_shrink_kernel<128, true> : lora_shrink_kernel<128, false>);
-        const uint32_t smem_bytes = narrow ? ShrinkSmem<64>::kBytes : ShrinkSmem<128>::kBytes;
-        static DeviceOnce once[4];
-        if ((e = allow_dynamic_smem(once[(narrow ? 2 : 0) + (g.bf16 ? 1 : 0)], kernel, static_cast<int>(smem_bytes))) != cudaSuccess)
-            return failed(e);
+        auto kernel = g.bf16 ? lora_shrink_kernel<true> : lora_shrink_kernel<false>;
+        static DeviceOnce once[2];
+        if ((e = allow_dynamic_smem(once[g.bf16 ? 1 : 0], kernel, kSmem)) != cudaSuccess) return failed(e);
         cfg.gridDim = dim3(static_cast<unsigned>(tiles * split), static_cast<unsigned>(chunks), 1);
         cfg.blockDim = dim3(kThreads, 1, 1);
-        cfg.dynamicSmemBytes = smem_bytes;
+        cfg.dynamicSmemBytes = kSmem;
         attr[1].id = cudaLaunchAttributeClusterDimension;
         attr[1].val.clusterDim.x = static_cast<unsigned>(split);
         attr[1].val.clusterDim.y = 1;
