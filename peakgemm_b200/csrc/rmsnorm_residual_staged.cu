@@ -103,9 +103,23 @@ rms_residual_bwd_staged_kernel(const RmsResidualBwdArgs a, const RmsResidualPart
         *abort_flag = 0;
         fence_mbar_init();
     }
-    __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const bool has_dy = FULL || a.dy, has_ds = FULL || a.ds, has_post = FULL || a.t.gamma_post;
+    {
+        const float *src[3] = {has_dy ? a.t.gamma_pre : nullptr, has_post ? a.t.gamma_post : nullptr,
+                               SCALE_COL ? a.t.res_scale : nullptr};
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (src[k])
+                for (int i = threadIdx.x; i < 2 * h8; i += blockDim.x)
+                    reinterpret_cast<float4 *>(smem)[(2 * k + (i & 1)) * p.cols8 + (i >> 1)] =
+                        __ldg(reinterpret_cast<const float4 *>(src[k]) + 2 * col0 + i);
+    }
+    __syncthreads();
+    if constexpr (CLUSTER) {                   // every CTA's barriers exist before anyone signals them
+        cluster_arrive();
+        cluster_wait();
+    }
     // the lower and upper halves of the vectors apart: a warp's 16-byte loads are consecutive
     const uint32_t half = 16 * p.cols8;
     const auto gamma_pre = [&](int idx, float2 (&f)[4]) { vec_load2(sbase + 16 * idx, half, f); };
@@ -131,24 +145,8 @@ rms_residual_bwd_staged_kernel(const RmsResidualBwdArgs a, const RmsResidualPart
                           static_cast<const uint4 *>(src[o]) + static_cast<int64_t>(row) * row8 + col0, row_bytes,
                           bar_full + slot * 8, pol);
     };
-    if (t == 0)                                // the first rows are on their way while the gains are copied
+    if (t == 0)
         for (int i = 0; i < per_group && r0 + i < r1; ++i) issue(r0 + i, i);
-    {
-        const float *src[3] = {has_dy ? a.t.gamma_pre : nullptr, has_post ? a.t.gamma_post : nullptr,
-                               SCALE_COL ? a.t.res_scale : nullptr};
-#pragma unroll
-        for (int k = 0; k < 3; ++k)
-            if (src[k])
-                for (int i = threadIdx.x; i < 2 * h8; i += blockDim.x)
-                    reinterpret_cast<float4 *>(smem)[(2 * k + (i & 1)) * p.cols8 + (i >> 1)] =
-                        __ldg(reinterpret_cast<const float4 *>(src[k]) + 2 * col0 + i);
-    }
-    __syncthreads();
-    if constexpr (CLUSTER) {                   // every CTA's barriers exist before anyone signals them
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
-    }
 
     const bool token_gate = GATE == 2 || (GATE == 3 && p.place[kGate] >= 0);
     const bool group_gate = GATE == 1 || (GATE == 3 && a.t.gate && !token_gate);
