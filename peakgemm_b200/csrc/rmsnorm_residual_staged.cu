@@ -47,21 +47,24 @@ struct StagedPlan {
 };
 
 struct Group {
-    int T, G, C, cols8;
+    int T, G, C, cols8, clusters;      // clusters: that fit the GPU at once
 };
 constexpr int kVpt = 2;                // vectors a thread owns: 128 registers a thread, 512 threads
 constexpr int kMaxThreads = 512;
 
+int clusters_at_once(int C, int sms);
+
 Group make_group(int64_t rows, int64_t h, int sms) {
     const int64_t h8 = h / 8;
-    Group g = {0, 0, 1, 0};
+    Group g = {0, 0, 1, 0, 0};
     while (g.C < 8 && h8 > 512 * g.C) g.C *= 2;
     if (h8 > 512 * g.C) return g;
     g.cols8 = static_cast<int>((h8 + g.C - 1) / g.C);
     g.T = ((g.cols8 + kVpt - 1) / kVpt + 31) / 32 * 32;
     g.G = kMaxThreads / g.T;
     if (g.G > kMaxGroups) g.G = kMaxGroups;
-    const int64_t per_cluster = (rows * g.C + sms - 1) / sms;
+    g.clusters = clusters_at_once(g.C, sms);
+    const int64_t per_cluster = (rows + g.clusters - 1) / g.clusters;
     if (g.G > per_cluster) g.G = static_cast<int>(per_cluster);
     return g;
 }
@@ -433,6 +436,40 @@ rms_residual_bwd_staged_kernel(const RmsResidualBwdArgs a, const RmsResidualPart
     }
 }
 
+// Clusters of C CTAs that the device holds at once: fewer than sms / C, since a cluster's CTAs share a GPC.  With one
+// that has to wait for another to end, a call takes almost twice as long: [8192, 16384] bf16, 8 gates, 806 us with sms / 4
+// clusters of 4, 481 with those that fit.
+int clusters_at_once(int C, int sms) {
+    if (C == 1) return sms;
+    static DeviceOnce once;
+    static int table[kMaxDevices][3] = {};
+    int dev = 0;
+    const auto fill = [&]() {
+        auto kernel = rms_residual_bwd_staged_kernel<true, true, 3, true, false>;       // they differ in nothing that counts here
+        for (int i = 0; i < 3; ++i) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(static_cast<unsigned>(sms / (2 << i) * (2 << i)), 1, 1);
+            cfg.blockDim = dim3(kMaxThreads, 1, 1);
+            cfg.dynamicSmemBytes = kSmemMost;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 2u << i;
+            attr[0].val.clusterDim.y = 1;
+            attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMost));
+            if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&table[dev][i], kernel, &cfg);
+            if (e != cudaSuccess) return e;
+        }
+        return cudaSuccess;
+    };
+    int n = 0;
+    if (current_device(&dev) == cudaSuccess && once.run(dev, fill) == cudaSuccess) n = table[dev][C == 2 ? 0 : C == 4 ? 1 : 2];
+    else cudaGetLastError();
+    return n < 1 ? 1 : n;
+}
+
 // Slots and shared memory: the gains (and a res_scale per column), the ring, row sums, barriers, abort flag.
 StagedPlan make_staged_plan(const RmsResidualBwdArgs &a, int sms) {
     const Group g = make_group(a.t.rows, a.t.h, sms);
@@ -512,7 +549,7 @@ uint32_t rmsnorm_residual_staged_workers(int64_t rows, int64_t h, int sms, uint3
     *ctas_per_row = static_cast<uint32_t>(g.C);
     if (g.T == 0) return 0;
     int64_t clusters = rows / g.G;                  // every worker has a row
-    if (clusters > sms / g.C) clusters = sms / g.C;
+    if (clusters > g.clusters) clusters = g.clusters;
     return static_cast<uint32_t>(clusters * g.G);
 }
 
