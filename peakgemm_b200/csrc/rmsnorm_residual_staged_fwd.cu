@@ -32,11 +32,12 @@ constexpr uint32_t kSmemMost = 232448;
 
 struct FwdPlan {
     int T, G, per_group;          // threads of a group, groups, slots of a group; T = 0: the width is not supported
+    bool staged_gate;             // the row's gate comes through the ring
     uint32_t slot_bytes, off_slot, off_red, off_bar, smem;
 };
 
-// FULL: gamma_post and y are there.
-template <bool BF16, bool GATE, bool SCALE_COL, bool FULL>
+// GATE: 0 none, 1 read by the threads, 2 through the ring.  FULL: gamma_post and y are there.
+template <bool BF16, int GATE, bool SCALE_COL, bool FULL>
 __global__ void __launch_bounds__(kMaxThreads, 1)
 rms_residual_fwd_staged_kernel(const RmsResidualFwdArgs a, const FwdPlan p, uint32_t workers, uint32_t rows_per_gate,
                                int *status) {
@@ -70,7 +71,7 @@ rms_residual_fwd_staged_kernel(const RmsResidualFwdArgs a, const FwdPlan p, uint
         mbar_arrive_expect_tx(bar, p.slot_bytes);
         bulk_load(dst, static_cast<const uint4 *>(a.u) + static_cast<int64_t>(row) * h8, row_bytes, bar, pol);
         bulk_load(dst + row_bytes, static_cast<const uint4 *>(a.residual) + static_cast<int64_t>(row) * h8, row_bytes, bar, pol);
-        if constexpr (GATE)
+        if constexpr (GATE == 2)
             bulk_load(dst + 2 * row_bytes, static_cast<const uint4 *>(a.t.gate) + static_cast<int64_t>(row / rows_per_gate) * h8,
                       row_bytes, bar, rows_per_gate == 1 ? pol : l2_policy_evict_last());
     };
@@ -122,6 +123,16 @@ rms_residual_fwd_staged_kernel(const RmsResidualFwdArgs a, const FwdPlan p, uint
     sum_of(0);
     const uint64_t stride = workers;
     for (uint64_t row = first;; row += stride, parity ^= 1u) {
+        uint4 gate[GATE == 1 ? VPT : 1];
+        if constexpr (GATE == 1) {
+            if (row < rows) {
+#pragma unroll
+                for (int j = 0; j < VPT; ++j) {
+                    const int idx = t + p.T * j;
+                    if (idx < h8) gate[j] = __ldg(static_cast<const uint4 *>(a.t.gate) + static_cast<int64_t>(static_cast<uint32_t>(row) / rows_per_gate) * h8 + idx);
+                }
+            }
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
             uu += __shfl_xor_sync(0xffffffffu, uu, o);
@@ -172,8 +183,9 @@ rms_residual_fwd_staged_kernel(const RmsResidualFwdArgs a, const FwdPlan p, uint
 #pragma unroll
                     for (int e = 0; e < 4; ++e) u[e] = mul2(mul2(u[e], r2), x[e]);
                 }
-                if constexpr (GATE) {
-                    vec_unpack2<BF16>(operand(ring, 2, idx), x);
+                if constexpr (GATE != 0) {
+                    if constexpr (GATE == 1) vec_unpack2<BF16>(gate[j], x);
+                    else vec_unpack2<BF16>(operand(ring, 2, idx), x);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) u[e] = mul2(u[e], x[e]);
                 }
@@ -202,28 +214,37 @@ rms_residual_fwd_staged_kernel(const RmsResidualFwdArgs a, const FwdPlan p, uint
     if (*abort_flag) __nanosleep(50000);       // let bulk copies still in flight land
 }
 
-FwdPlan make_plan(const RmsResidualTerms &t) {
+FwdPlan make_plan(const RmsResidualTerms &t, int sms) {
     FwdPlan p = {};
     const int64_t h8 = t.h / 8;
     if (h8 > 1024) return p;
     const int T = static_cast<int>(((h8 + kVpt - 1) / kVpt + 31) / 32 * 32);
     p.G = kMaxThreads / T;
     if (p.G > kMaxGroups) p.G = kMaxGroups;
-    p.slot_bytes = static_cast<uint32_t>(h8) * 16 * (t.gate ? 3 : 2);
     p.off_slot = static_cast<uint32_t>(h8) * 32 * (t.res_scale && !t.res_scale_one ? 3 : 2);
     const uint32_t fixed = p.G * (T / 32) * 2 * 8 + 16 + kMaxGroups * kMaxPerGroup * 8 + 16;
-    p.per_group = static_cast<int>((kSmemMost - p.off_slot - fixed) / p.slot_bytes) / p.G;
     // About 112 KiB of rows in flight from HBM, at least two slots for a group and three for a lone one (whose next row
     // has to be there while it works).  [rows, h] bf16, 134 M elements, us with 2 / 3 / 4 slots: h = 1024 (8 groups)
     // 196 / 180 / 192, 2048 (6) 171 / 192 / 193, 5120 (2) 202 / 163-181 / 167-188, with a gate per row 224 / 236 / 234,
     // 8192 (1) 281 / 174 / 166, with a gate per row 302 / 200 / 203.
     const bool token_gate = t.gate && t.gate_rows == t.rows;
     const int hbm_row = static_cast<int>(h8) * 16 * (token_gate ? 3 : 2) * p.G;
+    const int least = p.G == 1 ? 3 : 2;
     int want = (112 * 1024 + hbm_row / 2) / hbm_row;
-    if (want < (p.G == 1 ? 3 : 2)) want = p.G == 1 ? 3 : 2;
+    if (want < least) want = least;
     if (want > kMaxPerGroup) want = kMaxPerGroup;
-    if (p.per_group > want) p.per_group = want;
+    const auto slots_of = [&](int operands) {
+        const int n = static_cast<int>((kSmemMost - p.off_slot - fixed) / (static_cast<uint32_t>(h8) * 16 * operands)) / p.G;
+        return n > want ? want : n;
+    };
+    // A gate of several rows is staged with each of them where the ring keeps the least number of slots; else the threads
+    // read it from L2 themselves, unless the runs are short.  [16384, 8192], 8 gates, us staged / read: res_scale per column
+    // (two slots) 261 / 218, a single one (three) 189 / 207; [32768, 4096] 182 / 194, [131072, 1024] 176 / 190; short runs:
+    // [1003, 5120] 13.8 / 14.8.
+    p.staged_gate = t.gate && (token_gate || slots_of(3) >= least || t.rows < static_cast<int64_t>(sms) * p.G * 6);
+    p.per_group = slots_of(p.staged_gate ? 3 : 2);
     if (p.per_group < 1) return p;
+    p.slot_bytes = static_cast<uint32_t>(h8) * 16 * (p.staged_gate ? 3 : 2);
     p.T = T;
     p.off_red = p.off_slot + p.G * p.per_group * p.slot_bytes;
     p.off_bar = (p.off_red + p.G * (T / 32) * 2 * 8 + 15) / 16 * 16;
@@ -231,7 +252,7 @@ FwdPlan make_plan(const RmsResidualTerms &t) {
     return p;
 }
 
-template <bool BF16, bool GATE, bool SCALE_COL, bool FULL>
+template <bool BF16, int GATE, bool SCALE_COL, bool FULL>
 cudaError_t launch_fwd(const RmsResidualFwdArgs &a, const FwdPlan &p, int sms, int *status, cudaStream_t stream) {
     auto kernel = rms_residual_fwd_staged_kernel<BF16, GATE, SCALE_COL, FULL>;
     static DeviceOnce once;
@@ -257,15 +278,16 @@ cudaError_t launch_terms(const RmsResidualFwdArgs &a, const FwdPlan &p, int sms,
 #define PG_FWD(GATE, COL)                                                             \
     (full ? launch_fwd<BF16, GATE, COL, true>(a, p, sms, status, stream)              \
           : launch_fwd<BF16, GATE, COL, false>(a, p, sms, status, stream))
-    if (a.t.gate) return col ? PG_FWD(true, true) : PG_FWD(true, false);
-    return col ? PG_FWD(false, true) : PG_FWD(false, false);
+    if (!a.t.gate) return col ? PG_FWD(0, true) : PG_FWD(0, false);
+    if (!p.staged_gate) return col ? PG_FWD(1, true) : PG_FWD(1, false);
+    return col ? PG_FWD(2, true) : PG_FWD(2, false);
 #undef PG_FWD
 }
 
 }  // namespace
 
 bool rmsnorm_residual_staged_fwd_supported(const RmsResidualTerms &t, int sms) {
-    const FwdPlan p = make_plan(t);
+    const FwdPlan p = make_plan(t, sms);
     // every worker has a row (a CTA's groups begin with one each)
     return p.T != 0 && t.rows >= static_cast<int64_t>(sms) * p.G;
 }
@@ -274,7 +296,7 @@ cudaError_t rmsnorm_residual_staged_fwd(const RmsResidualFwdArgs &a, cudaStream_
     int sms = 0, *status = nullptr;
     const cudaError_t e = rmsnorm_device(&sms, &status);
     if (e != cudaSuccess) return e;
-    const FwdPlan p = make_plan(a.t);
+    const FwdPlan p = make_plan(a.t, sms);
     return a.t.bf16 ? launch_terms<true>(a, p, sms, status, stream) : launch_terms<false>(a, p, sms, status, stream);
 }
 

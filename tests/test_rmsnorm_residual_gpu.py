@@ -114,6 +114,16 @@ def test_gates_over_any_number_of_rows(cuda, rows, gates):
     check_backward(x, s, backward(x, s))
 
 
+@pytest.mark.parametrize("rows,h,gates,res,pre", [(1800, 8192, 5, 8192, True), (1800, 8000, 450, 8000, False),
+                                                  (300, 16384, 6, 1, True), (40, 32760, 8, 32760, True)])
+def test_wide_rows_share_gates(cuda, rows, h, gates, res, pre):
+    """Gates that do not fit the ring beside the rows; rows of several blocks, more of them than fit the device at once."""
+    x = make(rows, h, BF16, 69, pre=pre, gates=gates, res_scale=res)
+    s, y = forward(x)
+    check_forward(x, s, y)
+    check_backward(x, s, backward(x, s))
+
+
 def test_benchmark_size(cuda):
     x = make(8192, 4096, BF16, 64, gates=8, res_scale=1)
     s, y = forward(x)
