@@ -9,6 +9,7 @@
 //                 256 x BN x 16 MMA that reads both CTAs' shared memory and writes
 //                 both CTAs' tensor memory                 (tcgen05 cta_group::2)
 //   BN         tile width (64, 128, 256)
+//   LORA       every row's low-rank adapter is added as more blocks of k (lora_epilogue.cuh)
 //   STAGES     depth of the TMA -> MMA shared-memory ring (>= 4)
 //   MT         row blocks per CTA.  1: the tile is 128*CTA_GROUP rows.  2 (CTA pair, BN = 256): the pair owns a
 //              512 x 256 tile as two 256-row blocks that share every k-block of B; their two accumulators fill

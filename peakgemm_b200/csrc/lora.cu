@@ -11,11 +11,15 @@
 //
 // Down projection, per 128 rows of a (one tile): the adapters that occur in the tile's group of rows are listed in the
 // order of their first row; their A_i, `rank` rows of k elements each, stand below one another as the second operand,
-// cut into chunks of 64 to 128 rows, as many as the grid has clusters.  A cluster computes 128 rows x a chunk with tcgen05 (every row of a against
-// every listed adapter: the tensor pipe has time to spare, a and A_i are what costs), each CTA of the cluster a slice
-// of k; the partial sums meet through distributed shared memory in rank order.  Each CTA then writes its rows of V:
-// the scaled value, rounded once to the 16-bit type (the next product's operand type), for the rows that use the
-// adapter, zeros for the others (selected, not multiplied: a row's NaN stays its own).
+// cut into chunks of 64 to 128 rows, as many as the grid has clusters.  A cluster computes 128 rows x a chunk with
+// tcgen05 (every row of a against every listed adapter: the tensor pipe has time to spare, a and A_i are what costs),
+// each CTA of the cluster a slice of k; the partial sums meet through distributed shared memory in rank order.  Each CTA
+// then writes its rows of V: the scaled value, rounded once to the 16-bit type (the next product's operand type), for the
+// rows that use the adapter, zeros for the others (selected, not multiplied: a row's NaN stays its own).
+//
+// Bound by latency and by what one SM pulls from HBM, about 55 GB/s whatever the ring's depth: some 9 us of launch, first
+// loads, exchange and V, and 0.4 us per 24 KiB k-block.  128 x 4096 x 14336, 20 adapters of rank 64: 24.4 us alone (40 MB
+// from DRAM), the whole call 50 us where the product alone takes 27; 1003 x 4104 x 5128, 5 of rank 24: 54 of 41.
 
 #include <cuda.h>
 #include <cuda_runtime.h>
