@@ -93,6 +93,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst_smem, const void *src, ui
                  : "memory");
 }
 
+// A warp's sums to the buffer place `at` of every CTA of the cluster, arriving on the barrier at `bar` there.
+__device__ __forceinline__ void send_sums(uint32_t at, uint32_t bar, uint32_t cta, float x, float y, float z) {
+    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
+                 ::"r"(ptx::mapa(at, cta)), "f"(x), "f"(y), "f"(z), "f"(0.f), "r"(ptx::mapa(bar, cta)) : "memory");
+}
+
 // Named barrier `id` over `nthreads` consumer threads that also ORs a predicate across
 // them, so that "somebody abandoned a wait" is decided identically by the whole group.
 __device__ __forceinline__ bool group_barrier_or(uint32_t id, uint32_t nthreads, bool pred) {

@@ -79,6 +79,8 @@ struct RmsResidualParts {
     double *scale_one;      // n_one of them, where res_scale has one element
     uint32_t workers, n_one;
 };
+// Clusters of C CTAs, one to an SM, that the device holds at once (C a power of two up to 8).
+int rmsnorm_residual_clusters(int C, int sms);
 // Bulk-copy staged forward kernel (rmsnorm_residual_staged_fwd.cu), where it has the width and every worker a row.
 bool rmsnorm_residual_staged_fwd_supported(const RmsResidualTerms &t, int sms);
 cudaError_t rmsnorm_residual_staged_fwd(const RmsResidualFwdArgs &a, cudaStream_t stream);

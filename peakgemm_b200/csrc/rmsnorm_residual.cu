@@ -53,8 +53,8 @@ __device__ __forceinline__ void load_scale(const RmsResidualTerms &t, int idx, f
 // ---------------------------------------------------------------- forward ----
 
 // One block per row, thread t owns the vectors t, t + blockDim.x, ... (at most VPT) and holds the row in registers.
-// For few rows, and for 8192 < h <= 16384.  Bound by latency (loads, two block sums): [1, 4096] 3.3 us, [64, 8192] 4.5 us
-// with a launch of about 2.5 us, [8192, 16384] 282-316 us (0.55-0.65 of the copy bandwidth).
+// For few rows of h <= 16384.  Bound by latency (loads, two block sums): [1, 4096] 3.3 us, [64, 8192] 4.5 us with a
+// launch of about 2.5 us.
 template <int VPT, bool BF16>
 __global__ void __launch_bounds__(1024)
 rms_residual_fwd_kernel(const RmsResidualFwdArgs a, uint32_t rows_per_gate) {
@@ -134,7 +134,7 @@ rms_residual_fwd_kernel(const RmsResidualFwdArgs a, uint32_t rows_per_gate) {
     }
 }
 
-// Any h: the row is read three times (the second and third reads hit L2); [4096, 32768] 398-436 us, 0.4 of the copy
+// Any h: the row is read three times (the second and third reads hit L2); [2048, 65536] 384-416 us, 0.4-0.5 of the copy
 // bandwidth.  Nothing is written before the last pass, so s may be the residual and y may be u here too.
 template <bool BF16>
 __global__ void __launch_bounds__(1024)

@@ -4,7 +4,7 @@
 //     shared-memory slots; a thread owns VPT vectors of eight columns for the whole run.
 //   * Operand rows (dy, s, ds, u, residual, a token's gate) arrive by cp.async.bulk, so that the bytes in flight do not
 //     depend on registers.  A group's first thread issues them itself, for a slot that its group has just emptied: a
-//     producer warp would be the 17th (21st) and cost every thread a quarter of its registers.
+//     producer warp would be the 17th and cost every thread a quarter of its registers.
 //   * Per row: the sums over s, dy, u -> one barrier -> D, dresidual and the column sums, the sum over
 //     e * gamma_post * u -> second barrier, after which the slot is refilled -> du.
 //   * dgate and dgamma_post both come from q = sum of D * uhat over the rows of a gate: dgate = gamma_post * q,
@@ -13,6 +13,9 @@
 //   * Rows of more than 4096 columns are shared by a cluster of 2, 4 or 8 CTAs, at most 4096 columns each: the gains and
 //     a few rows fit into shared memory, and two or more rows are in work per SM, which hides the sums' latency.  The
 //     warps of all CTAs send their sums to every CTA with st.async (data and arrival in one, no fence).
+// [32768, 4096] bf16, 8 gates, one res_scale: 330 us, 0.87 of the copy bandwidth; [4099, 5120] fp16, a gate per token, 75 us;
+// [16384, 8192], 8 gates, res_scale per column, 437 us (0.66); [8192, 16384] 481-550 us (0.52-0.65).  What bounds it now is
+// issue and latency at 16 warps an SM (half of the issue slots busy, DRAM at 55 %): 128 registers a thread hold the column sums.
 // The workers' parts of the column sums go to tables that rmsnorm_residual.cu adds up in a fixed order.
 
 #include <cuda_runtime.h>
@@ -52,8 +55,6 @@ struct Group {
 constexpr int kVpt = 2;                // vectors a thread owns: 128 registers a thread, 512 threads
 constexpr int kMaxThreads = 512;
 
-int clusters_at_once(int C, int sms);
-
 Group make_group(int64_t rows, int64_t h, int sms) {
     const int64_t h8 = h / 8;
     Group g = {0, 0, 1, 0, 0};
@@ -63,16 +64,10 @@ Group make_group(int64_t rows, int64_t h, int sms) {
     g.T = ((g.cols8 + kVpt - 1) / kVpt + 31) / 32 * 32;
     g.G = kMaxThreads / g.T;
     if (g.G > kMaxGroups) g.G = kMaxGroups;
-    g.clusters = clusters_at_once(g.C, sms);
+    g.clusters = rmsnorm_residual_clusters(g.C, sms);
     const int64_t per_cluster = (rows + g.clusters - 1) / g.clusters;
     if (g.G > per_cluster) g.G = static_cast<int>(per_cluster);
     return g;
-}
-
-// A warp's sums to the buffer place `at` of every CTA of the cluster, arriving on the barrier at `bar` there.
-__device__ __forceinline__ void send_sums(uint32_t at, uint32_t bar, uint32_t cta, float x, float y, float z) {
-    asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];"
-                 ::"r"(mapa(at, cta)), "f"(x), "f"(y), "f"(z), "f"(0.f), "r"(mapa(bar, cta)) : "memory");
 }
 
 // Which terms a call has, where the kernel is compiled for them: gate 0 none, 1 one for several rows, 2 one for each row;
@@ -140,7 +135,7 @@ rms_residual_bwd_staged_kernel(const RmsResidualBwdArgs a, const RmsResidualPart
         const int slot = at * p.G + g;
         const uint64_t pol = l2_policy_evict_first();              // every row is read once
         const void *src[kOperands] = {a.dy, a.s, a.ds, a.u, a.residual, a.t.gate};
-        mbar_arrive_expect_tx(bar_full + slot * 8, p.slot_bytes / p.row_bytes * row_bytes);
+        mbar_arrive_expect_tx(bar_full + slot * 8, CLUSTER ? p.slot_bytes / p.row_bytes * row_bytes : p.slot_bytes);
 #pragma unroll
         for (int o = 0; o < kOperands; ++o)
             if (p.place[o] >= 0)
@@ -436,40 +431,6 @@ rms_residual_bwd_staged_kernel(const RmsResidualBwdArgs a, const RmsResidualPart
     }
 }
 
-// Clusters of C CTAs that the device holds at once: fewer than sms / C, since a cluster's CTAs share a GPC.  With one
-// that has to wait for another to end, a call takes almost twice as long: [8192, 16384] bf16, 8 gates, 806 us with sms / 4
-// clusters of 4, 481 with those that fit.
-int clusters_at_once(int C, int sms) {
-    if (C == 1) return sms;
-    static DeviceOnce once;
-    static int table[kMaxDevices][3] = {};
-    int dev = 0;
-    const auto fill = [&]() {
-        auto kernel = rms_residual_bwd_staged_kernel<true, true, 3, true, false>;       // they differ in nothing that counts here
-        for (int i = 0; i < 3; ++i) {
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(static_cast<unsigned>(sms / (2 << i) * (2 << i)), 1, 1);
-            cfg.blockDim = dim3(kMaxThreads, 1, 1);
-            cfg.dynamicSmemBytes = kSmemMost;
-            cudaLaunchAttribute attr[1];
-            attr[0].id = cudaLaunchAttributeClusterDimension;
-            attr[0].val.clusterDim.x = 2u << i;
-            attr[0].val.clusterDim.y = 1;
-            attr[0].val.clusterDim.z = 1;
-            cfg.attrs = attr;
-            cfg.numAttrs = 1;
-            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMost));
-            if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&table[dev][i], kernel, &cfg);
-            if (e != cudaSuccess) return e;
-        }
-        return cudaSuccess;
-    };
-    int n = 0;
-    if (current_device(&dev) == cudaSuccess && once.run(dev, fill) == cudaSuccess) n = table[dev][C == 2 ? 0 : C == 4 ? 1 : 2];
-    else cudaGetLastError();
-    return n < 1 ? 1 : n;
-}
-
 // Slots and shared memory: the gains (and a res_scale per column), the ring, row sums, barriers, abort flag.
 StagedPlan make_staged_plan(const RmsResidualBwdArgs &a, int sms) {
     const Group g = make_group(a.t.rows, a.t.h, sms);
@@ -543,6 +504,40 @@ cudaError_t launch_terms(const RmsResidualBwdArgs &a, const RmsResidualParts &pa
 }
 
 }  // namespace
+
+// Clusters of C CTAs that the device holds at once: fewer than sms / C, since a cluster's CTAs share a GPC.  With one
+// that has to wait for another to end, a call takes almost twice as long: [8192, 16384] bf16, 8 gates, 806 us with sms / 4
+// clusters of 4, 481 with those that fit.
+int rmsnorm_residual_clusters(int C, int sms) {
+    if (C == 1) return sms;
+    static DeviceOnce once;
+    static int table[kMaxDevices][3] = {};
+    int dev = 0;
+    const auto fill = [&]() {
+        auto kernel = rms_residual_bwd_staged_kernel<true, true, 3, true, false>;       // they differ in nothing that counts here
+        for (int i = 0; i < 3; ++i) {
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(static_cast<unsigned>(sms / (2 << i) * (2 << i)), 1, 1);
+            cfg.blockDim = dim3(kMaxThreads, 1, 1);
+            cfg.dynamicSmemBytes = kSmemMost;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = 2u << i;
+            attr[0].val.clusterDim.y = 1;
+            attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmemMost));
+            if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&table[dev][i], kernel, &cfg);
+            if (e != cudaSuccess) return e;
+        }
+        return cudaSuccess;
+    };
+    int n = 0;
+    if (current_device(&dev) == cudaSuccess && once.run(dev, fill) == cudaSuccess) n = table[dev][C == 2 ? 0 : C == 4 ? 1 : 2];
+    else cudaGetLastError();
+    return n < 1 ? 1 : n;
+}
 
 uint32_t rmsnorm_residual_staged_workers(int64_t rows, int64_t h, int sms, uint32_t *ctas_per_row) {
     const Group g = make_group(rows, h, sms);

@@ -115,7 +115,9 @@ def test_gates_over_any_number_of_rows(cuda, rows, gates):
 
 
 @pytest.mark.parametrize("rows,h,gates,res,pre", [(1800, 8192, 5, 8192, True), (1800, 8000, 450, 8000, False),
-                                                  (300, 16384, 6, 1, True), (40, 32760, 8, 32760, True)])
+                                                  (300, 16384, 6, 1, True), (40, 32760, 8, 32760, True),
+                                                  (700, 8200, 7, 8200, True), (500, 12296, 500, 1, False),
+                                                  (333, 32768, 3, 32768, True)])
 def test_wide_rows_share_gates(cuda, rows, h, gates, res, pre):
     """Gates that do not fit the ring beside the rows; rows of several blocks, more of them than fit the device at once."""
     x = make(rows, h, BF16, 69, pre=pre, gates=gates, res_scale=res)
