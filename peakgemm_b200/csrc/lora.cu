@@ -6,7 +6,7 @@
 // launched under programmatic stream serialisation: it streams the shared weights while this kernel runs and waits for
 // it only in front of the tile's last block.
 //
-// Few tokens (at most 64) of small ranks take plain fp32 dot products (lora_dot_kernel): a handful of blocks without
+// Few tokens of small ranks take plain fp32 dot products (lora_dot_kernel): a handful of blocks without
 // set-up, a few microseconds, beside which the GEMM's CTAs fit on the same SMs.  Otherwise the tensor cores:
 //
 // Down projection, per 128 rows of a (one tile): the adapters that occur in the tile's group of rows are listed in the
