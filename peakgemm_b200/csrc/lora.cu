@@ -6,7 +6,7 @@
 // launched under programmatic stream serialisation: it streams the shared weights while this kernel runs and waits for
 // it only in front of the tile's last block.
 //
-// Few tokens of small ranks take plain fp32 dot products (lora_dot_kernel): a handful of blocks without
+// Few tokens, or few rank elements of many adapters, take plain fp32 dot products (lora_dot_kernel): blocks without
 // set-up, a few microseconds, beside which the GEMM's CTAs fit on the same SMs.  Otherwise the tensor cores:
 //
 // Down projection, per 128 rows of a (one tile): the adapters that occur in the tile's group of rows are listed in the
@@ -377,11 +377,15 @@ Plan make_plan(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank, 
     return p;
 }
 
-// Dot products read an adapter's rows once for every token: up to 32 MiB of them they are done sooner than a tcgen05
-// launch (9 us and more).
-bool dot_pays(int64_t m, int64_t k, int64_t rank) {
-    static const int env = tune_env_int("PEAKGEMM_TUNE_LORA_DOT_MB", 32);
-    return m * k * rank * 2 <= static_cast<int64_t>(env) << 20;
+// Dot products read an adapter's rows once for every token, a tcgen05 launch once for every tile that uses it, but against
+// all rows of the tile.  m x n x k, pool, rank, us of the whole call with dot products / tcgen05:
+//   64 tokens and fewer: 1 x 4096 x 4096, 8, 16 10.8 / 15.9; 64 x 4096 x 4096, 32, 64 26.9 / 38.9; 32 x 4096 x 14336, 4, 64
+//   29.8 / 40.0; 16 x 4096 x 16384 (64 MiB of such reads), 16, 128 42.1 / 62.1; 64 x 4096 x 8192 (128 MiB), 1, 128 30.6 / 30.8
+//   more, a large pool, mixed: 128 x 4096 x 4096, 32, 16 25.2 / 31.5; 256 x 4096 x 4096, 64, 16 (32 MiB) 39.8 / 48.0
+//   more, a small pool: 128 x 4096 x 4096, 1, 16 19.0 / 16.5, 8, 64 28.7 / 26.5; 256 x 4096 x 4096, 8, 16 25.3 / 21.4
+bool dot_pays(int64_t m, int64_t k, int64_t rank, int64_t adapters) {
+    const int64_t most = m <= 64 ? 128 : adapters > 16 ? 32 : 0;
+    return m * k * rank * 2 <= most << 20;
 }
 
 // CTAs of a cluster over k: as many as keep the tiles within one wave and leave every CTA four k-blocks.  Fewer, beside
@@ -424,7 +428,7 @@ int hgemm_lora_launch(const GemmArgs &g, const LoraArgs &l, cudaStream_t stream,
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (g.m <= 65535 && dot_pays(g.m, g.k, l.rank)) {
+    if (g.m <= 65535 && dot_pays(g.m, g.k, l.rank, l.adapters)) {
         cfg.gridDim = dim3(static_cast<unsigned>(l.rank / kDotRanks), static_cast<unsigned>(g.m), 1);
         cfg.blockDim = dim3(kDotWarps * 32, 1, 1);
         if ((e = cudaLaunchKernelEx(&cfg, g.bf16 ? lora_dot_kernel<true> : lora_dot_kernel<false>,

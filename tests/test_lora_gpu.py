@@ -89,6 +89,15 @@ def test_large(cuda, m, n, k, ids):
     check(x, call(x))
 
 
+# few tokens with more rank elements than dot products are for, more tokens with a pool they are for
+@pytest.mark.parametrize("m,k,adapters,rank", [(17, 8192, 3, 512), (40, 4104, 5, 512), (64, 8200, 9, 128), (1, 131080, 1, 512),
+                                               (65, 1032, 20, 16), (130, 520, 64, 24), (513, 264, 17, 8)])
+@pytest.mark.parametrize("ids", ["mixed", "runs"])
+def test_both_down_projections(cuda, m, k, adapters, rank, ids):
+    x = make(m, 264, k, adapters, rank, F16, 92, ids, terms=m % 2 == 0)
+    check(x, call(x))
+
+
 @pytest.mark.parametrize("terms", ["scale", "row_scale", "bias", "residual", ""])
 @pytest.mark.parametrize("m", [5, 130, 600])
 def test_each_term_alone(cuda, m, terms):
