@@ -174,8 +174,9 @@ int pg_hgemm_fused(void *d, const void *a, const void *b,
  * uses adapter t = ids[i] of a pool, or none,
  *     d[i,j] = round_to_dtype(row_scale[i] * (sum_k a[i,k] b[j,k] + scale[t] * sum_r v[i,r] lora_b[t,j,r]) + bias[j]
  *                             + residual[i,j]),        v[i,r] = sum_k a[i,k] lora_a[t,r,k]
- * with fp32 sums and optional terms as there; scale[t] * v[i,r] is rounded once to `dtype`, the operand type of the
- * second product (fp16: its magnitude has to stay below 65504).  Every different adapter among the 128 to 512
+ * with fp32 sums and optional terms as there; scale[t] * v[i,r] goes into the second product as the sum of two values of
+ * `dtype`, its operand type, which leaves an error of 2^-16 of it in bf16, 2^-22 in fp16 (fp16: its magnitude has to stay
+ * below 65504).  Every different adapter among the 128 to 512
  * consecutive rows that share a tile is work for the whole tile: keep the rows of an adapter adjacent in large batches.
  *   lora_a   [adapters, rank, k] of `dtype`, dense: the down projections, in the weights' layout
  *   lora_b   [adapters, n, rank] of `dtype`, dense: the up projections, in the weights' layout

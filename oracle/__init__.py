@@ -341,15 +341,16 @@ def rmsnorm_residual_inputs(rows: int, h: int, dtype: torch.dtype, seed: int, *,
 # --------------------------------------------------- adapters beside a projection ----
 # PARITY UNPINNED: the reference has no adapters; the definition in float64, on the inputs' device.
 
-def gemm_lora(a, b, lora_a, lora_b, ids, scale=None, row_scale=None, bias=None, residual=None):
+def gemm_lora(a, b, lora_a, lora_b, ids, scale=None, row_scale=None, bias=None, residual=None, v_terms: int = 1):
     """(d, bound) unrounded, float64.
 
     bound: fp32 sums of products in another order are within 2^-17 of the sum of absolute values (gemm_fused_slack);
-    v = scale * a A^T may be rounded once to the 16-bit type before the second product: half a step, eps / 2 of itself
-    (and half the smallest step, where v is below the normal range)."""
+    v = scale * a A^T may go into the second product as the sum of v_terms values of the 16-bit type, each the rounding of
+    what the ones before leave: half a step, eps / 2, of itself with one term, (eps / 2)^2 with two (and half the smallest
+    step, where what is rounded is below the normal range)."""
     L, r, k = lora_a.shape
     ids = ids.long()
-    u16 = torch.finfo(a.dtype).eps / 2
+    u16 = (torch.finfo(a.dtype).eps / 2) ** v_terms
     tiny = torch.finfo(a.dtype).smallest_normal * torch.finfo(a.dtype).eps / 2
     x, w = a.double(), b.double()
     d, e = x @ w.t(), 2.0 ** -17 * (x.abs() @ w.abs().t())

@@ -125,7 +125,7 @@ def gemm_peak_lora(d: torch.Tensor, a: torch.Tensor, b: torch.Tensor, lora_a: to
     ``ids``: int32, one per row of ``a``, in any order; an id outside 0..L-1 (such as -1) means no adapter.  ``scale``:
     float32 [L].  The other terms as in ``gemm_peak_fused``; with ``row_scale`` = rstd (``rms_norm_linear``) fold gamma
     into lora_a as into the weights: ``fold_gamma(lora_a.view(-1, k), gamma).view_as(lora_a)``.
-    ``scale[i] * (a[t] @ lora_a[i]^T)`` is rounded once to a's dtype.  In batches of many hundred rows keep the rows of an
+    ``scale[i] * (a[t] @ lora_a[i]^T)`` keeps twice the bits of a's dtype (fp16: it has to stay below 65504).  In batches of many hundred rows keep the rows of an
     adapter adjacent: each adapter among the rows of a tile is work for the whole tile.
     """
     assert a.dtype in [torch.half, torch.bfloat16]

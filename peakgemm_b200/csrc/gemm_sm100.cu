@@ -548,20 +548,21 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     if (!ok) break;
                     load_block(u.kb1 - 1);
                     for (uint32_t kb = u.kb1; kb < u.kb1 + extra.count; ++kb) {
-                        const uint32_t parts = extra.parts(lora.d), width2 = lora.d.width * 2;
-                        take_stage(C::kStageBytes / (2 * kBK) * width2 * parts, extra.info(lora.d, kb, u.kb1));
+                        const uint32_t parts = extra.parts(lora.d);
+                        const uint32_t v_bytes = lora_v_row_bytes(lora.d), b_bytes = lora_b_row_bytes(lora.d);
+                        take_stage((MT * kBM * v_bytes + C::kBRows * b_bytes) * parts, extra.info(lora.d, kb, u.kb1));
                         if (!ok) break;
                         const uint32_t fb = (CTA_GROUP == 2) ? full0 + stage * 8 : bar_full + stage * 8;
                         for (uint32_t i = 0; i < parts; ++i) {
                             const int32_t rx = extra.next(lora.d);
 #pragma unroll
                             for (uint32_t mt = 0; mt < MT; ++mt) {
-                                const uint32_t da = smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox + i * kBM * width2;
+                                const uint32_t da = smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox + i * kBM * v_bytes;
                                 const int32_t rv = extra.v_row + static_cast<int32_t>(mt * kBlockM + rank * kBM);
-                                if constexpr (CTA_GROUP == 2) tma_load_2d_pair(da, &lora.tm_v, fb, rx, rv);
-                                else tma_load_2d(da, &lora.tm_v, fb, rx, rv);
+                                if constexpr (CTA_GROUP == 2) tma_load_2d_pair(da, &lora.tm_v, fb, 2 * rx, rv);
+                                else tma_load_2d(da, &lora.tm_v, fb, 2 * rx, rv);
                             }
-                            const uint32_t db = smem_base + C::kOffB + stage * C::kBBytes + i * C::kBRows * width2;
+                            const uint32_t db = smem_base + C::kOffB + stage * C::kBBytes + i * C::kBRows * b_bytes;
                             if constexpr (CTA_GROUP == 2) tma_load_2d_pair(db, &lora.tm_b, fb, rx, extra.b_row + row_b);
                             else tma_load_2d(db, &lora.tm_b, fb, rx, extra.b_row + row_b);
                         }
@@ -627,10 +628,10 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                         last = (info & kLoraLast) != 0;
 #pragma unroll
                         for (uint32_t mt = 0; mt < MT; ++mt)
-                            lora_stage_mma<CTA_GROUP>(tmem_base + (MT == 2 ? mt : acc) * BN,
-                                                      smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox,
-                                                      smem_base + C::kOffB + stage * C::kBBytes, kBM, C::kBRows, idesc,
-                                                      info & 0x77u, lora.d.width);
+                            lora_stage_mma<CTA_GROUP, true>(tmem_base + (MT == 2 ? mt : acc) * BN,
+                                                            smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox,
+                                                            smem_base + C::kOffB + stage * C::kBBytes, kBM, C::kBRows, idesc,
+                                                            info & 0x77u, lora.d);
                         umma_commit<CTA_GROUP>(bar_empty + stage * 8);
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                     }
@@ -1097,13 +1098,14 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 if constexpr (LORA) {
                     if (kb + 1 >= kb1) stage_info[stage] = extra.info(lora.d, kb, kb1);
                     if (kb >= kb1) {
-                        const uint32_t parts = extra.parts(lora.d), width2 = lora.d.width * 2;
-                        mbar_arrive_expect_tx(bar_full + stage * 8, parts * width2 * (kBM + BN));
+                        const uint32_t parts = extra.parts(lora.d);
+                        const uint32_t v_bytes = lora_v_row_bytes(lora.d), b_bytes = lora_b_row_bytes(lora.d);
+                        mbar_arrive_expect_tx(bar_full + stage * 8, parts * (kBM * v_bytes + BN * b_bytes));
                         for (uint32_t i = 0; i < parts; ++i) {
                             const int32_t rx = extra.next(lora.d);
-                            tma_load_2d(smem_base + C::kOffA + stage * C::kABytes + i * kBM * width2, &lora.tm_v,
-                                        bar_full + stage * 8, rx, extra.v_row);
-                            tma_load_2d(smem_base + C::kOffB + stage * C::kBBytes + i * BN * width2, &lora.tm_b,
+                            tma_load_2d(smem_base + C::kOffA + stage * C::kABytes + i * kBM * v_bytes, &lora.tm_v,
+                                        bar_full + stage * 8, 2 * rx, extra.v_row);
+                            tma_load_2d(smem_base + C::kOffB + stage * C::kBBytes + i * BN * b_bytes, &lora.tm_b,
                                         bar_full + stage * 8, rx, extra.b_row + static_cast<int32_t>(ni * BN));
                         }
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
@@ -1147,8 +1149,8 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     tc_fence_after_sync();
                     const uint32_t info = stage_info[stage];
                     last = (info & kLoraLast) != 0;
-                    lora_stage_mma<1>(tmem_base, smem_base + C::kOffA + stage * C::kABytes,
-                                      smem_base + C::kOffB + stage * C::kBBytes, kBM, BN, idesc, info & 0x77u, lora.d.width);
+                    lora_stage_mma<1, true>(tmem_base, smem_base + C::kOffA + stage * C::kABytes,
+                                            smem_base + C::kOffB + stage * C::kBBytes, kBM, BN, idesc, info & 0x77u, lora.d);
                     umma_commit<1>(bar_empty + stage * 8);
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
@@ -1641,14 +1643,15 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                 if constexpr (LORA) {
                     if (kb + 1 >= kb1) stage_info[stage] = extra.info(lora.d, kb, kb1);
                     if (kb >= kb1) {
-                        const uint32_t parts = extra.parts(lora.d), width2 = lora.d.width * 2;
-                        mbar_arrive_expect_tx(bar_full + stage * 8, parts * width2 * (kBM + TOK));
+                        const uint32_t parts = extra.parts(lora.d);
+                        const uint32_t v_bytes = lora_v_row_bytes(lora.d), b_bytes = lora_b_row_bytes(lora.d);
+                        mbar_arrive_expect_tx(bar_full + stage * 8, parts * (kBM * b_bytes + TOK * v_bytes));
                         for (uint32_t i = 0; i < parts; ++i) {
                             const int32_t rx = extra.next(lora.d);
-                            tma_load_2d(smem_base + C::kOffW + stage * C::kWBytes + i * kBM * width2, &lora.tm_b,
+                            tma_load_2d(smem_base + C::kOffW + stage * C::kWBytes + i * kBM * b_bytes, &lora.tm_b,
                                         bar_full + stage * 8, rx, extra.b_row + static_cast<int32_t>(ni * kBM));
-                            tma_load_2d(smem_base + C::kOffT + stage * C::kTBytes + i * TOK * width2, &lora.tm_v,
-                                        bar_full + stage * 8, rx, extra.v_row);
+                            tma_load_2d(smem_base + C::kOffT + stage * C::kTBytes + i * TOK * v_bytes, &lora.tm_v,
+                                        bar_full + stage * 8, 2 * rx, extra.v_row);
                         }
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                         continue;
@@ -1691,8 +1694,8 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                     tc_fence_after_sync();
                     const uint32_t info = stage_info[stage];
                     last = (info & kLoraLast) != 0;
-                    lora_stage_mma<1>(tmem_base, smem_base + C::kOffW + stage * C::kWBytes,
-                                      smem_base + C::kOffT + stage * C::kTBytes, kBM, TOK, idesc, info & 0x77u, lora.d.width);
+                    lora_stage_mma<1, false>(tmem_base, smem_base + C::kOffT + stage * C::kTBytes,
+                                             smem_base + C::kOffW + stage * C::kWBytes, TOK, kBM, idesc, info & 0x77u, lora.d);
                     umma_commit<1>(bar_empty + stage * 8);
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
@@ -1964,10 +1967,11 @@ bool fill_lora(LoraParam<true> *p, const GemmArgs &g, uint32_t v_rows, uint32_t 
     p->d = {l.ids, l.table, static_cast<const uint16_t *>(l.v), static_cast<const uint16_t *>(l.b),
             static_cast<const uint16_t *>(g.a), static_cast<const uint16_t *>(g.b), g.lda, g.ldb,
             static_cast<uint32_t>(g.k), static_cast<uint32_t>(g.n), static_cast<uint32_t>(l.rank),
-            static_cast<uint32_t>((l.rank + kBK - 1) / kBK), l.rank <= 16 ? 16u : l.rank <= 32 ? 32u : 64u,
+            static_cast<uint32_t>(lora_v_cols(l.rank) / (2 * lora_width(l.rank))), lora_width(l.rank),
             static_cast<uint32_t>(l.max_slots),
             static_cast<uint32_t>(l.group_rows), static_cast<uint32_t>(l.table_stride)};
-    return make_tmap(&p->tm_v, l.v, groups * l.max_slots * l.group_rows, l.rank, l.rank, v_rows, g.bf16, false, p->d.width) &&
+    const int64_t cols = lora_v_cols(l.rank);
+    return make_tmap(&p->tm_v, l.v, groups * l.max_slots * l.group_rows, cols, cols, v_rows, g.bf16, false, 2 * p->d.width) &&
            make_tmap(&p->tm_b, l.b, l.adapters * g.n, l.rank, l.rank, b_rows, g.bf16, false, p->d.width);
 }
 

@@ -6,6 +6,12 @@
 
 namespace pg {
 
+// Rank elements of a block of V's rows, which hold each block twice (lora_epilogue.cuh), and the elements of such a row.
+constexpr uint32_t lora_width(int64_t rank) { return rank <= 16 ? 16u : 32u; }
+constexpr int64_t lora_v_cols(int64_t rank) {
+    return (rank + lora_width(rank) - 1) / lora_width(rank) * (2 * lora_width(rank));
+}
+
 // What the GEMM kernels need to add the adapters' up projections (see lora_epilogue.cuh).
 struct LoraGemm {
     const int32_t *ids, *table;

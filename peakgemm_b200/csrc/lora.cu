@@ -14,7 +14,7 @@
 // cut into chunks of 64 to 128 rows, as many as the grid has clusters.  A cluster computes 128 rows x a chunk with
 // tcgen05 (every row of a against every listed adapter: the tensor pipe has time to spare, a and A_i are what costs),
 // each CTA of the cluster a slice of k; the partial sums meet through distributed shared memory in rank order.  Each CTA
-// then writes its rows of V: the scaled value, rounded once to the 16-bit type (the next product's operand type), for the
+// then writes its rows of V: the scaled value as two 16-bit terms (the next product's operand type) for the
 // rows that use the adapter, zeros for the others (selected, not multiplied: a row's NaN stays its own).
 //
 // Bound by latency and by what one SM pulls from HBM, about 55 GB/s whatever the ring's depth: some 9 us of launch, first
@@ -54,13 +54,33 @@ constexpr uint32_t kOffSlots = kOffIds + kMaxGroup * 4;         // the adapters 
 constexpr uint32_t kSmem = kOffSlots + kMaxGroup * 4 + 1024;
 static_assert(kSmem <= 232448, "exceeds 227 KiB of shared memory");
 
+// Eight values as two 16-bit terms: hi = round(f), lo = round(f - hi); what hi cannot hold (infinity, NaN) is hi's alone.
+template <bool BF16>
+__device__ __forceinline__ void split_terms(const float (&f)[8], uint4 &hi, uint4 &lo) {
+    float h[8], l[8];
+    hi = vec_pack<BF16>(f);
+    vec_unpack<BF16>(hi, h);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) l[e] = fabsf(h[e]) < __int_as_float(0x7f800000) ? f[e] - h[e] : 0.f;
+    lo = vec_pack<BF16>(l);
+}
+
 struct Shrink {
     const int32_t *ids;
     const float *scale;
     int32_t *table;
     uint4 *v;
     uint32_t m, k, adapters, rank, max_slots, group_rows, table_stride;
+    uint32_t width, v_cols8;       // of a block of V's rows, elements; of a row, vectors of eight
     uint32_t piece;                // rows of A per load: 8 .. 64, divides rank
+
+    // Where rank elements 8 r8 .. 8 r8 + 7 of V's row stand, in vectors; their lo terms are width / 8 behind.
+    __device__ __forceinline__ int64_t v_at(int64_t row, uint32_t r8) const {
+        const uint32_t w8 = width / 8;
+        return row * v_cols8 + r8 / w8 * (2 * w8) + r8 % w8;
+    }
+    // The last eight of an odd number of them: the MMA reads sixteen, so eight zeros follow.
+    __device__ __forceinline__ bool ends_odd(uint32_t r8) const { return (rank & 8u) && 8 * r8 + 8 == rank; }
 };
 
 template <bool BF16>
@@ -245,7 +265,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 if (in_group >= p.group_rows || row >= p.m) continue;
                 const int32_t id = ids[in_group];
                 const uint32_t at = c * chunk + 8 * g, slot = at / p.rank, r = at - slot * p.rank;
-                uint4 out = make_uint4(0, 0, 0, 0);
+                uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
                 if (slots[slot] == id) {
                     float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                     for (uint32_t s = 0; s < S; ++s) {
@@ -255,13 +275,15 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                         f[4] += b.x; f[5] += b.y; f[6] += b.z; f[7] += b.w;
                     }
                     const float scale = p.scale ? p.scale[id] : 1.f;
-                    out.x = pack2<BF16>(f[0] * scale, f[1] * scale);
-                    out.y = pack2<BF16>(f[2] * scale, f[3] * scale);
-                    out.z = pack2<BF16>(f[4] * scale, f[5] * scale);
-                    out.w = pack2<BF16>(f[6] * scale, f[7] * scale);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[e] *= scale;
+                    split_terms<BF16>(f, hi, lo);
                 }
                 const int64_t v_row = (static_cast<int64_t>(group) * p.max_slots + slot) * p.group_rows + in_group;
-                p.v[(v_row * p.rank + r) / 8] = out;
+                uint4 *out = p.v + p.v_at(v_row, r / 8);
+                out[0] = hi;
+                out[p.width / 8] = lo;
+                if (p.ends_odd(r / 8)) out[1] = out[p.width / 8 + 1] = make_uint4(0, 0, 0, 0);
             }
         }
         if (c + gridDim.y < chunks) {      // the receive buffer and the accumulator are free again everywhere
@@ -343,20 +365,26 @@ lora_dot_kernel(const uint4 *x, int64_t ldx8, const uint4 *a, const Shrink p) {
         if (threadIdx.x == 0) table[0] = static_cast<int32_t>(n);
         for (uint32_t i = threadIdx.x; i < n; i += kDotWarps * 32) table[1 + i] = slots[i];
     }
-    // the row of every slot: the scaled value, rounded once, in the slot of the row's adapter, zeros in the others
+    // the row of every slot: the scaled value in two terms in the slot of the row's adapter, zeros in the others
     for (uint32_t slot = threadIdx.x; slot < n; slot += kDotWarps * 32) {
-        uint2 out = make_uint2(0, 0);
+        uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
         if (slots[slot] == id) {
             const float scale = p.scale ? p.scale[id] : 1.f;
-            float v[kDotRanks] = {};
+            float v[8] = {};
 #pragma unroll
             for (uint32_t w = 0; w < kDotWarps; ++w)
 #pragma unroll
                 for (uint32_t r = 0; r < kDotRanks; ++r) v[r] += red[w][r];
-            out = make_uint2(pack2<BF16>(v[0] * scale, v[1] * scale), pack2<BF16>(v[2] * scale, v[3] * scale));
+#pragma unroll
+            for (uint32_t r = 0; r < kDotRanks; ++r) v[r] *= scale;
+            split_terms<BF16>(v, hi, lo);
         }
         const int64_t row = (static_cast<int64_t>(group) * p.max_slots + slot) * p.group_rows + (t - group0);
-        reinterpret_cast<uint2 *>(p.v)[(row * p.rank + r0) / 4] = out;
+        uint2 *out = reinterpret_cast<uint2 *>(p.v + p.v_at(row, r0 / 8)) + r0 % 8 / 4;      // half a vector
+        const uint32_t to_lo = p.width / 4;
+        out[0] = make_uint2(hi.x, hi.y);
+        out[to_lo] = make_uint2(lo.x, lo.y);
+        if (p.ends_odd(r0 / 8)) out[2] = out[to_lo + 2] = make_uint2(0, 0);
     }
 }
 
@@ -373,7 +401,7 @@ Plan make_plan(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank, 
     p.table_stride = (1 + p.max_slots + 3) / 4 * 4;
     p.v_rows = p.groups * p.max_slots * p.group_rows;
     p.off_v = (static_cast<size_t>(p.groups) * p.table_stride * 4 + 255) / 256 * 256;
-    p.bytes = p.off_v + static_cast<size_t>(p.v_rows) * rank * 2;
+    p.bytes = p.off_v + static_cast<size_t>(p.v_rows) * lora_v_cols(rank) * 2;
     return p;
 }
 
@@ -420,7 +448,8 @@ int hgemm_lora_launch(const GemmArgs &g, const LoraArgs &l, cudaStream_t stream,
 
     Shrink s = {l.ids, l.scale, table, reinterpret_cast<uint4 *>(v), static_cast<uint32_t>(g.m), static_cast<uint32_t>(g.k),
                 static_cast<uint32_t>(l.adapters), static_cast<uint32_t>(l.rank), static_cast<uint32_t>(p.max_slots),
-                static_cast<uint32_t>(p.group_rows), static_cast<uint32_t>(p.table_stride), 8};
+                static_cast<uint32_t>(p.group_rows), static_cast<uint32_t>(p.table_stride), lora_width(l.rank),
+                static_cast<uint32_t>(lora_v_cols(l.rank) / 8), 8};
     cudaLaunchConfig_t cfg = {};
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];

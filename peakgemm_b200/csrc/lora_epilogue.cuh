@@ -6,12 +6,13 @@
 // The contribution is added in fp32 before the one rounding, and the output is neither read again nor written twice.
 // A tile's rows form a group; lora.cu writes the group's adapters in the order of their first row ("slots") into a table
 // and the masked V of each slot, [group rows, rank], next to it.
-// A stage of the operand ring takes 64 elements of k: one block of a rank over 32, two adapters of a rank up to 32, four
-// of a rank up to 16.  Each is a part of its own in the stage, 64, 32 or 16 elements wide, with the swizzle of that
-// width (128, 64 or 32 bytes).  64 x 14336 x 4096, rank 16, 32 adapters in the batch: one adapter per stage, a ring of
-// 6 KiB stages, 44.6 us; four of them 37 us, of which the product alone takes 24.5.  What bounds the rest is the rate of
-// a TMA load of short rows, about 1.8 ns for each row of 32 bytes: 0.34 us per adapter and CTA.  Where a tile has few
-// adapters their blocks hide behind the product: 4096 x 14336 x 4096, 8 adapters in runs, 368 us of 364.
+// V is a sum and keeps its bits: it goes in as two 16-bit terms, hi = round(v) and lo = round(v - hi), both multiplied with
+// the same B_i, which leaves an error of (eps / 2)^2 of itself.  A row of V is `width` elements of hi, the lo of the same,
+// and so on; width is 16 for a rank up to 16, else 32.
+// A stage of the operand ring takes 64 elements of V's rows: 32 of a rank, or two adapters of a rank up to 16.  Each is a
+// part of its own in the stage, with the swizzle of its width (128 or 64 bytes for V, half as many for B_i).  64 x 14336 x 4096, rank 16, 32 adapters in the batch: 41.9 us, of which the product alone takes 24.5 (with V as one term,
+// four adapters in a stage, 37.3).  What bounds the rest is the rate of a TMA load of short rows, about 1.8 ns for each row
+// whatever its width, and the turn of a stage.  Where a tile has few adapters their blocks hide behind the product.
 #pragma once
 
 #include <cuda.h>
@@ -26,11 +27,11 @@ namespace {
 struct LoraDev {
     const int32_t *ids;         // [m]
     const int32_t *table;       // per group table_stride words: the number of slots, then the slots' adapters
-    const uint16_t *v;          // [groups][max_slots][group_rows][rank]
+    const uint16_t *v;          // [groups][max_slots][group_rows][2 * rank_blocks * width]
     const uint16_t *b;          // [adapters][n][rank]
     const uint16_t *x, *w;      // the product's operands
     int64_t ldx, ldw;
-    uint32_t k, n, rank, rank_blocks, width, max_slots, group_rows, table_stride;     // width: of a part, 16, 32 or 64
+    uint32_t k, n, rank, rank_blocks, width, max_slots, group_rows, table_stride;     // width: rank elements of a part
 };
 
 template <bool LORA> struct LoraParam {};
@@ -50,6 +51,8 @@ struct LoraBlocks {
     const int32_t *adapters = nullptr;
     int32_t v_row = 0, b_row = 0;      // of the part that next() returned
 
+    static __device__ __forceinline__ uint32_t pack(const LoraDev &d) { return kBK / (2 * d.width); }      // parts of a full stage
+
     __device__ __forceinline__ void load(const LoraDev &d, uint32_t group) {
         const int32_t *t = d.table + static_cast<size_t>(group) * d.table_stride;
         head = *reinterpret_cast<const int4 *>(t);
@@ -61,25 +64,25 @@ struct LoraBlocks {
         slot = first;
         slot_step = step;
         rb = 0;
-        const uint32_t mine = slots > first ? (slots - first + step - 1) / step : 0u, pack = kBK / d.width;
-        count = pack > 1 ? (mine + pack - 1) / pack : mine * d.rank_blocks;
+        const uint32_t mine = slots > first ? (slots - first + step - 1) / step : 0u;
+        count = d.width < 32 ? (mine + pack(d) - 1) / pack(d) : mine * d.rank_blocks;
     }
     // Parts of the stage that next() will fill.
     __device__ __forceinline__ uint32_t parts(const LoraDev &d) const {
-        return min(kBK / d.width, (slots - slot + slot_step - 1) / slot_step);
+        return min(pack(d), (slots - slot + slot_step - 1) / slot_step);
     }
     // The word of the stage that block kb goes to (block kb1 - 1 is the product's last).
     __device__ __forceinline__ uint32_t info(const LoraDev &d, uint32_t kb, uint32_t kb1) const {
         const uint32_t last = kb + 1 >= kb1 && kb + 1 - kb1 == count ? kLoraLast : 0u;
         if (kb < kb1) return kBK / kUmmaK | last;
-        return min(d.width, d.rank - rb * kBK + kUmmaK - 1) / kUmmaK | last | parts(d) << 4;
+        return min(d.width, d.rank - rb * d.width + kUmmaK - 1) / kUmmaK | last | parts(d) << 4;
     }
-    // Moves to the next part; returns its first rank element.
+    // Moves to the next part; returns its first rank element, half of its first column in V.
     __device__ __forceinline__ int32_t next(const LoraDev &d) {
         v_row = static_cast<int32_t>((base + slot) * d.group_rows);
         const int32_t adapter = slot == 0 ? head.y : slot == 1 ? head.z : slot == 2 ? head.w : adapters[slot];
         b_row = adapter * static_cast<int32_t>(d.n);
-        const int32_t x = static_cast<int32_t>(rb * kBK);
+        const int32_t x = static_cast<int32_t>(rb * d.width);
         if (++rb == d.rank_blocks) {
             rb = 0;
             slot += slot_step;
@@ -88,15 +91,25 @@ struct LoraBlocks {
     }
 };
 
-// The MMAs of a stage of adapter parts: A's parts from smem_a, a_rows rows each, B's from smem_b, b_rows rows each.
-template <int CTA_GROUP>
-__device__ __forceinline__ void lora_stage_mma(uint32_t tmem_d, uint32_t smem_a, uint32_t smem_b, uint32_t a_rows,
-                                               uint32_t b_rows, uint32_t idesc, uint32_t info, uint32_t width) {
+// Bytes of a part in the stage: a row of V's operand, a row of B_i's.
+__device__ __forceinline__ uint32_t lora_v_row_bytes(const LoraDev &d) { return d.width * 4; }
+__device__ __forceinline__ uint32_t lora_b_row_bytes(const LoraDev &d) { return d.width * 2; }
+
+// The MMAs of a stage of adapter parts: V's parts from smem_v, v_rows rows each, B_i's from smem_b, b_rows rows each.
+// V_FIRST: V is the MMA's A operand (its rows are the accumulator's), else its B operand.
+template <int CTA_GROUP, bool V_FIRST>
+__device__ __forceinline__ void lora_stage_mma(uint32_t tmem_d, uint32_t smem_v, uint32_t smem_b, uint32_t v_rows,
+                                               uint32_t b_rows, uint32_t idesc, uint32_t info, const LoraDev &d) {
     const uint32_t parts = info >> 4, steps = info & 7u;
+    const uint32_t v_bytes = lora_v_row_bytes(d), b_bytes = lora_b_row_bytes(d);
     for (uint32_t i = 0; i < parts; ++i) {
-        const uint64_t da = ptx::smem_desc_k(smem_a + i * a_rows * width * 2, width * 2);
-        const uint64_t db = ptx::smem_desc_k(smem_b + i * b_rows * width * 2, width * 2);
-        for (uint32_t k = 0; k < steps; ++k) ptx::umma_f16<CTA_GROUP>(tmem_d, da + 2 * k, db + 2 * k, idesc, 1u);
+        const uint64_t dv = ptx::smem_desc_k(smem_v + i * v_rows * v_bytes, v_bytes);
+        const uint64_t db = ptx::smem_desc_k(smem_b + i * b_rows * b_bytes, b_bytes);
+        for (uint32_t k = 0; k < 2 * steps; ++k) {               // hi, then lo: 32 bytes = +2 in the >>4 address field
+            const uint32_t lo = k >= steps ? 1u : 0u, at = k - lo * steps;
+            const uint64_t v = dv + 2 * (lo * d.width / kUmmaK + at), b = db + 2 * at;
+            ptx::umma_f16<CTA_GROUP>(tmem_d, V_FIRST ? v : b, V_FIRST ? b : v, idesc, 1u);
+        }
     }
 }
 
@@ -133,13 +146,17 @@ __device__ __noinline__ float lora_exact(const LoraDev &d, uint32_t group, uint3
     }
     if (mine >= 0) {
         const uint32_t in_group = row - group * d.group_rows;
+        const uint32_t w8 = d.width / 8;
         const uint4 *v = reinterpret_cast<const uint4 *>(d.v) +
-                         ((static_cast<int64_t>(group) * d.max_slots + mine) * d.group_rows + in_group) * r8;
+                         ((static_cast<int64_t>(group) * d.max_slots + mine) * d.group_rows + in_group) * (2 * d.rank_blocks * w8);
         const uint4 *b = reinterpret_cast<const uint4 *>(d.b) + (static_cast<int64_t>(id) * d.n + col) * r8;
         for (uint32_t r = 0; r < r8; ++r) {
-            vec_unpack<BF16>(v[r], f);
+            const uint4 *hi = v + r / w8 * (2 * w8) + r % w8;
+            float lo[8];
+            vec_unpack<BF16>(*hi, f);
+            vec_unpack<BF16>(hi[w8], lo);
             vec_unpack<BF16>(b[r], g);
-            for (int e = 0; e < 8; ++e) sum = fmaf(f[e], g[e], sum);
+            for (int e = 0; e < 8; ++e) sum = fmaf(f[e] + lo[e], g[e], sum);
         }
     }
     return sum;

@@ -98,6 +98,21 @@ def test_both_down_projections(cuda, m, k, adapters, rank, ids):
     check(x, call(x))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("m", [1, 17, 64, 100, 200, 300, 600])
+@pytest.mark.parametrize("rank", [8, 16, 24, 32, 40, 72, 512])
+def test_down_projection_keeps_its_bits(cuda, m, rank, dtype):
+    """The down projection's sums go into the second product as two 16-bit terms, within (eps / 2)^2 of themselves, not as
+    one.  Adapters that outweigh the product: there one term shows."""
+    x = make(m, 392, 264, 5, rank, dtype, 97)
+    x["b"] *= 2.0 ** -6
+    d = call(x)
+    torch.cuda.synchronize()
+    ref, bound = oracle.gemm_lora(**x, v_terms=2)
+    ok = helpers.elementwise_ok(d, ref.float(), (bound + 2.0 ** -24 * ref.abs()).float())
+    assert ok.all(), f"{int((~ok).sum())} of {ok.numel()} elements off, worst {(d.double() - ref).abs()[~ok].max().item():.3g}"
+
+
 @pytest.mark.parametrize("terms", ["scale", "row_scale", "bias", "residual", ""])
 @pytest.mark.parametrize("m", [5, 130, 600])
 def test_each_term_alone(cuda, m, terms):
