@@ -186,7 +186,10 @@ int pg_hgemm_fused(void *d, const void *a, const void *b,
  * row_scale = rstd, fold gamma into lora_a as into b.  adapters == 0 is pg_hgemm_fused.
  * rank % 8 == 0, 8 <= rank <= 512, adapters * rank and adapters * n < 2^31; otherwise pg_hgemm_fused's
  * preconditions.  residual may be d itself.  workspace: pg_hgemm_lora_workspace_bytes bytes, 256-byte aligned device
- * memory, no initialisation, private to the call until its kernels have finished.
+ * memory, no initialisation, private to the call until its kernels have finished: about 4 * m * rank (rank rounded up to
+ * 16, or to a multiple of 32) and, for each 128 to 512 rows, 20 to 68 bytes for each adapter that they can use; up to 64
+ * rows 4 * rank * rows * min(rows, adapters), rows rounded up to 16, 32 or 64.
+ * A value that is not finite, in an adapter or in a row of a, reaches only the rows that use the adapter, or that row.
  * The reference project has no adapters.
  */
 size_t pg_hgemm_lora_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank);

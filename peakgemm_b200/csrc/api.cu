@@ -28,7 +28,6 @@ int from_launch(int r, cudaError_t e) {
         case pg::kLaunchOk: return PG_OK;
         case pg::kLaunchCuda: return cuda_fail(e);
         case pg::kLaunchNotSm100: return PG_ERR_NOT_SM100;
-        case pg::kLaunchTooLarge: return PG_ERR_UNSUPPORTED;
         default: return PG_ERR_BAD_ARG;
     }
 }

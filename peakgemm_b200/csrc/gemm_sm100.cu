@@ -620,7 +620,15 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
                 if constexpr (LORA) {
+                    LoraLanes<MT * CTA_GROUP> lanes;
+                    if (ok && !last) {
+                        if (it == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+                        uint32_t mi, ni;
+                        tile_coords(group_m, u.tile, m_tiles, n_tiles, mi, ni, (flags & kFlagSerpentine) != 0);
+                        lanes.open(lora.d, mi);
+                    }
                     while (ok && !last) {            // the adapters' stages
+                        lanes.load(lora.d);
                         ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                         if (!ok) break;
                         tc_fence_after_sync();
@@ -631,7 +639,8 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                             lora_stage_mma<CTA_GROUP, true>(tmem_base + (MT == 2 ? mt : acc) * BN,
                                                             smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox,
                                                             smem_base + C::kOffB + stage * C::kBBytes, kBM, C::kBRows, idesc,
-                                                            info & 0x77u, lora.d);
+                                                            info & 0x77u, lora.d, lanes.off, mt * CTA_GROUP);
+                        lanes.step(lora.d, info >> 4);
                         umma_commit<CTA_GROUP>(bar_empty + stage * 8);
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                     }
@@ -699,11 +708,6 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     if (lane == 0) mbar_arrive_cluster(acc_empty_leader + mt * 8);
                     const bool row_ok = row0 + lane < M;
                     const float rs = fused ? epi_row_scale(epi, row_ok, row0 + lane) : 1.f;
-                    if constexpr (LORA) {
-#pragma unroll
-                        for (uint32_t cb = 0; cb < 4; ++cb)
-                            lora_repair<BF16>(v[cb], lora.d, mi, row0 + lane, ni * BN + half * 128u + cb * 32u, M);
-                    }
                     if (wide_boxes) {
                         // Stores that cross NVLink (peer destinations, or a multicast one): two 32 x 64 boxes with
                         // 128-byte rows over the warp's whole staging area, one at a time.  Half as many, twice as
@@ -897,11 +901,6 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                             d[2] = __float_as_uint(__uint_as_float(d[2]) + p.z);
                             d[3] = __float_as_uint(__uint_as_float(d[3]) + p.w);
                         }
-                    }
-                    if constexpr (LORA) {
-#pragma unroll
-                        for (uint32_t cb = 0; cb < 2; ++cb)
-                            lora_repair<BF16>(v[cb], lora.d, mi, row0 + lane, ni * BN + ch * kStoreCols + cb * 32u, M);
                     }
                     // the store issued two chunks ago from this buffer must have finished reading it
                     if (lane == 0) bulk_wait_group_read<1>();
@@ -1143,14 +1142,22 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
             if constexpr (LORA) {
+                LoraLanes<1> lanes;
+                if (ok && !last) {
+                    asm volatile("griddepcontrol.wait;" ::: "memory");
+                    lanes.open(lora.d, mi, rank, (k_blocks + per - 1) / per);
+                }
                 while (ok && !last) {                // the adapters' stages
+                    lanes.load(lora.d);
                     ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                     if (!ok) break;
                     tc_fence_after_sync();
                     const uint32_t info = stage_info[stage];
                     last = (info & kLoraLast) != 0;
                     lora_stage_mma<1, true>(tmem_base, smem_base + C::kOffA + stage * C::kABytes,
-                                            smem_base + C::kOffB + stage * C::kBBytes, kBM, BN, idesc, info & 0x77u, lora.d);
+                                            smem_base + C::kOffB + stage * C::kBBytes, kBM, BN, idesc, info & 0x77u, lora.d,
+                                            lanes.off, 0);
+                    lanes.step(lora.d, info >> 4);
                     umma_commit<1>(bar_empty + stage * 8);
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
@@ -1243,7 +1250,6 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     }
                     const uint32_t gcol = ni * BN + rank * W + 8u * g;
                     if (grow < M && gcol < N) {
-                        if constexpr (LORA) lora_repair<BF16, 8>(f, lora.d, mi, grow, gcol, M);
                         if (fused) epi_apply8<BF16>(f, rs, epi, true, grow, gcol);
                         uint4 out;
                         out.x = pack2<BF16>(f[0], f[1]);
@@ -1694,8 +1700,10 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                     tc_fence_after_sync();
                     const uint32_t info = stage_info[stage];
                     last = (info & kLoraLast) != 0;
+                    constexpr uint4 all[2][1] = {};
                     lora_stage_mma<1, false>(tmem_base, smem_base + C::kOffT + stage * C::kTBytes,
-                                             smem_base + C::kOffW + stage * C::kWBytes, TOK, kBM, idesc, info & 0x77u, lora.d);
+                                             smem_base + C::kOffW + stage * C::kWBytes, TOK, kBM, idesc, info & 0x77u, lora.d,
+                                             all, 0);
                     umma_commit<1>(bar_empty + stage * 8);
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
@@ -1765,7 +1773,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                     if (bad) {
 #pragma unroll
                         for (uint32_t mi = 0; mi < TOK; ++mi)
-                            if (mi < M && f[mi] != f[mi]) f[mi] = lora_exact<BF16>(lora.d, 0, mi, n_glob, f[mi]);
+                            if (mi < M && f[mi] != f[mi]) f[mi] = lora_exact<BF16>(lora.d, mi, n_glob, f[mi]);
                     }
                 }
                 if (epi.any()) {
@@ -1963,15 +1971,15 @@ EpiArgs make_epi(const GemmArgs &g) {
 bool fill_lora(LoraParam<false> *, const GemmArgs &, uint32_t, uint32_t) { return true; }
 bool fill_lora(LoraParam<true> *p, const GemmArgs &g, uint32_t v_rows, uint32_t b_rows) {
     const LoraGemm &l = *g.lora;
-    const int64_t groups = (g.m + l.group_rows - 1) / l.group_rows;
     p->d = {l.ids, l.table, static_cast<const uint16_t *>(l.v), static_cast<const uint16_t *>(l.b),
             static_cast<const uint16_t *>(g.a), static_cast<const uint16_t *>(g.b), g.lda, g.ldb,
             static_cast<uint32_t>(g.k), static_cast<uint32_t>(g.n), static_cast<uint32_t>(l.rank),
             static_cast<uint32_t>(lora_v_cols(l.rank) / (2 * lora_width(l.rank))), lora_width(l.rank),
             static_cast<uint32_t>(l.max_slots),
-            static_cast<uint32_t>(l.group_rows), static_cast<uint32_t>(l.table_stride)};
+            static_cast<uint32_t>(l.group_rows), static_cast<uint32_t>(l.slot_rows), static_cast<uint32_t>(l.table_stride),
+            static_cast<uint32_t>(l.mask_off)};
     const int64_t cols = lora_v_cols(l.rank);
-    return make_tmap(&p->tm_v, l.v, groups * l.max_slots * l.group_rows, cols, cols, v_rows, g.bf16, false, 2 * p->d.width) &&
+    return make_tmap(&p->tm_v, l.v, l.slot_rows ? l.max_slots * l.slot_rows : g.m, cols, cols, v_rows, g.bf16, false, 2 * p->d.width) &&
            make_tmap(&p->tm_b, l.b, l.adapters * g.n, l.rank, l.rank, b_rows, g.bf16, false, p->d.width);
 }
 

@@ -16,7 +16,7 @@ constexpr int64_t lora_v_cols(int64_t rank) {
 struct LoraGemm {
     const int32_t *ids, *table;
     const void *v, *b;
-    int64_t adapters, rank, max_slots, group_rows, table_stride;
+    int64_t adapters, rank, max_slots, group_rows, slot_rows, table_stride, mask_off;
 };
 
 struct GemmArgs {
@@ -43,7 +43,7 @@ struct GemmArgs {
     const LoraGemm *lora = nullptr;     // adapters beside b (hgemm_launch_with_lora only)
 };
 
-enum LaunchResult { kLaunchOk = 0, kLaunchCuda = 1, kLaunchNotSm100 = 2, kLaunchBadConfig = 3, kLaunchTooLarge = 4 };
+enum LaunchResult { kLaunchOk = 0, kLaunchCuda = 1, kLaunchNotSm100 = 2, kLaunchBadConfig = 3 };
 
 // variant: 0 auto, 1 = one CTA per tile, 2 = CTA pair per tile, 3 = cluster split-K, 4 = skinny,
 // 5 = CTA pair with two row blocks per CTA (512 x 256 tiles); block_n: 0 auto, 64, 128, 256.

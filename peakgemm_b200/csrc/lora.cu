@@ -15,7 +15,8 @@
 // tcgen05 (every row of a against every listed adapter: the tensor pipe has time to spare, a and A_i are what costs),
 // each CTA of the cluster a slice of k; the partial sums meet through distributed shared memory in rank order.  Each CTA
 // then writes its rows of V: the scaled value as two 16-bit terms (the next product's operand type) for the
-// rows that use the adapter, zeros for the others (selected, not multiplied: a row's NaN stays its own).
+// rows that use the adapter; where V is stored for each slot, zeros for the others (selected, not multiplied: a row's NaN
+// stays its own).
 //
 // Bound by latency and by what one SM pulls from HBM, about 55 GB/s whatever the ring's depth: some 9 us of launch, first
 // loads, exchange and V, and 0.4 us per 24 KiB k-block.  128 x 4096 x 14336, 20 adapters of rank 64: 24.4 us alone (40 MB
@@ -70,10 +71,14 @@ struct Shrink {
     const float *scale;
     int32_t *table;
     uint4 *v;
-    uint32_t m, k, adapters, rank, max_slots, group_rows, table_stride;
+    uint32_t m, k, adapters, rank, max_slots, group_rows, slot_rows, table_stride, mask_off;      // see LoraDev
     uint32_t width, v_cols8;       // of a block of V's rows, elements; of a row, vectors of eight
     uint32_t piece;                // rows of A per load: 8 .. 64, divides rank
 
+    // The mask word of row r of the group, and the 31 behind it, for a slot.
+    __device__ __forceinline__ int32_t &mask(uint32_t group, uint32_t slot, uint32_t r) const {
+        return table[static_cast<size_t>(group) * table_stride + mask_off + slot * (group_rows / 32) + r / 32];
+    }
     // Where rank elements 8 r8 .. 8 r8 + 7 of V's row stand, in vectors; their lo terms are width / 8 behind.
     __device__ __forceinline__ int64_t v_at(int64_t row, uint32_t r8) const {
         const uint32_t w8 = width / 8;
@@ -169,6 +174,15 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
         int32_t *t = p.table + static_cast<size_t>(group) * p.table_stride;
         if (threadIdx.x == 0) t[0] = static_cast<int32_t>(n_slots);
         for (uint32_t i = threadIdx.x; i < n_slots; i += kThreads) t[1 + i] = slots[i];
+    }
+    if (warp >= 2 && rank == 0 && p.slot_rows == 0) {
+        // which of the tile's rows do not use a slot's adapter; the last tile answers for the rest of its group too
+        const uint32_t in_group = row0 - group0, end = row0 + kBM >= p.m ? p.group_rows : in_group + kBM;
+        for (uint32_t s = blockIdx.y + gridDim.y * (warp - 2); s < n_slots; s += gridDim.y * 4)
+            for (uint32_t r = in_group; r < end; r += 32) {
+                const uint32_t off = __ballot_sync(0xffffffffu, ids[r + lane] != slots[s]);
+                if (lane == 0) p.mask(group, s, r) = off;
+            }
     }
     __syncwarp();              // the cluster barrier wants whole warps
     cluster_arrive();          // every CTA of the cluster is running before anyone writes into its shared memory
@@ -266,6 +280,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                 const int32_t id = ids[in_group];
                 const uint32_t at = c * chunk + 8 * g, slot = at / p.rank, r = at - slot * p.rank;
                 uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+                if (slots[slot] != id && p.slot_rows == 0) continue;
                 if (slots[slot] == id) {
                     float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
                     for (uint32_t s = 0; s < S; ++s) {
@@ -279,7 +294,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
                     for (int e = 0; e < 8; ++e) f[e] *= scale;
                     split_terms<BF16>(f, hi, lo);
                 }
-                const int64_t v_row = (static_cast<int64_t>(group) * p.max_slots + slot) * p.group_rows + in_group;
+                const int64_t v_row = p.slot_rows ? static_cast<int64_t>(slot) * p.slot_rows + row : row;
                 uint4 *out = p.v + p.v_at(v_row, r / 8);
                 out[0] = hi;
                 out[p.width / 8] = lo;
@@ -365,8 +380,17 @@ lora_dot_kernel(const uint4 *x, int64_t ldx8, const uint4 *a, const Shrink p) {
         if (threadIdx.x == 0) table[0] = static_cast<int32_t>(n);
         for (uint32_t i = threadIdx.x; i < n; i += kDotWarps * 32) table[1 + i] = slots[i];
     }
-    // the row of every slot: the scaled value in two terms in the slot of the row's adapter, zeros in the others
+    if (blockIdx.x == 0 && p.slot_rows == 0) {          // the group's blocks share the slots' masks
+        for (uint32_t s = t - group0; s < n; s += group_end - group0)
+            for (uint32_t r = warp * 32; r < p.group_rows; r += kDotWarps * 32) {
+                const int32_t other = group0 + r + lane < group_end ? checked(p.ids[group0 + r + lane]) : -1;
+                const uint32_t off = __ballot_sync(0xffffffffu, other != slots[s]);
+                if (lane == 0) p.mask(group, s, r) = off;
+            }
+    }
+    // the scaled value in two terms; V for each slot: in the slot of the row's adapter, zeros in the others
     for (uint32_t slot = threadIdx.x; slot < n; slot += kDotWarps * 32) {
+        if (slots[slot] != id && p.slot_rows == 0) continue;
         uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
         if (slots[slot] == id) {
             const float scale = p.scale ? p.scale[id] : 1.f;
@@ -379,7 +403,7 @@ lora_dot_kernel(const uint4 *x, int64_t ldx8, const uint4 *a, const Shrink p) {
             for (uint32_t r = 0; r < kDotRanks; ++r) v[r] *= scale;
             split_terms<BF16>(v, hi, lo);
         }
-        const int64_t row = (static_cast<int64_t>(group) * p.max_slots + slot) * p.group_rows + (t - group0);
+        const int64_t row = p.slot_rows ? static_cast<int64_t>(slot) * p.slot_rows + t : t;
         uint2 *out = reinterpret_cast<uint2 *>(p.v + p.v_at(row, r0 / 8)) + r0 % 8 / 4;      // half a vector
         const uint32_t to_lo = p.width / 4;
         out[0] = make_uint2(hi.x, hi.y);
@@ -389,7 +413,7 @@ lora_dot_kernel(const uint4 *x, int64_t ldx8, const uint4 *a, const Shrink p) {
 }
 
 struct Plan {
-    int64_t group_rows, groups, max_slots, table_stride, v_rows;
+    int64_t group_rows, groups, max_slots, slot_rows, table_stride, mask_off;
     size_t off_v, bytes;
 };
 
@@ -398,10 +422,12 @@ Plan make_plan(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank, 
     p.group_rows = lora_group_rows(m, n, k, sms);
     p.groups = (m + p.group_rows - 1) / p.group_rows;
     p.max_slots = adapters < p.group_rows ? adapters : p.group_rows;
-    p.table_stride = (1 + p.max_slots + 3) / 4 * 4;
-    p.v_rows = p.groups * p.max_slots * p.group_rows;
+    p.slot_rows = p.group_rows < kBM ? p.group_rows : 0;      // the kernel for few tokens
+    p.mask_off = (1 + p.max_slots + 3) / 4 * 4;
+    p.table_stride = p.mask_off + (p.slot_rows ? 0 : p.max_slots * (p.group_rows / 32));
+    const int64_t v_rows = p.slot_rows ? p.max_slots * p.slot_rows : m;
     p.off_v = (static_cast<size_t>(p.groups) * p.table_stride * 4 + 255) / 256 * 256;
-    p.bytes = p.off_v + static_cast<size_t>(p.v_rows) * lora_v_cols(rank) * 2;
+    p.bytes = p.off_v + static_cast<size_t>(v_rows) * lora_v_cols(rank) * 2;
     return p;
 }
 
@@ -442,13 +468,13 @@ int hgemm_lora_launch(const GemmArgs &g, const LoraArgs &l, cudaStream_t stream,
     if (e != cudaSuccess) return failed(e);
     if (cc != 10) return kLaunchNotSm100;
     const Plan p = make_plan(g.m, g.n, g.k, l.adapters, l.rank, sms);
-    if (p.v_rows > 2147483647) return kLaunchTooLarge;           // V's rows are counted in 32 bits
     int32_t *table = static_cast<int32_t *>(l.workspace);
     uint8_t *v = static_cast<uint8_t *>(l.workspace) + p.off_v;
 
     Shrink s = {l.ids, l.scale, table, reinterpret_cast<uint4 *>(v), static_cast<uint32_t>(g.m), static_cast<uint32_t>(g.k),
                 static_cast<uint32_t>(l.adapters), static_cast<uint32_t>(l.rank), static_cast<uint32_t>(p.max_slots),
-                static_cast<uint32_t>(p.group_rows), static_cast<uint32_t>(p.table_stride), lora_width(l.rank),
+                static_cast<uint32_t>(p.group_rows), static_cast<uint32_t>(p.slot_rows), static_cast<uint32_t>(p.table_stride),
+                static_cast<uint32_t>(p.mask_off), lora_width(l.rank),
                 static_cast<uint32_t>(lora_v_cols(l.rank) / 8), 8};
     cudaLaunchConfig_t cfg = {};
     cfg.stream = stream;
@@ -491,7 +517,8 @@ int hgemm_lora_launch(const GemmArgs &g, const LoraArgs &l, cudaStream_t stream,
         if ((e = cudaLaunchKernelEx(&cfg, kernel, tm_x, tm_a, s, status)) != cudaSuccess) return failed(e);
     }
 
-    const LoraGemm lg = {l.ids, table, v, l.b, l.adapters, l.rank, p.max_slots, p.group_rows, p.table_stride};
+    const LoraGemm lg = {l.ids, table, v, l.b, l.adapters, l.rank, p.max_slots, p.group_rows, p.slot_rows, p.table_stride,
+                         p.mask_off};
     GemmArgs with = g;
     with.lora = &lg;
     return hgemm_launch_with_lora(with, stream, cuda_err);

@@ -2,16 +2,19 @@
 //
 // The up projection is more k: with v[t] = scale * x[t] A^T (lora.cu) a tile's accumulator gets, behind the k-blocks of
 // x W^T, the rank elements of every adapter that occurs among the tile's rows:
-//     acc[t, j] += sum_r V[t, r] B_i[j, r],     V = v for the rows t that use adapter i, zeros for the others.
+//     acc[t, j] += sum_r v[t, r] B_i[j, r]      for the rows t that use adapter i, and no others.
 // The contribution is added in fp32 before the one rounding, and the output is neither read again nor written twice.
-// A tile's rows form a group; lora.cu writes the group's adapters in the order of their first row ("slots") into a table
-// and the masked V of each slot, [group rows, rank], next to it.
+// A tile's rows form a group; lora.cu writes the group's adapters in the order of their first row ("slots") into a table.
+// Where the tile's rows are the accumulator's lanes, the table holds a mask of the rows that do not use the slot's adapter,
+// and the MMA leaves those lanes as they are: V is stored once, and no row meets another one's adapter.  The kernel for few
+// tokens has the tokens as columns; there V is stored for each slot, zeros in the rows of other adapters, at most 64 x 64.
 // V is a sum and keeps its bits: it goes in as two 16-bit terms, hi = round(v) and lo = round(v - hi), both multiplied with
 // the same B_i, which leaves an error of (eps / 2)^2 of itself.  A row of V is `width` elements of hi, the lo of the same,
 // and so on; width is 16 for a rank up to 16, else 32.
 // A stage of the operand ring takes 64 elements of V's rows: 32 of a rank, or two adapters of a rank up to 16.  Each is a
-// part of its own in the stage, with the swizzle of its width (128 or 64 bytes for V, half as many for B_i).  64 x 14336 x 4096, rank 16, 32 adapters in the batch: 41.9 us, of which the product alone takes 24.5 (with V as one term,
-// four adapters in a stage, 37.3).  What bounds the rest is the rate of a TMA load of short rows, about 1.8 ns for each row
+// part of its own in the stage, with the swizzle of its width (128 or 64 bytes for V, half as many for B_i).
+// 64 x 14336 x 4096, rank 16, 32 adapters in the batch: 41.9 us, of which the product alone takes 24.5 (with V as one
+// term, four adapters in a stage, 37.3).  What bounds the rest is the rate of a TMA load of short rows, about 1.8 ns for each row
 // whatever its width, and the turn of a stage.  Where a tile has few adapters their blocks hide behind the product.
 #pragma once
 
@@ -26,12 +29,14 @@ namespace {
 
 struct LoraDev {
     const int32_t *ids;         // [m]
-    const int32_t *table;       // per group table_stride words: the number of slots, then the slots' adapters
-    const uint16_t *v;          // [groups][max_slots][group_rows][2 * rank_blocks * width]
+    const int32_t *table;       // per group table_stride words: the number of slots, the slots' adapters; from mask_off on
+                                // group_rows / 32 words for each slot, a bit set for every row that does not use it
+    const uint16_t *v;          // [m][2 * rank_blocks * width]; slot_rows > 0: [max_slots][slot_rows][...]
     const uint16_t *b;          // [adapters][n][rank]
     const uint16_t *x, *w;      // the product's operands
     int64_t ldx, ldw;
-    uint32_t k, n, rank, rank_blocks, width, max_slots, group_rows, table_stride;     // width: rank elements of a part
+    uint32_t k, n, rank, rank_blocks, width;      // width: rank elements of a part
+    uint32_t max_slots, group_rows, slot_rows, table_stride, mask_off;
 };
 
 template <bool LORA> struct LoraParam {};
@@ -46,7 +51,7 @@ constexpr uint32_t kLoraLast = 8u;
 
 // The producer's walk over a tile's adapters: slots first, first + step, ..., in `count` stages.
 struct LoraBlocks {
-    uint32_t count = 0, slot = 0, slot_step = 1, slots = 0, rb = 0, base = 0;
+    uint32_t count = 0, slot = 0, slot_step = 1, slots = 0, rb = 0, row0 = 0;
     int4 head = {0, 0, 0, 0};          // the table's first words: the number of slots and three adapters
     const int32_t *adapters = nullptr;
     int32_t v_row = 0, b_row = 0;      // of the part that next() returned
@@ -57,7 +62,7 @@ struct LoraBlocks {
         const int32_t *t = d.table + static_cast<size_t>(group) * d.table_stride;
         head = *reinterpret_cast<const int4 *>(t);
         adapters = t + 1;
-        base = group * d.max_slots;
+        row0 = group * d.group_rows;
     }
     __device__ __forceinline__ void open(const LoraDev &d, uint32_t first = 0, uint32_t step = 1) {
         slots = min(static_cast<uint32_t>(head.x), d.max_slots);
@@ -79,7 +84,7 @@ struct LoraBlocks {
     }
     // Moves to the next part; returns its first rank element, half of its first column in V.
     __device__ __forceinline__ int32_t next(const LoraDev &d) {
-        v_row = static_cast<int32_t>((base + slot) * d.group_rows);
+        v_row = static_cast<int32_t>(row0 + slot * d.slot_rows);
         const int32_t adapter = slot == 0 ? head.y : slot == 1 ? head.z : slot == 2 ? head.w : adapters[slot];
         b_row = adapter * static_cast<int32_t>(d.n);
         const int32_t x = static_cast<int32_t>(rb * d.width);
@@ -91,33 +96,68 @@ struct LoraBlocks {
     }
 };
 
-// Bytes of a part in the stage: a row of V's operand, a row of B_i's.
+// Bytes of a part's rows in the stage: of V's, of B_i's.
 __device__ __forceinline__ uint32_t lora_v_row_bytes(const LoraDev &d) { return d.width * 4; }
 __device__ __forceinline__ uint32_t lora_b_row_bytes(const LoraDev &d) { return d.width * 2; }
 
+// The MMA issuer's walk over the same slots: which rows each stage's parts leave alone.  BLOCKS: uint4 of a slot's mask.
+template <int BLOCKS>
+struct LoraLanes {
+    const uint4 *masks = nullptr;
+    uint32_t slot = 0, slot_step = 1, rb = 0;
+    uint4 off[2][BLOCKS];              // of the next stage's parts
+
+    __device__ __forceinline__ void open(const LoraDev &d, uint32_t group, uint32_t first = 0, uint32_t step = 1) {
+        masks = reinterpret_cast<const uint4 *>(d.table + static_cast<size_t>(group) * d.table_stride + d.mask_off);
+        slot = first;
+        slot_step = step;
+        rb = 0;
+    }
+    // Ahead of the wait for the stage; a slot behind the last one in use reads what nobody uses.
+    __device__ __forceinline__ void load(const LoraDev &d) {
+#pragma unroll
+        for (uint32_t i = 0; i < 2; ++i) {
+            const uint32_t s = slot + i * slot_step;
+            if (s >= d.max_slots || (i == 1 && d.width == 32)) continue;
+#pragma unroll
+            for (uint32_t j = 0; j < BLOCKS; ++j) off[i][j] = __ldcg(masks + static_cast<size_t>(s) * BLOCKS + j);
+        }
+    }
+    __device__ __forceinline__ void step(const LoraDev &d, uint32_t parts) {
+        if (d.width == 32 && ++rb < d.rank_blocks) return;
+        rb = 0;
+        slot += parts * slot_step;
+    }
+};
+
 // The MMAs of a stage of adapter parts: V's parts from smem_v, v_rows rows each, B_i's from smem_b, b_rows rows each.
-// V_FIRST: V is the MMA's A operand (its rows are the accumulator's), else its B operand.
-template <int CTA_GROUP, bool V_FIRST>
+// LANES: V's rows are the accumulator's lanes, and part i leaves the lanes of off[i][first ...] alone; else V is the MMA's
+// B operand and has zeros in the rows that do not use the adapter.
+template <int CTA_GROUP, bool LANES, int BLOCKS>
 __device__ __forceinline__ void lora_stage_mma(uint32_t tmem_d, uint32_t smem_v, uint32_t smem_b, uint32_t v_rows,
-                                               uint32_t b_rows, uint32_t idesc, uint32_t info, const LoraDev &d) {
+                                               uint32_t b_rows, uint32_t idesc, uint32_t info, const LoraDev &d,
+                                               const uint4 (&off)[2][BLOCKS], uint32_t first) {
     const uint32_t parts = info >> 4, steps = info & 7u;
     const uint32_t v_bytes = lora_v_row_bytes(d), b_bytes = lora_b_row_bytes(d);
-    for (uint32_t i = 0; i < parts; ++i) {
+#pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        if (i >= parts) break;
         const uint64_t dv = ptx::smem_desc_k(smem_v + i * v_rows * v_bytes, v_bytes);
         const uint64_t db = ptx::smem_desc_k(smem_b + i * b_rows * b_bytes, b_bytes);
         for (uint32_t k = 0; k < 2 * steps; ++k) {               // hi, then lo: 32 bytes = +2 in the >>4 address field
             const uint32_t lo = k >= steps ? 1u : 0u, at = k - lo * steps;
             const uint64_t v = dv + 2 * (lo * d.width / kUmmaK + at), b = db + 2 * at;
-            ptx::umma_f16<CTA_GROUP>(tmem_d, V_FIRST ? v : b, V_FIRST ? b : v, idesc, 1u);
+            if constexpr (LANES) ptx::umma_f16_lanes<CTA_GROUP>(tmem_d, v, b, idesc, &off[i][first]);
+            else ptx::umma_f16<CTA_GROUP>(tmem_d, b, v, idesc, 1u);
         }
     }
 }
 
-// A zero of V times an infinity or NaN in another row's adapter is NaN: such an element is computed again from its own
-// row's terms alone.  `acc` unless one of the group's other adapters holds such a value in this column.
+// Few tokens: a zero of V times an infinity or NaN in another row's adapter is NaN; such an element is computed again from
+// its own row's terms alone.  `acc` unless one of the batch's other adapters holds such a value in this column.
 template <bool BF16>
-__device__ __noinline__ float lora_exact(const LoraDev &d, uint32_t group, uint32_t row, uint32_t col, float acc) {
-    const int32_t *t = d.table + static_cast<size_t>(group) * d.table_stride;
+__device__ __noinline__ float lora_exact(const LoraDev &d, uint32_t row, uint32_t col, float acc) {
+    const int32_t *t = d.table;
     const int32_t slots = t[0], id = d.ids[row];
     int32_t mine = -1;
     bool other = false;
@@ -145,10 +185,9 @@ __device__ __noinline__ float lora_exact(const LoraDev &d, uint32_t group, uint3
         for (int e = 0; e < 8; ++e) sum = fmaf(f[e], g[e], sum);
     }
     if (mine >= 0) {
-        const uint32_t in_group = row - group * d.group_rows;
         const uint32_t w8 = d.width / 8;
         const uint4 *v = reinterpret_cast<const uint4 *>(d.v) +
-                         ((static_cast<int64_t>(group) * d.max_slots + mine) * d.group_rows + in_group) * (2 * d.rank_blocks * w8);
+                         (static_cast<int64_t>(mine) * d.slot_rows + row) * (2 * d.rank_blocks * w8);
         const uint4 *b = reinterpret_cast<const uint4 *>(d.b) + (static_cast<int64_t>(id) * d.n + col) * r8;
         for (uint32_t r = 0; r < r8; ++r) {
             const uint4 *hi = v + r / w8 * (2 * w8) + r % w8;
@@ -160,24 +199,6 @@ __device__ __noinline__ float lora_exact(const LoraDev &d, uint32_t group, uint3
         }
     }
     return sum;
-}
-
-// N accumulators of row `row`, columns col, col + 1, ...
-template <bool BF16, int N>
-__device__ __forceinline__ void lora_repair(float (&f)[N], const LoraDev &d, uint32_t group, uint32_t row, uint32_t col,
-                                            uint32_t M) {
-    bool bad = false;
-#pragma unroll
-    for (int i = 0; i < N; ++i) bad |= f[i] != f[i];
-    if (!bad || row >= M) return;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-        if (f[i] != f[i] && col + i < d.n) f[i] = lora_exact<BF16>(d, group, row, col + i, f[i]);
-}
-template <bool BF16>
-__device__ __forceinline__ void lora_repair(uint32_t (&v)[32], const LoraDev &d, uint32_t group, uint32_t row, uint32_t col,
-                                            uint32_t M) {
-    lora_repair<BF16, 32>(reinterpret_cast<float(&)[32]>(v), d, group, row, col, M);
 }
 
 }  // namespace

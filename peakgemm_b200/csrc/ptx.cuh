@@ -334,6 +334,32 @@ __device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t desc_a, uint6
             : "memory");
 }
 
+// The same, adding into the lanes (rows of D) alone whose bit in `off` is 0: bit 0 of off[0].x is the first row, off[1] the
+// second CTA's of a pair.
+template <int CTA_GROUP>
+__device__ __forceinline__ void umma_f16_lanes(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                               const uint4 *off) {
+    if constexpr (CTA_GROUP == 1)
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, 1, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n\t"
+            "}\n"
+            ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(off[0].x), "r"(off[0].y), "r"(off[0].z), "r"(off[0].w)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.b32 p, 1, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n\t"
+            "}\n"
+            ::"r"(tmem_d), "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(off[0].x), "r"(off[0].y), "r"(off[0].z), "r"(off[0].w),
+              "r"(off[1].x), "r"(off[1].y), "r"(off[1].z), "r"(off[1].w)
+            : "memory");
+}
+
 // Arrive (count 1) on `bar` once every tcgen05.mma this thread issued before has
 // completed.  `bar` is a barrier of the issuing CTA.
 template <int CTA_GROUP>

@@ -157,6 +157,46 @@ def test_one_request_does_not_touch_another(cuda, m, value):
     assert not torch.isfinite(d[7].float()).any() and not torch.isfinite(d[9].float()).any()
 
 
+@pytest.mark.parametrize("m", [100, 300, 700])
+def test_an_adapter_without_a_finite_value(cuda, m):
+    """One request's adapter is NaN altogether, at a long k: the other rows stay exact, no wait runs out, and the call takes
+    no longer than without it (some tens of microseconds)."""
+    x = make(m, 1032, 8192, 6, 16, BF16, 98)
+    x["ids"][x["ids"] == 2] = 1
+    x["ids"][3] = 2
+    call(x)
+    x["lora_b"][2] = float("nan")
+    x["lora_b"][5, ::7] = float("inf")
+    x["a"][6] = float("nan")
+    torch.cuda.synchronize()
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    start.record()
+    d = call(x, torch.empty(m, 1032, dtype=BF16, device="cuda"))
+    end.record()
+    keep = [t for t in range(m) if t not in (3, 6) and x["ids"][t] != 5]
+    check(x, d, keep)
+    assert d[3].isnan().all() and d[6].isnan().all()
+    assert start.elapsed_time(end) < 10.0
+
+
+@pytest.mark.parametrize("m,n,k,adapters,rank", [(8192, 3328, 256, 700, 8), (1100, 520, 264, 600, 40), (300, 264, 136, 1000, 16)])
+def test_hundreds_of_adapters_in_a_tile(cuda, m, n, k, adapters, rank):
+    x = make(m, n, k, adapters, rank, BF16, 99)
+    check(x, call(x))
+
+
+def test_scratch_does_not_grow_with_the_pool(cuda):
+    """Twice V's bits for every row (rank 64: 256 bytes), and a few words for each adapter that the rows of a tile can use."""
+    from peakgemm_b200 import capi
+
+    for m, n, k in ((128, 4096, 4096), (1000, 4096, 4096), (4096, 14336, 4096), (32768, 4096, 4096)):
+        for pool in (1, 512, 100000):
+            table = (m // 128 + 4) * (min(pool, 512) + 4) * (4 + 512 // 8)
+            assert 0 < capi.hgemm_lora_workspace_bytes(m, n, k, pool, 64) <= m * 64 * 4 + table + 512
+    for m in (1, 16, 64):                       # the tokens of a small batch once for each adapter they can use
+        assert capi.hgemm_lora_workspace_bytes(m, 4096, 4096, 100000, 64) <= 64 * 64 * 64 * 4 + 1024
+
+
 @pytest.mark.parametrize("m", [9, 130, 600])
 def test_pitches_and_untouched_surroundings(cuda, m):
     """Matrices that are blocks of wider ones; columns beside the output and rows behind it stay as they were."""
