@@ -185,10 +185,11 @@ int pg_hgemm_fused(void *d, const void *a, const void *b,
  * An adapter of a smaller rank is padded with zeros in lora_a or lora_b, and finite values in the other.  With
  * row_scale = rstd, fold gamma into lora_a as into b.  adapters == 0 is pg_hgemm_fused.
  * rank % 8 == 0, 8 <= rank <= 512, adapters * rank and adapters * n < 2^31; otherwise pg_hgemm_fused's
- * preconditions.  residual may be d itself.  workspace: pg_hgemm_lora_workspace_bytes bytes, 256-byte aligned device
- * memory, no initialisation, private to the call until its kernels have finished: about 4 * m * rank (rank rounded up to
- * 16, or to a multiple of 32) and, for each 128 to 512 rows, 20 to 68 bytes for each adapter that they can use; up to 64
- * rows 4 * rank * rows * min(rows, adapters), rows rounded up to 16, 32 or 64.
+ * preconditions.  residual may be d itself.  workspace: pg_hgemm_lora_workspace_bytes bytes (0 for sizes that the call
+ * refuses, and where it needs none), 256-byte aligned device memory, no initialisation, private to the call until its
+ * kernels have finished: about 4 * m * rank (rank rounded up to 16, or to a multiple of 32) and, for each 128 to 512 rows,
+ * 20 to 68 bytes for each adapter that they can use; up to 64 rows 4 * rank * rows * min(rows, adapters), rows rounded up
+ * to 16, 32 or 64.
  * A value that is not finite, in an adapter or in a row of a, reaches only the rows that use the adapter, or that row.
  * The reference project has no adapters.
  */

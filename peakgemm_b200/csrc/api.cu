@@ -194,6 +194,11 @@ int fused_args(pg::GemmArgs &g, void *d, const void *a, const void *b, int64_t m
     return PG_OK;
 }
 
+// Ranks that the adapters' kernels take, and a pool whose rows are counted in 32 bits; all three positive.
+bool lora_pool_ok(int64_t n, int64_t adapters, int64_t rank) {
+    return rank % 8 == 0 && rank <= kMaxRank && adapters <= kMaxDim / rank && adapters <= kMaxDim / n;
+}
+
 }  // namespace
 
 extern "C" {
@@ -215,7 +220,8 @@ int pg_hgemm_fused(void *d, const void *a, const void *b, int64_t m, int64_t n, 
 }
 
 size_t pg_hgemm_lora_workspace_bytes(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank) {
-    if (m <= 0 || n <= 0 || k <= 0 || adapters <= 0 || rank <= 0 || rank > kMaxRank || m > kMaxDim) return 0;
+    if (m <= 0 || n <= 0 || k <= 0 || adapters <= 0 || rank <= 0) return 0;
+    if (n % 8 != 0 || k % 8 != 0 || m > kMaxDim || n > kMaxDim || k > kMaxDim || !lora_pool_ok(n, adapters, rank)) return 0;
     size_t bytes = 0;
     if (pg::lora_workspace_bytes(m, n, k, adapters, rank, &bytes) != cudaSuccess) {
         cudaGetLastError();
@@ -237,7 +243,7 @@ int pg_hgemm_lora(void *d, const void *a, const void *b, int64_t m, int64_t n, i
     const int st = fused_args(g, d, a, b, m, n, k, lda, ldb, ldd, row_scale, bias, residual, ldr, dtype);
     if (st != PG_OK) return st;
     if (!lora_a || !lora_b || !ids || !workspace || rank <= 0) return PG_ERR_BAD_ARG;
-    if (rank % 8 != 0 || rank > kMaxRank || adapters > kMaxDim / rank || adapters > kMaxDim / n) return PG_ERR_UNSUPPORTED;
+    if (!lora_pool_ok(n, adapters, rank)) return PG_ERR_UNSUPPORTED;
     if (!aligned16(lora_a) || !aligned16(lora_b) || ((reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(scale)) & 3u) ||
         (reinterpret_cast<uintptr_t>(workspace) & 255u))
         return PG_ERR_MISALIGNED;

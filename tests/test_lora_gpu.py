@@ -197,6 +197,17 @@ def test_scratch_does_not_grow_with_the_pool(cuda):
         assert capi.hgemm_lora_workspace_bytes(m, 4096, 4096, 100000, 64) <= 64 * 64 * 64 * 4 + 1024
 
 
+def test_no_scratch_for_a_call_that_is_refused(cuda):
+    """A rank or a matrix that is no multiple of 8, an index of 2^31 or more: pg_hgemm_lora refuses, and the query says 0."""
+    from peakgemm_b200 import capi
+
+    size = capi.hgemm_lora_workspace_bytes
+    assert size(64, 64, 64, 4, 16) > 0
+    for a in ((64, 64, 64, 4, 12), (64, 60, 64, 4, 16), (64, 64, 60, 4, 16), (64, 64, 64, 2 ** 27, 16), (64, 64, 64, 2 ** 25 + 1, 64),
+              (2 ** 31, 64, 64, 4, 16), (64, 2 ** 31, 64, 4, 16), (64, 64, 2 ** 31, 4, 16)):
+        assert size(*a) == 0, a
+
+
 @pytest.mark.parametrize("m", [9, 130, 600])
 def test_pitches_and_untouched_surroundings(cuda, m):
     """Matrices that are blocks of wider ones; columns beside the output and rows behind it stay as they were."""
