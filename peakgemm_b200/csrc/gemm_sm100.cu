@@ -507,7 +507,7 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     }
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 };
-                LoraBlocks extra;                    // the adapters' blocks behind the product's own
+                LoraBlocks<false> extra;             // the adapters' blocks behind the product's own
                 if constexpr (LORA)
                     if (it > 0) extra.load(lora.d, mi);
                 // With adapters the last block is taken apart below: in the loop, the few instructions that ask for it
@@ -1084,7 +1084,7 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             uint32_t stage = 0, phase = 0;
             // the weights pass through once (evict first); the activations are what every CTA re-reads (evict last)
             const uint64_t pol_stream = l2_policy_evict_first(), pol_keep = l2_policy_evict_last();
-            LoraBlocks extra;   // this CTA's share of the adapters' k-blocks (CTAs without a k-slice get none)
+            LoraBlocks<false> extra;   // this CTA's share of the adapters' k-blocks (CTAs without a k-slice get none)
             for (uint32_t kb = kb0; kb < kb1 + extra.count; ++kb) {
                 if constexpr (LORA) {
                     if (kb + 1 == kb1) {
@@ -1558,10 +1558,11 @@ struct SnCfg {
     static constexpr uint32_t kOffW = 0;
     static constexpr uint32_t kOffT = kOffW + STAGES * kWBytes;
     static constexpr uint32_t kOffBar = kOffT + STAGES * kTBytes;
-    static constexpr uint32_t kNumBars = 2 * STAGES + 1;
+    static constexpr uint32_t kNumBars = 2 * STAGES + 2;
     static constexpr uint32_t kOffMisc = kOffBar + kNumBars * 8;
     static constexpr uint32_t kOffInfo = kOffMisc + 16;                 // LORA: what each stage holds
-    static constexpr uint32_t kOffRecv = (kOffInfo + STAGES * 4 + 15) & ~15u;   // [TOK/4][S slots x 128/S rows][4] fp32, S > 1 only
+    static constexpr uint32_t kOffSpoilt = kOffInfo + STAGES * 4;       // LORA: slots to leave out, two words
+    static constexpr uint32_t kOffRecv = (kOffSpoilt + 8 + 15) & ~15u;   // [TOK/4][S slots x 128/S rows][4] fp32, S > 1 only
     static constexpr uint32_t kRecvBytes = kBM * TOK * 4;
     static constexpr uint32_t kSmemNoRecv = kOffRecv + 1024;
     static constexpr uint32_t kSmemBytes = kSmemNoRecv + kRecvBytes;
@@ -1589,10 +1590,16 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
     const uint32_t bar_full = smem_base + C::kOffBar;
     const uint32_t bar_empty = bar_full + STAGES * 8;
     const uint32_t bar_acc_full = bar_empty + STAGES * 8;
+    const uint32_t bar_verdict = bar_acc_full + 8;     // LORA: every epilogue warp has said which slots are spoilt
     const uint32_t tmem_slot = smem_base + C::kOffMisc;
     volatile uint32_t *tmem_slot_gen = reinterpret_cast<volatile uint32_t *>(smem_gen + C::kOffMisc);
     volatile uint32_t *abort_flag = tmem_slot_gen + 1;
     volatile uint32_t *stage_info = reinterpret_cast<volatile uint32_t *>(smem_gen + C::kOffInfo);
+    uint32_t *spoilt_words = reinterpret_cast<uint32_t *>(smem_gen + C::kOffSpoilt);
+    const auto spoilt_slots = [&]() {
+        const volatile uint32_t *w = spoilt_words;
+        return static_cast<uint64_t>(w[1]) << 32 | w[0];
+    };
     const WaitCtx ctx{abort_flag, status};
 
     const uint32_t ni = blockIdx.x / S;               // which 128 weight rows
@@ -1607,6 +1614,10 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
             mbar_init(bar_empty + s * 8, 1);
         }
         mbar_init(bar_acc_full, 1);
+        if constexpr (LORA) {
+            mbar_init(bar_verdict, kEpiWarps);
+            spoilt_words[0] = spoilt_words[1] = 0;
+        }
         *abort_flag = 0;
         fence_mbar_init();
         prefetch_tensormap(&tm_tok);
@@ -1636,41 +1647,51 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
             uint32_t stage = 0, phase = 0;
             // the weights pass through once (evict first); the activations are what every CTA re-reads (evict last)
             const uint64_t pol_stream = l2_policy_evict_first(), pol_keep = l2_policy_evict_last();
-            LoraBlocks extra;   // this CTA's share of the adapters' k-blocks (CTAs without a k-slice get none)
-            for (uint32_t kb = kb0; kb < kb1 + extra.count; ++kb) {
-                if constexpr (LORA) {
-                    if (kb + 1 == kb1) {
-                        asm volatile("griddepcontrol.wait;" ::: "memory");
-                        extra.load(lora.d, 0);
-                        extra.open(lora.d, rank, (k_blocks + per - 1) / per);
-                    }
-                }
-                if (!wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty)) break;
-                if constexpr (LORA) {
-                    if (kb + 1 >= kb1) stage_info[stage] = extra.info(lora.d, kb, kb1);
-                    if (kb >= kb1) {
-                        const uint32_t parts = extra.parts(lora.d);
-                        const uint32_t v_bytes = lora_v_row_bytes(lora.d), b_bytes = lora_b_row_bytes(lora.d);
-                        mbar_arrive_expect_tx(bar_full + stage * 8, parts * (kBM * b_bytes + TOK * v_bytes));
-                        for (uint32_t i = 0; i < parts; ++i) {
-                            const int32_t rx = extra.next(lora.d);
-                            tma_load_2d(smem_base + C::kOffW + stage * C::kWBytes + i * kBM * b_bytes, &lora.tm_b,
-                                        bar_full + stage * 8, rx, extra.b_row + static_cast<int32_t>(ni * kBM));
-                            tma_load_2d(smem_base + C::kOffT + stage * C::kTBytes + i * TOK * v_bytes, &lora.tm_v,
-                                        bar_full + stage * 8, 2 * rx, extra.v_row);
+            LoraBlocks<true> extra;   // this CTA's share of the adapters' k-blocks (CTAs without a k-slice get none)
+            bool ok = has_k, again = false;
+            do {                      // with adapters once more, without the spoilt slots, where there are any
+                extra.count = 0;
+                for (uint32_t kb = kb0; kb < kb1 + extra.count; ++kb) {
+                    if constexpr (LORA) {
+                        if (kb + 1 == kb1) {
+                            if (!again) asm volatile("griddepcontrol.wait;" ::: "memory");
+                            extra.load(lora.d, 0);
+                            extra.open(lora.d, rank, (k_blocks + per - 1) / per);
                         }
-                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-                        continue;
                     }
+                    ok = wait_bar(bar_empty + stage * 8, phase ^ 1u, ctx, kStProducerEmpty);
+                    if (!ok) break;
+                    if constexpr (LORA) {
+                        if (kb + 1 >= kb1) stage_info[stage] = extra.info(lora.d, kb, kb1);
+                        if (kb >= kb1) {
+                            const uint32_t parts = extra.parts(lora.d);
+                            const uint32_t v_bytes = lora_v_row_bytes(lora.d), b_bytes = lora_b_row_bytes(lora.d);
+                            mbar_arrive_expect_tx(bar_full + stage * 8, parts * (kBM * b_bytes + TOK * v_bytes));
+                            for (uint32_t i = 0; i < parts; ++i) {
+                                const int32_t rx = extra.next(lora.d);
+                                tma_load_2d(smem_base + C::kOffW + stage * C::kWBytes + i * kBM * b_bytes, &lora.tm_b,
+                                            bar_full + stage * 8, rx, extra.b_row + static_cast<int32_t>(ni * kBM));
+                                tma_load_2d(smem_base + C::kOffT + stage * C::kTBytes + i * TOK * v_bytes, &lora.tm_v,
+                                            bar_full + stage * 8, 2 * rx, extra.v_row);
+                            }
+                            if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                            continue;
+                        }
+                    }
+                    mbar_arrive_expect_tx(bar_full + stage * 8, C::kStageBytes);
+                    const int32_t kx = static_cast<int32_t>(kb * kBK);
+                    tma_load_2d_hint(smem_base + C::kOffW + stage * C::kWBytes, &tm_w, bar_full + stage * 8, kx,
+                                     static_cast<int32_t>(ni * kBM), pol_stream);
+                    tma_load_2d_hint(smem_base + C::kOffT + stage * C::kTBytes, &tm_tok, bar_full + stage * 8, kx, 0,
+                                     pol_keep);
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
-                mbar_arrive_expect_tx(bar_full + stage * 8, C::kStageBytes);
-                const int32_t kx = static_cast<int32_t>(kb * kBK);
-                tma_load_2d_hint(smem_base + C::kOffW + stage * C::kWBytes, &tm_w, bar_full + stage * 8, kx,
-                                 static_cast<int32_t>(ni * kBM), pol_stream);
-                tma_load_2d_hint(smem_base + C::kOffT + stage * C::kTBytes, &tm_tok, bar_full + stage * 8, kx, 0,
-                                 pol_keep);
-                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-            }
+                if constexpr (LORA) {
+                    if (!ok || again || M == 1 || !wait_bar(bar_verdict, 0, ctx, kStProducerEmpty)) break;
+                    extra.skip = spoilt_slots();
+                    again = extra.skip != 0;
+                }
+            } while (again);
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -1678,37 +1699,45 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
             constexpr uint32_t idesc = instr_desc_f16(BF16, kBM, TOK);
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            bool last = !LORA;
-            for (uint32_t kb = kb0; kb < kb1; ++kb) {
-                ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
-                if (!ok) break;
-                tc_fence_after_sync();
-                if constexpr (LORA)
-                    if (kb + 1 == kb1) last = (stage_info[stage] & kLoraLast) != 0;
-                const uint64_t dw = smem_desc_k_sw128(smem_base + C::kOffW + stage * C::kWBytes);
-                const uint64_t dt = smem_desc_k_sw128(smem_base + C::kOffT + stage * C::kTBytes);
-#pragma unroll
-                for (uint32_t k = 0; k < kBK / kUmmaK; ++k)
-                    umma_f16<1>(tmem_base, dw + 2 * k, dt + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
-                umma_commit<1>(bar_empty + stage * 8);
-                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-            }
-            if constexpr (LORA) {
-                while (ok && !last) {                // the adapters' stages
+            bool again = false;
+            do {
+                bool last = !LORA;
+                for (uint32_t kb = kb0; kb < kb1; ++kb) {
                     ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
                     if (!ok) break;
                     tc_fence_after_sync();
-                    const uint32_t info = stage_info[stage];
-                    last = (info & kLoraLast) != 0;
-                    constexpr uint4 all[2][1] = {};
-                    lora_stage_mma<1, false>(tmem_base, smem_base + C::kOffT + stage * C::kTBytes,
-                                             smem_base + C::kOffW + stage * C::kWBytes, TOK, kBM, idesc, info & 0x77u, lora.d,
-                                             all, 0);
+                    if constexpr (LORA)
+                        if (kb + 1 == kb1) last = (stage_info[stage] & kLoraLast) != 0;
+                    const uint64_t dw = smem_desc_k_sw128(smem_base + C::kOffW + stage * C::kWBytes);
+                    const uint64_t dt = smem_desc_k_sw128(smem_base + C::kOffT + stage * C::kTBytes);
+#pragma unroll
+                    for (uint32_t k = 0; k < kBK / kUmmaK; ++k)
+                        umma_f16<1>(tmem_base, dw + 2 * k, dt + 2 * k, idesc, (kb > kb0 || k > 0) ? 1u : 0u);
                     umma_commit<1>(bar_empty + stage * 8);
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
-            }
-            if (ok) umma_commit<1>(bar_acc_full);
+                if constexpr (LORA) {
+                    while (ok && !last) {                // the adapters' stages
+                        ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        const uint32_t info = stage_info[stage];
+                        last = (info & kLoraLast) != 0;
+                        constexpr uint4 all[2][1] = {};
+                        lora_stage_mma<1, false>(tmem_base, smem_base + C::kOffT + stage * C::kTBytes,
+                                                 smem_base + C::kOffW + stage * C::kWBytes, TOK, kBM, idesc, info & 0x77u, lora.d,
+                                                 all, 0);
+                        umma_commit<1>(bar_empty + stage * 8);
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    }
+                }
+                if (ok) umma_commit<1>(bar_acc_full);
+                if constexpr (LORA) {
+                    if (!ok || again || M == 1 || !wait_bar(bar_verdict, 0, ctx, kStMmaAccEmpty)) break;
+                    tc_fence_after_sync();           // the epilogue has read the accumulator
+                    again = spoilt_slots() != 0;
+                }
+            } while (again);
         }
         __syncwarp();
     } else {
@@ -1722,7 +1751,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
             tc_fence_after_sync();
         }
         float f[TOK];
-        if (has_k && ok) {
+        const auto load_sums = [&]() {
 #pragma unroll
             for (uint32_t g8 = 0; g8 < TOK / 8; ++g8) {
                 uint32_t o[8];
@@ -1731,11 +1760,39 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
 #pragma unroll
                 for (int i = 0; i < 8; ++i) f[8 * g8 + i] = __uint_as_float(o[i]);
             }
+        };
+        if (has_k && ok) {
+            load_sums();
         } else {
 #pragma unroll
             for (int i = 0; i < TOK; ++i) f[i] = 0.f;
         }
         tc_fence_before_sync();
+        const uint32_t n_glob = ni * kBM + row;
+        if constexpr (LORA) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");
+            if (has_k && M > 1) {      // a single token meets no adapter but its own
+                const uint64_t spoilt = lora_spoilt<BF16, TOK>(f, lora.d, M, n_glob, rank, (k_blocks + per - 1) / per);
+                if (lane == 0) {
+                    if (spoilt) {
+                        atomicOr(spoilt_words, static_cast<uint32_t>(spoilt));
+                        atomicOr(spoilt_words + 1, static_cast<uint32_t>(spoilt >> 32));
+                    }
+                    mbar_arrive(bar_verdict);
+                }
+                __syncwarp();
+                if (spoilt) {          // this warp's sums come again without the slots that any warp named
+                    ok = wait_bar(bar_verdict, 0, ctx, kStEpiAccFull) && wait_bar(bar_acc_full, 1, ctx, kStEpiAccFull);
+                    ok = __all_sync(0xffffffffu, ok);
+                    tc_fence_after_sync();
+                    if (ok) {
+                        load_sums();
+                        lora_add_spoilt<BF16, TOK>(f, lora.d, M, n_glob, spoilt_slots());
+                    }
+                    tc_fence_before_sync();
+                }
+            }
+        }
         const uint32_t owner = row / rows_per;
         const uint32_t recv_local = smem_base + C::kOffRecv;
         if (S > 1 && owner != rank) {
@@ -1752,7 +1809,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
             cluster_wait();
         }
         if (owner == rank) {
-            if (epi.pdl_all || LORA) asm volatile("griddepcontrol.wait;" ::: "memory");
+            if (epi.pdl_all) asm volatile("griddepcontrol.wait;" ::: "memory");
             const float *recv = reinterpret_cast<const float *>(smem_gen + C::kOffRecv);
             for (uint32_t r2 = 0; r2 < S; ++r2) {
                 if (r2 == rank) continue;
@@ -1764,18 +1821,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                 }
             }
             // C[mi, n] = D[n, mi]: for each token the 32 lanes of a warp write 32 consecutive columns of C
-            const uint32_t n_glob = ni * kBM + row;
             if (n_glob < N) {
-                if constexpr (LORA) {
-                    bool bad = false;
-#pragma unroll
-                    for (uint32_t mi = 0; mi < TOK; ++mi) bad |= mi < M && f[mi] != f[mi];
-                    if (bad) {
-#pragma unroll
-                        for (uint32_t mi = 0; mi < TOK; ++mi)
-                            if (mi < M && f[mi] != f[mi]) f[mi] = lora_exact<BF16>(lora.d, mi, n_glob, f[mi]);
-                    }
-                }
                 if (epi.any()) {
                     // thread = one column of C: its bias once, then per token the row scale (one address for the
                     // whole warp) and the residual element (32 consecutive columns per warp)
@@ -1972,8 +2018,7 @@ bool fill_lora(LoraParam<false> *, const GemmArgs &, uint32_t, uint32_t) { retur
 bool fill_lora(LoraParam<true> *p, const GemmArgs &g, uint32_t v_rows, uint32_t b_rows) {
     const LoraGemm &l = *g.lora;
     p->d = {l.ids, l.table, static_cast<const uint16_t *>(l.v), static_cast<const uint16_t *>(l.b),
-            static_cast<const uint16_t *>(g.a), static_cast<const uint16_t *>(g.b), g.lda, g.ldb,
-            static_cast<uint32_t>(g.k), static_cast<uint32_t>(g.n), static_cast<uint32_t>(l.rank),
+            static_cast<uint32_t>(g.n), static_cast<uint32_t>(l.rank),
             static_cast<uint32_t>(lora_v_cols(l.rank) / (2 * lora_width(l.rank))), lora_width(l.rank),
             static_cast<uint32_t>(l.max_slots),
             static_cast<uint32_t>(l.group_rows), static_cast<uint32_t>(l.slot_rows), static_cast<uint32_t>(l.table_stride),

@@ -33,9 +33,7 @@ struct LoraDev {
                                 // group_rows / 32 words for each slot, a bit set for every row that does not use it
     const uint16_t *v;          // [m][2 * rank_blocks * width]; slot_rows > 0: [max_slots][slot_rows][...]
     const uint16_t *b;          // [adapters][n][rank]
-    const uint16_t *x, *w;      // the product's operands
-    int64_t ldx, ldw;
-    uint32_t k, n, rank, rank_blocks, width;      // width: rank elements of a part
+    uint32_t n, rank, rank_blocks, width;         // width: rank elements of a part
     uint32_t max_slots, group_rows, slot_rows, table_stride, mask_off;
 };
 
@@ -49,9 +47,12 @@ template <> struct LoraParam<true> {
 // bit 3 whether the tile ends with the stage, bits 4-6 the number of adapter parts (0: a block of the product).
 constexpr uint32_t kLoraLast = 8u;
 
-// The producer's walk over a tile's adapters: slots first, first + step, ..., in `count` stages.
+// The producer's walk over a tile's adapters: slots first, first + step, ..., in `count` stages.  SKIP: without those of
+// `skip`, of at most 64 slots.
+template <bool SKIP>
 struct LoraBlocks {
-    uint32_t count = 0, slot = 0, slot_step = 1, slots = 0, rb = 0, row0 = 0;
+    uint32_t count = 0, slot = 0, slot_step = 1, left = 0, rb = 0, row0 = 0;
+    uint64_t skip = 0;
     int4 head = {0, 0, 0, 0};          // the table's first words: the number of slots and three adapters
     const int32_t *adapters = nullptr;
     int32_t v_row = 0, b_row = 0;      // of the part that next() returned
@@ -65,16 +66,24 @@ struct LoraBlocks {
         row0 = group * d.group_rows;
     }
     __device__ __forceinline__ void open(const LoraDev &d, uint32_t first = 0, uint32_t step = 1) {
-        slots = min(static_cast<uint32_t>(head.x), d.max_slots);
+        const uint32_t slots = min(static_cast<uint32_t>(head.x), d.max_slots);
         slot = first;
         slot_step = step;
         rb = 0;
-        const uint32_t mine = slots > first ? (slots - first + step - 1) / step : 0u;
-        count = d.width < 32 ? (mine + pack(d) - 1) / pack(d) : mine * d.rank_blocks;
+        left = slots > first ? (slots - first + step - 1) / step : 0u;
+        if constexpr (SKIP)
+            if (skip) {
+                for (uint32_t s = first; s < slots; s += step) left -= skip >> s & 1u;
+                if (left) pass_over();
+            }
+        count = d.width < 32 ? (left + pack(d) - 1) / pack(d) : left * d.rank_blocks;
+    }
+    __device__ __forceinline__ void pass_over() {
+        while (skip >> slot & 1u) slot += slot_step;
     }
     // Parts of the stage that next() will fill.
     __device__ __forceinline__ uint32_t parts(const LoraDev &d) const {
-        return min(pack(d), (slots - slot + slot_step - 1) / slot_step);
+        return min(pack(d), left);
     }
     // The word of the stage that block kb goes to (block kb1 - 1 is the product's last).
     __device__ __forceinline__ uint32_t info(const LoraDev &d, uint32_t kb, uint32_t kb1) const {
@@ -91,6 +100,9 @@ struct LoraBlocks {
         if (++rb == d.rank_blocks) {
             rb = 0;
             slot += slot_step;
+            --left;
+            if constexpr (SKIP)
+                if (left) pass_over();
         }
         return x;
     }
@@ -153,52 +165,74 @@ __device__ __forceinline__ void lora_stage_mma(uint32_t tmem_d, uint32_t smem_v,
     }
 }
 
-// Few tokens: a zero of V times an infinity or NaN in another row's adapter is NaN; such an element is computed again from
-// its own row's terms alone.  `acc` unless one of the batch's other adapters holds such a value in this column.
+// Few tokens: a zero of V times an infinity or NaN in another row's adapter is NaN.  A CTA in whose sums that may have
+// happened makes them again without the slots that hold such values (its "spoilt" slots), and adds those slots' values to
+// the rows that use them here: the weights pass by twice, whatever is not finite.  64 x 14336 x 4096, 6 adapters of rank 16,
+// 40 us; with one of NaN alone, or with one NaN in it, 65 (each element computed again by a warp took 1700).
+
+// Which of the slots first, first + step, ... (at most 64 in all) are not finite in column `col`.
 template <bool BF16>
-__device__ __noinline__ float lora_exact(const LoraDev &d, uint32_t row, uint32_t col, float acc) {
-    const int32_t *t = d.table;
-    const int32_t slots = t[0], id = d.ids[row];
-    int32_t mine = -1;
-    bool other = false;
-    const uint32_t r8 = d.rank / 8;
-    float f[8], g[8];
-    for (int32_t s = 0; s < slots; ++s) {
-        const int32_t a = t[1 + s];
-        if (a == id) {
-            mine = s;
-            continue;
-        }
-        const uint4 *b = reinterpret_cast<const uint4 *>(d.b) + (static_cast<int64_t>(a) * d.n + col) * r8;
+__device__ __noinline__ uint64_t lora_spoilt_slots(const LoraDev &d, uint32_t col, uint32_t first, uint32_t step) {
+    const uint32_t r8 = d.rank / 8, slots = min(static_cast<uint32_t>(d.table[0]), d.max_slots);
+    uint64_t spoilt = 0;
+    for (uint32_t s = first; s < slots; s += step) {
+        const uint4 *b = reinterpret_cast<const uint4 *>(d.b) + (static_cast<int64_t>(d.table[1 + s]) * d.n + col) * r8;
+        bool found = false;
+#pragma unroll 4
         for (uint32_t r = 0; r < r8; ++r) {
-            vec_unpack<BF16>(b[r], f);
-            for (int e = 0; e < 8; ++e) other |= !(fabsf(f[e]) < __int_as_float(0x7f800000));     // infinity or NaN
+            float g[8];
+            vec_unpack<BF16>(__ldg(b + r), g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) found |= !(fabsf(g[e]) < __int_as_float(0x7f800000));
         }
+        spoilt |= static_cast<uint64_t>(found) << s;
     }
-    if (!other) return acc;
+    return spoilt;
+}
+
+// The same for a warp's 32 columns, where one of them has a NaN; every lane gets the slots of all.
+template <bool BF16, int TOK>
+__device__ __forceinline__ uint64_t lora_spoilt(const float (&f)[TOK], const LoraDev &d, uint32_t tokens, uint32_t col,
+                                                uint32_t first, uint32_t step) {
+    bool bad = false;
+#pragma unroll
+    for (uint32_t t = 0; t < TOK; ++t) bad |= t < tokens && f[t] != f[t];
+    bad = bad && col < d.n;
+    if (!__any_sync(0xffffffffu, bad)) return 0;
+    const uint64_t mine = bad ? lora_spoilt_slots<BF16>(d, col, first, step) : 0;
+    return static_cast<uint64_t>(__reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mine >> 32))) << 32 |
+           __reduce_or_sync(0xffffffffu, static_cast<uint32_t>(mine));
+}
+
+// What token t gets in column `col` from its adapter's slot.
+template <bool BF16>
+__device__ __noinline__ float lora_slot_value(const LoraDev &d, uint32_t t, uint32_t col, uint32_t slot) {
+    const uint32_t r8 = d.rank / 8, w8 = d.width / 8;
+    const uint4 *b = reinterpret_cast<const uint4 *>(d.b) + (static_cast<int64_t>(d.table[1 + slot]) * d.n + col) * r8;
+    const uint4 *v = reinterpret_cast<const uint4 *>(d.v) + (static_cast<int64_t>(slot) * d.slot_rows + t) * (2 * d.rank_blocks * w8);
     float sum = 0.f;
-    const uint4 *x = reinterpret_cast<const uint4 *>(d.x + static_cast<int64_t>(row) * d.ldx);
-    const uint4 *w = reinterpret_cast<const uint4 *>(d.w + static_cast<int64_t>(col) * d.ldw);
-    for (uint32_t c = 0; c < d.k / 8; ++c) {
-        vec_unpack<BF16>(x[c], f);
-        vec_unpack<BF16>(w[c], g);
-        for (int e = 0; e < 8; ++e) sum = fmaf(f[e], g[e], sum);
-    }
-    if (mine >= 0) {
-        const uint32_t w8 = d.width / 8;
-        const uint4 *v = reinterpret_cast<const uint4 *>(d.v) +
-                         (static_cast<int64_t>(mine) * d.slot_rows + row) * (2 * d.rank_blocks * w8);
-        const uint4 *b = reinterpret_cast<const uint4 *>(d.b) + (static_cast<int64_t>(id) * d.n + col) * r8;
-        for (uint32_t r = 0; r < r8; ++r) {
-            const uint4 *hi = v + r / w8 * (2 * w8) + r % w8;
-            float lo[8];
-            vec_unpack<BF16>(*hi, f);
-            vec_unpack<BF16>(hi[w8], lo);
-            vec_unpack<BF16>(b[r], g);
-            for (int e = 0; e < 8; ++e) sum = fmaf(f[e] + lo[e], g[e], sum);
-        }
+    for (uint32_t r = 0; r < r8; ++r) {
+        const uint4 *hi = v + r / w8 * (2 * w8) + r % w8;
+        float x[8], lo[8], g[8];
+        vec_unpack<BF16>(*hi, x);
+        vec_unpack<BF16>(hi[w8], lo);
+        vec_unpack<BF16>(__ldg(b + r), g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(x[e] + lo[e], g[e], sum);
     }
     return sum;
+}
+
+// Adds to the tokens' sums in column `col` what they get from those of the slots that they use.
+template <bool BF16, int TOK>
+__device__ __forceinline__ void lora_add_spoilt(float (&f)[TOK], const LoraDev &d, uint32_t tokens, uint32_t col, uint64_t which) {
+    for (; which; which &= which - 1) {
+        const uint32_t slot = __ffsll(static_cast<long long>(which)) - 1;
+        const int32_t adapter = d.table[1 + slot];
+#pragma unroll
+        for (uint32_t t = 0; t < TOK; ++t)
+            if (t < tokens && col < d.n && d.ids[t] == adapter) f[t] += lora_slot_value<BF16>(d, t, col, slot);
+    }
 }
 
 }  // namespace

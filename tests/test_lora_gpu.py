@@ -157,10 +157,10 @@ def test_one_request_does_not_touch_another(cuda, m, value):
     assert not torch.isfinite(d[7].float()).any() and not torch.isfinite(d[9].float()).any()
 
 
-@pytest.mark.parametrize("m", [100, 300, 700])
+@pytest.mark.parametrize("m", [12, 32, 64, 100, 300, 700])
 def test_an_adapter_without_a_finite_value(cuda, m):
     """One request's adapter is NaN altogether, at a long k: the other rows stay exact, no wait runs out, and the call takes
-    no longer than without it (some tens of microseconds)."""
+    no longer than without it over 64 rows (some tens of microseconds), up to 64 rows about twice as long."""
     x = make(m, 1032, 8192, 6, 16, BF16, 98)
     x["ids"][x["ids"] == 2] = 1
     x["ids"][3] = 2
@@ -176,7 +176,7 @@ def test_an_adapter_without_a_finite_value(cuda, m):
     keep = [t for t in range(m) if t not in (3, 6) and x["ids"][t] != 5]
     check(x, d, keep)
     assert d[3].isnan().all() and d[6].isnan().all()
-    assert start.elapsed_time(end) < 10.0
+    assert start.elapsed_time(end) < 1.0
 
 
 @pytest.mark.parametrize("m,n,k,adapters,rank", [(8192, 3328, 256, 700, 8), (1100, 520, 264, 600, 40), (300, 264, 136, 1000, 16)])
