@@ -245,8 +245,8 @@ def rmsnorm_inputs(rows: int, h: int, dtype: torch.dtype, seed: int):
 # PARITY UNPINNED: the reference has neither operator; these restate the definitions in float64, on the inputs' device,
 # together with per-element bounds on what an fp32 evaluation may be off by.
 #
-# Bounds.  The sums over a row are sums of h products in some tree order: each of a row's at most 64 serial additions,
-# 5 shuffle levels and 32 warp sums rounds by 2^-24, so a sum of positive terms is within 2^-17 of itself, rstd (its
+# Bounds.  The sums over a row are sums of h products in some tree order: each of a row's at most 64 serial additions in
+# 32 bits (a thread's further ones, which grow with h, are in 64), 5 shuffle levels and 32 warp sums rounds by 2^-24, so a sum of positive terms is within 2^-17 of itself, rstd (its
 # inverse square root) within 2^-18 + 2^-22, and a sum of mixed terms within 2^-17 of the sum of their absolute values.
 # REL = 2^-17 covers a product of such a factor with the few roundings of the elementwise arithmetic.
 

@@ -33,6 +33,13 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
     return t;
 }
 
+__device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8]) {
+    float t = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t = fmaf(a[e], b[e], t);
+    return t;
+}
+
 struct Row {
     const uint4 *gate;     // the row's gate, or null
     __device__ __forceinline__ Row(const RmsResidualTerms &t, uint32_t row, uint32_t rows_per_gate) {
@@ -135,7 +142,8 @@ rms_residual_fwd_kernel(const RmsResidualFwdArgs a, uint32_t rows_per_gate) {
 }
 
 // Any h: the row is read three times (the second and third reads hit L2); [2048, 65536] 384-416 us, 0.4-0.5 of the copy
-// bandwidth.  Nothing is written before the last pass, so s may be the residual and y may be u here too.
+// bandwidth.  Nothing is written before the last pass, so s may be the residual and y may be u here too.  A thread's sums
+// of eight squares are added in 64 bits: their number grows with h.
 template <bool BF16>
 __global__ void __launch_bounds__(1024)
 rms_residual_fwd_wide_kernel(const RmsResidualFwdArgs a, uint32_t rows_per_gate) {
@@ -149,7 +157,7 @@ rms_residual_fwd_wide_kernel(const RmsResidualFwdArgs a, uint32_t rows_per_gate)
         float rstd_u = 1.f, rstd_s = 1.f;
         for (int pass = a.t.gamma_post ? 0 : 1; pass < 3; ++pass) {
             if (pass == 1 && !a.y) continue;
-            float ss = 0.f;
+            double ss = 0.0;
             for (int idx = threadIdx.x; idx < h8; idx += blockDim.x) {
                 float f[8], g[8], x[8];
                 vec_unpack<BF16>(u[idx], f);
@@ -170,8 +178,7 @@ rms_residual_fwd_wide_kernel(const RmsResidualFwdArgs a, uint32_t rows_per_gate)
                     for (int e = 0; e < 8; ++e) f[e] = fmaf(g[e], x[e], f[e]);
                 }
                 if (pass < 2) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+                    ss += static_cast<double>(dot8(f, f));
                 } else {
                     static_cast<uint4 *>(a.s)[base + idx] = vec_pack<BF16>(f);
                     if (a.y) {
@@ -182,8 +189,8 @@ rms_residual_fwd_wide_kernel(const RmsResidualFwdArgs a, uint32_t rows_per_gate)
                     }
                 }
             }
-            if (pass == 0) rstd_u = 1.f / sqrtf(block_sum(ss, red[0]) * inv_h + a.t.eps);
-            if (pass == 1) rstd_s = 1.f / sqrtf(block_sum(ss, red[1]) * inv_h + a.t.eps);
+            if (pass == 0) rstd_u = 1.f / sqrtf(block_sum(static_cast<float>(ss), red[0]) * inv_h + a.t.eps);
+            if (pass == 1) rstd_s = 1.f / sqrtf(block_sum(static_cast<float>(ss), red[1]) * inv_h + a.t.eps);
         }
         __syncthreads();
     }
@@ -191,7 +198,7 @@ rms_residual_fwd_wide_kernel(const RmsResidualFwdArgs a, uint32_t rows_per_gate)
 
 // --------------------------------------------------------------- backward ----
 
-// What a row contributes to its elements' gradients: D = ds + cs.x * w - cs.y * s, du = cu.x * e * gamma_post - cu.y * u.
+// What a row contributes to its elements' gradients: D = ds + rstd_s * w - ms * s, du = rstd_u * e * gamma_post - mu * u.
 struct RowStats {
     float rstd_s, ms;     // rstd(s), rstd(s)^3 * mean(w * s)
     float rstd_u, mu;     // rstd(u), rstd(u)^3 * mean(e * gamma_post * u)
@@ -227,7 +234,7 @@ rms_residual_bwd_stats_kernel(const RmsResidualBwdArgs a, RowStats *stats, uint3
         const int64_t base = static_cast<int64_t>(row) * h8;
         const Row r(a.t, row, rows_per_gate);
         RowStats st = {1.f, 0.f, 1.f, 0.f};
-        float ss = 0.f, ws = 0.f, uu = 0.f;
+        double ss = 0.0, ws = 0.0, uu = 0.0;           // of sums of eight: their number grows with h
         for (int idx = threadIdx.x; idx < h8; idx += blockDim.x) {
             float f[8], g[8], d[8];
             if (a.dy) {
@@ -235,24 +242,22 @@ rms_residual_bwd_stats_kernel(const RmsResidualBwdArgs a, RowStats *stats, uint3
                 vec_unpack<BF16>(static_cast<const uint4 *>(a.dy)[base + idx], d);
                 vec_load_f32(a.t.gamma_pre + 8 * idx, g);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    ss = fmaf(f[e], f[e], ss);
-                    ws = fmaf(d[e] * g[e], f[e], ws);
-                }
+                for (int e = 0; e < 8; ++e) d[e] *= g[e];
+                ss += static_cast<double>(dot8(f, f));
+                ws += static_cast<double>(dot8(d, f));
             }
             if (a.t.gamma_post) {
                 vec_unpack<BF16>(static_cast<const uint4 *>(a.u)[base + idx], f);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) uu = fmaf(f[e], f[e], uu);
+                uu += static_cast<double>(dot8(f, f));
             }
         }
         if (a.dy) {
-            st.rstd_s = 1.f / sqrtf(block_sum(ss, red[0]) * inv_h + a.t.eps);
-            st.ms = block_sum(ws, red[1]) * inv_h * st.rstd_s * (st.rstd_s * st.rstd_s);
+            st.rstd_s = 1.f / sqrtf(block_sum(static_cast<float>(ss), red[0]) * inv_h + a.t.eps);
+            st.ms = block_sum(static_cast<float>(ws), red[1]) * inv_h * st.rstd_s * (st.rstd_s * st.rstd_s);
         }
         if (a.t.gamma_post) {
-            st.rstd_u = 1.f / sqrtf(block_sum(uu, red[2]) * inv_h + a.t.eps);
-            float eu = 0.f;
+            st.rstd_u = 1.f / sqrtf(block_sum(static_cast<float>(uu), red[2]) * inv_h + a.t.eps);
+            double eu = 0.0;
             for (int idx = threadIdx.x; idx < h8; idx += blockDim.x) {
                 float D[8], f[8], g[8], x[8];
                 load_stream_grad<BF16>(a, base + idx, idx, st, D, x, g);
@@ -264,9 +269,10 @@ rms_residual_bwd_stats_kernel(const RmsResidualBwdArgs a, RowStats *stats, uint3
                     for (int e = 0; e < 8; ++e) g[e] *= x[e];
                 }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) eu = fmaf(D[e] * g[e], f[e], eu);
+                for (int e = 0; e < 8; ++e) D[e] *= g[e];
+                eu += static_cast<double>(dot8(D, f));
             }
-            st.mu = block_sum(eu, red[3]) * inv_h * st.rstd_u * (st.rstd_u * st.rstd_u);
+            st.mu = block_sum(static_cast<float>(eu), red[3]) * inv_h * st.rstd_u * (st.rstd_u * st.rstd_u);
         }
         if (threadIdx.x == 0) stats[row] = st;
         __syncthreads();

@@ -126,6 +126,19 @@ def test_wide_rows_share_gates(cuda, rows, h, gates, res, pre):
     check_backward(x, s, backward(x, s))
 
 
+@pytest.mark.parametrize("h", [65544, 1 << 20, 1 << 22])
+def test_sums_over_any_width_keep_their_bits(cuda, h):
+    """A row of one value, 1.9765625, whose square every fp32 addition rounds the same way from 1024 on: thousands of them
+    one after the other are 2^-14 off, eight times what the bounds allow a sum over a row."""
+    x = make(2, h, BF16, 70, gates=0, res_scale=0)
+    x["u"].fill_(1.9765625)
+    s, y = forward(x)
+    check_forward(x, s, y)
+    check_backward(x, s, backward(x, s))
+    s.fill_(1.9765625)
+    check_backward(x, s, backward(x, s))
+
+
 def test_benchmark_size(cuda):
     x = make(8192, 4096, BF16, 64, gates=8, res_scale=1)
     s, y = forward(x)
