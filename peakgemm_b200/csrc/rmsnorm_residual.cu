@@ -60,84 +60,80 @@ __device__ __forceinline__ void load_scale(const RmsResidualTerms &t, int idx, f
 // ---------------------------------------------------------------- forward ----
 
 // One block per row, thread t owns the vectors t, t + blockDim.x, ... (at most VPT) and holds the row in registers.
-// For few rows of h <= 16384.  Bound by latency (loads, two block sums): [1, 4096] 3.3 us, [64, 8192] 4.5 us with a
-// launch of about 2.5 us.
+// For few rows of h <= 16384 (with one for every worker of the staged kernel that one runs).  Bound by latency (loads, two
+// block sums): replayed in a graph, [1, 4096] 3.3 us, [64, 8192] 4.5 us with a launch of about 2.5 us.
 template <int VPT, bool BF16>
 __global__ void __launch_bounds__(1024)
 rms_residual_fwd_kernel(const RmsResidualFwdArgs a, uint32_t rows_per_gate) {
     __shared__ float red[2][32];
     const int h8 = static_cast<int>(a.t.h / 8);
     const float inv_h = 1.f / static_cast<float>(a.t.h);
-    for (uint32_t row = blockIdx.x; row < a.t.rows; row += gridDim.x) {
-        const int64_t base = static_cast<int64_t>(row) * h8;
-        const Row r(a.t, row, rows_per_gate);
-        uint4 uv[VPT], rv[VPT];
+    const uint32_t row = blockIdx.x;
+    const int64_t base = static_cast<int64_t>(row) * h8;
+    const Row r(a.t, row, rows_per_gate);
+    uint4 uv[VPT], rv[VPT];
+#pragma unroll
+    for (int j = 0; j < VPT; ++j) {
+        const int idx = threadIdx.x + blockDim.x * j;
+        const bool in = idx < h8;
+        uv[j] = in ? static_cast<const uint4 *>(a.u)[base + idx] : make_uint4(0, 0, 0, 0);
+        rv[j] = in ? static_cast<const uint4 *>(a.residual)[base + idx] : make_uint4(0, 0, 0, 0);
+    }
+    float rstd_u = 1.f;
+    if (a.t.gamma_post) {
+        float ss = 0.f;
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
-            const int idx = threadIdx.x + blockDim.x * j;
-            const bool in = idx < h8;
-            uv[j] = in ? static_cast<const uint4 *>(a.u)[base + idx] : make_uint4(0, 0, 0, 0);
-            rv[j] = in ? static_cast<const uint4 *>(a.residual)[base + idx] : make_uint4(0, 0, 0, 0);
+            float f[8];
+            vec_unpack<BF16>(uv[j], f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
         }
-        float rstd_u = 1.f;
-        if (a.t.gamma_post) {
-            float ss = 0.f;
+        rstd_u = 1.f / sqrtf(block_sum(ss, red[0]) * inv_h + a.t.eps);
+    }
+    float s[VPT][8], ss = 0.f;
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                float f[8];
-                vec_unpack<BF16>(uv[j], f);
+    for (int j = 0; j < VPT; ++j) {
+        const int idx = threadIdx.x + blockDim.x * j;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+        for (int e = 0; e < 8; ++e) s[j][e] = 0.f;
+        if (idx < h8) {
+            float f[8], g[8];
+            vec_unpack<BF16>(uv[j], f);
+            if (a.t.gamma_post) {
+                vec_load_f32(a.t.gamma_post + 8 * idx, g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = (f[e] * rstd_u) * g[e];
             }
-            rstd_u = 1.f / sqrtf(block_sum(ss, red[0]) * inv_h + a.t.eps);
+            if (r.gate) {
+                vec_unpack<BF16>(__ldg(r.gate + idx), g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] *= g[e];
+            }
+            float x[8];
+            vec_unpack<BF16>(rv[j], x);
+            load_scale(a.t, idx, g);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                s[j][e] = fmaf(g[e], x[e], f[e]);
+                ss = fmaf(s[j][e], s[j][e], ss);
+            }
+            static_cast<uint4 *>(a.s)[base + idx] = vec_pack<BF16>(s[j]);
         }
-        float s[VPT][8], ss = 0.f;
+    }
+    if (a.y) {
+        const float rstd_s = 1.f / sqrtf(block_sum(ss, red[1]) * inv_h + a.t.eps);
 #pragma unroll
         for (int j = 0; j < VPT; ++j) {
             const int idx = threadIdx.x + blockDim.x * j;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[j][e] = 0.f;
             if (idx < h8) {
-                float f[8], g[8];
-                vec_unpack<BF16>(uv[j], f);
-                if (a.t.gamma_post) {
-                    vec_load_f32(a.t.gamma_post + 8 * idx, g);
+                float g[8];
+                vec_load_f32(a.t.gamma_pre + 8 * idx, g);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = (f[e] * rstd_u) * g[e];
-                }
-                if (r.gate) {
-                    vec_unpack<BF16>(__ldg(r.gate + idx), g);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] *= g[e];
-                }
-                float x[8];
-                vec_unpack<BF16>(rv[j], x);
-                load_scale(a.t, idx, g);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    s[j][e] = fmaf(g[e], x[e], f[e]);
-                    ss = fmaf(s[j][e], s[j][e], ss);
-                }
-                static_cast<uint4 *>(a.s)[base + idx] = vec_pack<BF16>(s[j]);
+                for (int e = 0; e < 8; ++e) g[e] *= s[j][e] * rstd_s;
+                static_cast<uint4 *>(a.y)[base + idx] = vec_pack<BF16>(g);
             }
         }
-        if (a.y) {
-            const float rstd_s = 1.f / sqrtf(block_sum(ss, red[1]) * inv_h + a.t.eps);
-#pragma unroll
-            for (int j = 0; j < VPT; ++j) {
-                const int idx = threadIdx.x + blockDim.x * j;
-                if (idx < h8) {
-                    float g[8];
-                    vec_load_f32(a.t.gamma_pre + 8 * idx, g);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) g[e] *= s[j][e] * rstd_s;
-                    static_cast<uint4 *>(a.y)[base + idx] = vec_pack<BF16>(g);
-                }
-            }
-        }
-        // red[0] and red[1] are free again for the next row: whoever writes red[0] there has passed the barrier of
-        // red[1]; without y (or without gamma_post) there is no such barrier in between
-        if (blockDim.x > 32 && (!a.y || !a.t.gamma_post)) __syncthreads();
     }
 }
 
@@ -497,11 +493,9 @@ cudaError_t rmsnorm_residual_fwd_launch(const RmsResidualFwdArgs &a, cudaStream_
     if (e != cudaSuccess) return e;
     if (rmsnorm_residual_staged_fwd_supported(a.t, sms)) return rmsnorm_residual_staged_fwd(a, stream);
     const int64_t h8 = a.t.h / 8;
-    int64_t grid = static_cast<int64_t>(sms) * 16;
-    if (grid > a.t.rows) grid = a.t.rows;
     const uint32_t rpg = rows_per_gate(a.t);
-    const unsigned g = static_cast<unsigned>(grid);
     if (h8 <= 2048) {
+        const unsigned g = static_cast<unsigned>(a.t.rows);
         const int vpt = h8 <= 64 ? 1 : 2;
         int threads = static_cast<int>((h8 + vpt - 1) / vpt + 31) / 32 * 32;
         if (vpt == 1) {
@@ -512,6 +506,8 @@ cudaError_t rmsnorm_residual_fwd_launch(const RmsResidualFwdArgs &a, cudaStream_
             else rms_residual_fwd_kernel<2, false><<<g, threads, 0, stream>>>(a, rpg);
         }
     } else {
+        const int64_t most = static_cast<int64_t>(sms) * 16;
+        const unsigned g = static_cast<unsigned>(a.t.rows < most ? a.t.rows : most);
         if (a.t.bf16) rms_residual_fwd_wide_kernel<true><<<g, 1024, 0, stream>>>(a, rpg);
         else rms_residual_fwd_wide_kernel<false><<<g, 1024, 0, stream>>>(a, rpg);
     }
