@@ -66,6 +66,24 @@ __device__ __forceinline__ void split_terms(const float (&f)[8], uint4 &hi, uint
     lo = vec_pack<BF16>(l);
 }
 
+// The distinct ids that are not negative among `rows` rows, in the order of their first row, by one warp: 32 rows at a
+// time, first against each other, then against the list so far.  Returns their number.
+template <class IdAt>
+__device__ __forceinline__ uint32_t list_slots(uint32_t rows, uint32_t lane, int32_t *slots, const IdAt &id_at) {
+    uint32_t n = 0;
+    for (uint32_t r = 0; r < rows; r += 32) {
+        const int32_t id = r + lane < rows ? id_at(r + lane) : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, id);       // every lane takes part
+        bool fresh = id >= 0 && __ffs(same) - 1 == static_cast<int>(lane);
+        for (uint32_t e = 0; e < n; ++e) fresh = fresh && slots[e] != id;
+        const uint32_t who = __ballot_sync(0xffffffffu, fresh);
+        if (fresh) slots[n + __popc(who & ((1u << lane) - 1u))] = id;
+        n += __popc(who);
+        __syncwarp();
+    }
+    return n;
+}
+
 struct Shrink {
     const int32_t *ids;
     const float *scale;
@@ -148,19 +166,7 @@ lora_shrink_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_consta
     tc_fence_after_sync();
     const uint32_t tmem = misc[0];
     if (warp == 2) {
-        // The distinct ids in the order of their first row: 32 rows at a time, first against each other, then against
-        // the list so far.
-        uint32_t n = 0;
-        for (uint32_t r = 0; r < p.group_rows; r += 32) {
-            const int32_t id = r + lane < p.group_rows ? ids[r + lane] : -1;
-            const uint32_t same = __match_any_sync(0xffffffffu, id);       // every lane takes part
-            bool fresh = id >= 0 && __ffs(same) - 1 == static_cast<int>(lane);
-            for (uint32_t e = 0; e < n; ++e) fresh = fresh && slots[e] != id;
-            const uint32_t who = __ballot_sync(0xffffffffu, fresh);
-            if (fresh) slots[n + __popc(who & ((1u << lane) - 1u))] = id;
-            n += __popc(who);
-            __syncwarp();
-        }
+        const uint32_t n = list_slots(p.group_rows, lane, slots, [&](uint32_t r) { return ids[r]; });
         if (lane == 0) misc[2] = n;
     }
     __syncthreads();
@@ -334,18 +340,8 @@ lora_dot_kernel(const uint4 *x, int64_t ldx8, const uint4 *a, const Shrink p) {
     const auto checked = [&](int32_t id) { return id >= 0 && static_cast<uint32_t>(id) < p.adapters ? id : -1; };
     const int32_t id = checked(p.ids[t]);
     const uint32_t group = t / p.group_rows, group0 = group * p.group_rows, group_end = min(p.m, group0 + p.group_rows);
-    if (warp == 0) {                     // the distinct ids in the order of their first row
-        uint32_t n = 0;
-        for (uint32_t r = group0; r < group_end; r += 32) {
-            const int32_t mine = r + lane < group_end ? checked(p.ids[r + lane]) : -1;
-            const uint32_t same = __match_any_sync(0xffffffffu, mine);       // every lane takes part
-            bool fresh = mine >= 0 && __ffs(same) - 1 == static_cast<int>(lane);
-            for (uint32_t e = 0; e < n; ++e) fresh = fresh && slots[e] != mine;
-            const uint32_t who = __ballot_sync(0xffffffffu, fresh);
-            if (fresh) slots[n + __popc(who & ((1u << lane) - 1u))] = mine;
-            n += __popc(who);
-            __syncwarp();
-        }
+    if (warp == 0) {
+        const uint32_t n = list_slots(group_end - group0, lane, slots, [&](uint32_t r) { return checked(p.ids[group0 + r]); });
         if (lane == 0) s_count = n;
     }
     float sum[kDotRanks] = {};
