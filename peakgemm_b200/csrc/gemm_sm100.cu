@@ -369,6 +369,9 @@ __device__ __forceinline__ bool wait_count_patiently(const uint32_t *counter, ui
     return true;
 }
 
+// Stages that a tile's V stays for (lora_epilogue.cuh).
+template <int STAGES> constexpr int kLoraHold = STAGES / 2 + 1;
+
 template <int CTA_GROUP, int BN, int STAGES, int MT, bool BF16, bool LORA>
 __global__ void __launch_bounds__(MT == 2 ? kThreadsWide : kThreads, 1)
 hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
@@ -507,7 +510,7 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     }
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 };
-                LoraBlocks<false> extra;             // the adapters' blocks behind the product's own
+                LoraTile<kLoraHold<STAGES>> extra;   // the adapters' blocks behind the product's own
                 if constexpr (LORA)
                     if (it > 0) extra.load(lora.d, mi);
                 // With adapters the last block is taken apart below: in the loop, the few instructions that ask for it
@@ -548,24 +551,28 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                     if (!ok) break;
                     load_block(u.kb1 - 1);
                     for (uint32_t kb = u.kb1; kb < u.kb1 + extra.count; ++kb) {
-                        const uint32_t parts = extra.parts(lora.d);
-                        const uint32_t v_bytes = lora_v_row_bytes(lora.d), b_bytes = lora_b_row_bytes(lora.d);
-                        take_stage((MT * kBM * v_bytes + C::kBRows * b_bytes) * parts, extra.info(lora.d, kb, u.kb1));
+                        const uint32_t parts = extra.parts(lora.d), b_bytes = lora_b_row_bytes(lora.d);
+                        const uint32_t v_total = extra.brings_v() ? MT * kBM * lora_v_row_bytes(lora.d) : 0u;
+                        take_stage(v_total + C::kBRows * b_bytes * parts, extra.info(lora.d, kb, u.kb1));
                         if (!ok) break;
                         const uint32_t fb = (CTA_GROUP == 2) ? full0 + stage * 8 : bar_full + stage * 8;
-                        for (uint32_t i = 0; i < parts; ++i) {
-                            const int32_t rx = extra.next(lora.d);
+                        const int32_t rx = static_cast<int32_t>(extra.rb * lora.d.width);
+                        if (v_total) {
 #pragma unroll
                             for (uint32_t mt = 0; mt < MT; ++mt) {
-                                const uint32_t da = smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox + i * kBM * v_bytes;
-                                const int32_t rv = extra.v_row + static_cast<int32_t>(mt * kBlockM + rank * kBM);
+                                const uint32_t da = smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox;
+                                const int32_t rv = row_a + static_cast<int32_t>(mt * kBlockM);
                                 if constexpr (CTA_GROUP == 2) tma_load_2d_pair(da, &lora.tm_v, fb, 2 * rx, rv);
                                 else tma_load_2d(da, &lora.tm_v, fb, 2 * rx, rv);
                             }
-                            const uint32_t db = smem_base + C::kOffB + stage * C::kBBytes + i * C::kBRows * b_bytes;
-                            if constexpr (CTA_GROUP == 2) tma_load_2d_pair(db, &lora.tm_b, fb, rx, extra.b_row + row_b);
-                            else tma_load_2d(db, &lora.tm_b, fb, rx, extra.b_row + row_b);
                         }
+                        for (uint32_t i = 0; i < parts; ++i) {
+                            const uint32_t db = smem_base + C::kOffB + stage * C::kBBytes + i * C::kBRows * b_bytes;
+                            const int32_t rb = extra.next(lora.d) + row_b;
+                            if constexpr (CTA_GROUP == 2) tma_load_2d_pair(db, &lora.tm_b, fb, rx, rb);
+                            else tma_load_2d(db, &lora.tm_b, fb, rx, rb);
+                        }
+                        extra.end_stage();
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                     }
                 }
@@ -627,6 +634,7 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                         tile_coords(group_m, u.tile, m_tiles, n_tiles, mi, ni, (flags & kFlagSerpentine) != 0);
                         lanes.open(lora.d, mi);
                     }
+                    uint32_t v_stage = 0;
                     while (ok && !last) {            // the adapters' stages
                         lanes.load(lora.d);
                         ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
@@ -634,14 +642,16 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                         tc_fence_after_sync();
                         const uint32_t info = stage_info[stage];
                         last = (info & kLoraLast) != 0;
+                        if (info & kLoraV) v_stage = stage;
 #pragma unroll
                         for (uint32_t mt = 0; mt < MT; ++mt)
-                            lora_stage_mma<CTA_GROUP, true>(tmem_base + (MT == 2 ? mt : acc) * BN,
-                                                            smem_base + C::kOffA + stage * C::kABytes + mt * C::kABox,
-                                                            smem_base + C::kOffB + stage * C::kBBytes, kBM, C::kBRows, idesc,
-                                                            info & 0x77u, lora.d, lanes.off, mt * CTA_GROUP);
-                        lanes.step(lora.d, info >> 4);
-                        umma_commit<CTA_GROUP>(bar_empty + stage * 8);
+                            lora_stage_mma<CTA_GROUP>(tmem_base + (MT == 2 ? mt : acc) * BN,
+                                                      smem_base + C::kOffA + v_stage * C::kABytes + mt * C::kABox,
+                                                      smem_base + C::kOffB + stage * C::kBBytes, C::kBRows, idesc, info,
+                                                      lora.d, lanes.off, mt * CTA_GROUP);
+                        lanes.step(info);
+                        if (stage != v_stage) umma_commit<CTA_GROUP>(bar_empty + stage * 8);
+                        if (info & kLoraRelease) umma_commit<CTA_GROUP>(bar_empty + v_stage * 8);
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                     }
                 }
@@ -1084,7 +1094,7 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
             uint32_t stage = 0, phase = 0;
             // the weights pass through once (evict first); the activations are what every CTA re-reads (evict last)
             const uint64_t pol_stream = l2_policy_evict_first(), pol_keep = l2_policy_evict_last();
-            LoraBlocks<false> extra;   // this CTA's share of the adapters' k-blocks (CTAs without a k-slice get none)
+            LoraTile<kLoraHold<STAGES>> extra;   // this CTA's share of the adapters' k-blocks (CTAs without a k-slice get none)
             for (uint32_t kb = kb0; kb < kb1 + extra.count; ++kb) {
                 if constexpr (LORA) {
                     if (kb + 1 == kb1) {
@@ -1097,16 +1107,17 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                 if constexpr (LORA) {
                     if (kb + 1 >= kb1) stage_info[stage] = extra.info(lora.d, kb, kb1);
                     if (kb >= kb1) {
-                        const uint32_t parts = extra.parts(lora.d);
-                        const uint32_t v_bytes = lora_v_row_bytes(lora.d), b_bytes = lora_b_row_bytes(lora.d);
-                        mbar_arrive_expect_tx(bar_full + stage * 8, parts * (kBM * v_bytes + BN * b_bytes));
-                        for (uint32_t i = 0; i < parts; ++i) {
-                            const int32_t rx = extra.next(lora.d);
-                            tma_load_2d(smem_base + C::kOffA + stage * C::kABytes + i * kBM * v_bytes, &lora.tm_v,
-                                        bar_full + stage * 8, 2 * rx, extra.v_row);
+                        const uint32_t parts = extra.parts(lora.d), b_bytes = lora_b_row_bytes(lora.d);
+                        const uint32_t v_total = extra.brings_v() ? kBM * lora_v_row_bytes(lora.d) : 0u;
+                        const int32_t rx = static_cast<int32_t>(extra.rb * lora.d.width);
+                        mbar_arrive_expect_tx(bar_full + stage * 8, v_total + parts * BN * b_bytes);
+                        if (v_total)
+                            tma_load_2d(smem_base + C::kOffA + stage * C::kABytes, &lora.tm_v, bar_full + stage * 8, 2 * rx,
+                                        static_cast<int32_t>(mi * kBM));
+                        for (uint32_t i = 0; i < parts; ++i)
                             tma_load_2d(smem_base + C::kOffB + stage * C::kBBytes + i * BN * b_bytes, &lora.tm_b,
-                                        bar_full + stage * 8, rx, extra.b_row + static_cast<int32_t>(ni * BN));
-                        }
+                                        bar_full + stage * 8, rx, extra.next(lora.d) + static_cast<int32_t>(ni * BN));
+                        extra.end_stage();
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                         continue;
                     }
@@ -1147,6 +1158,7 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     asm volatile("griddepcontrol.wait;" ::: "memory");
                     lanes.open(lora.d, mi, rank, (k_blocks + per - 1) / per);
                 }
+                uint32_t v_stage = 0;
                 while (ok && !last) {                // the adapters' stages
                     lanes.load(lora.d);
                     ok = wait_bar(bar_full + stage * 8, phase, ctx, kStMmaFull);
@@ -1154,11 +1166,12 @@ hgemm_splitk_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_const
                     tc_fence_after_sync();
                     const uint32_t info = stage_info[stage];
                     last = (info & kLoraLast) != 0;
-                    lora_stage_mma<1, true>(tmem_base, smem_base + C::kOffA + stage * C::kABytes,
-                                            smem_base + C::kOffB + stage * C::kBBytes, kBM, BN, idesc, info & 0x77u, lora.d,
-                                            lanes.off, 0);
-                    lanes.step(lora.d, info >> 4);
-                    umma_commit<1>(bar_empty + stage * 8);
+                    if (info & kLoraV) v_stage = stage;
+                    lora_stage_mma<1>(tmem_base, smem_base + C::kOffA + v_stage * C::kABytes,
+                                      smem_base + C::kOffB + stage * C::kBBytes, BN, idesc, info, lora.d, lanes.off, 0);
+                    lanes.step(info);
+                    if (stage != v_stage) umma_commit<1>(bar_empty + stage * 8);
+                    if (info & kLoraRelease) umma_commit<1>(bar_empty + v_stage * 8);
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
@@ -1647,7 +1660,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
             uint32_t stage = 0, phase = 0;
             // the weights pass through once (evict first); the activations are what every CTA re-reads (evict last)
             const uint64_t pol_stream = l2_policy_evict_first(), pol_keep = l2_policy_evict_last();
-            LoraBlocks<true> extra;   // this CTA's share of the adapters' k-blocks (CTAs without a k-slice get none)
+            LoraBlocks extra;         // this CTA's share of the adapters' k-blocks (CTAs without a k-slice get none)
             bool ok = has_k, again = false;
             do {                      // with adapters once more, without the spoilt slots, where there are any
                 extra.count = 0;
@@ -1670,7 +1683,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                             for (uint32_t i = 0; i < parts; ++i) {
                                 const int32_t rx = extra.next(lora.d);
                                 tma_load_2d(smem_base + C::kOffW + stage * C::kWBytes + i * kBM * b_bytes, &lora.tm_b,
-                                            bar_full + stage * 8, rx, extra.b_row + static_cast<int32_t>(ni * kBM));
+                                            bar_full + stage * 8, rx, extra.up_row + static_cast<int32_t>(ni * kBM));
                                 tma_load_2d(smem_base + C::kOffT + stage * C::kTBytes + i * TOK * v_bytes, &lora.tm_v,
                                             bar_full + stage * 8, 2 * rx, extra.v_row);
                             }
@@ -1723,10 +1736,8 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                         tc_fence_after_sync();
                         const uint32_t info = stage_info[stage];
                         last = (info & kLoraLast) != 0;
-                        constexpr uint4 all[2][1] = {};
-                        lora_stage_mma<1, false>(tmem_base, smem_base + C::kOffT + stage * C::kTBytes,
-                                                 smem_base + C::kOffW + stage * C::kWBytes, TOK, kBM, idesc, info & 0x77u, lora.d,
-                                                 all, 0);
+                        lora_slot_mma(tmem_base, smem_base + C::kOffT + stage * C::kTBytes,
+                                      smem_base + C::kOffW + stage * C::kWBytes, TOK, idesc, info, lora.d);
                         umma_commit<1>(bar_empty + stage * 8);
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                     }
