@@ -629,7 +629,7 @@ hgemm_tcgen05_kernel(const __grid_constant__ CUtensorMap tm_a,
                 if constexpr (LORA) {
                     LoraLanes<MT * CTA_GROUP> lanes;
                     if (ok && !last) {
-                        if (it == 0) asm volatile("griddepcontrol.wait;" ::: "memory");
+                        asm volatile("griddepcontrol.wait;" ::: "memory");      // for the masks
                         uint32_t mi, ni;
                         tile_coords(group_m, u.tile, m_tiles, n_tiles, mi, ni, (flags & kFlagSerpentine) != 0);
                         lanes.open(lora.d, mi);

@@ -179,6 +179,18 @@ def test_an_adapter_without_a_finite_value(cuda, m):
     assert start.elapsed_time(end) < 1.0
 
 
+@pytest.mark.parametrize("m,n,k", [(8192, 3328, 256), (3000, 4096, 512), (2500, 8200, 136)])
+@pytest.mark.parametrize("without", ["first", "last", "between"])
+def test_tiles_without_adapters_beside_tiles_with(cuda, m, n, k, without):
+    """Kernels that take several tiles one after the other: the first, the last or every other tile row has no adapter."""
+    x = make(m, n, k, 5, 24, BF16, 100, "mixed")
+    row = torch.arange(m, device="cuda")
+    none = {"first": row < 5 * m // 8, "last": row >= 3 * m // 8, "between": row // 512 % 2 == 0}[without]
+    x["ids"][none] = -1
+    for _ in range(3):
+        check(x, call(x))
+
+
 @pytest.mark.parametrize("m,n,k,adapters,rank", [(8192, 3328, 256, 700, 8), (1100, 520, 264, 600, 40), (300, 264, 136, 1000, 16)])
 def test_hundreds_of_adapters_in_a_tile(cuda, m, n, k, adapters, rank):
     x = make(m, n, k, adapters, rank, BF16, 99)
