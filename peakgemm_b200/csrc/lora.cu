@@ -19,8 +19,8 @@
 // stays its own).
 //
 // Bound by latency and by what one SM pulls from HBM, about 55 GB/s whatever the ring's depth: some 9 us of launch, first
-// loads, exchange and V, and 0.4 us per 24 KiB k-block.  128 x 4096 x 14336, 20 adapters of rank 64: 24.4 us alone (40 MB
-// from DRAM), the whole call 50 us where the product alone takes 27; 1003 x 4104 x 5128, 5 of rank 24: 54 of 41.
+// loads, exchange and V, and 0.4 us per 24 KiB k-block.  128 x 4096 x 14336, 20 adapters of rank 64: 25 us alone (40 MB
+// from DRAM), both launches 52 us in a CUDA graph where the product alone takes 27; 1003 x 4104 x 5128, 5 of rank 24: 55 of 41.
 
 #include <cuda.h>
 #include <cuda_runtime.h>
@@ -428,11 +428,12 @@ Plan make_plan(int64_t m, int64_t n, int64_t k, int64_t adapters, int64_t rank, 
 }
 
 // Dot products read an adapter's rows once for every token, a tcgen05 launch once for every tile that uses it, but against
-// all rows of the tile.  m x n x k, pool, rank, us of the whole call with dot products / tcgen05:
-//   64 tokens and fewer: 1 x 4096 x 4096, 8, 16 10.8 / 15.9; 64 x 4096 x 4096, 32, 64 26.9 / 38.9; 32 x 4096 x 14336, 4, 64
-//   29.8 / 40.0; 16 x 4096 x 16384 (64 MiB of such reads), 16, 128 42.1 / 62.1; 64 x 4096 x 8192 (128 MiB), 1, 128 30.6 / 30.8
-//   more, a large pool, mixed: 128 x 4096 x 4096, 32, 16 25.2 / 31.5; 256 x 4096 x 4096, 64, 16 (32 MiB) 39.8 / 48.0
-//   more, a small pool: 128 x 4096 x 4096, 1, 16 19.0 / 16.5, 8, 64 28.7 / 26.5; 256 x 4096 x 4096, 8, 16 25.3 / 21.4
+// all rows of the tile.  m x n x k, pool, rank, us of both launches in a CUDA graph with dot products / tcgen05:
+//   64 tokens and fewer: 1 x 4096 x 4096, 8, 16 10.8 / 15.9; 64 x 4096 x 4096, 32, 64 32.3 / 44.1; 32 x 4096 x 14336, 4, 64
+//   30.9 / 41.0; 16 x 4096 x 16384 (64 MiB of such reads), 16, 128 43.6 / 65.7; 64 x 4096 x 8192 (128 MiB), 1, 128 32.2 / 31.8
+//   more, a large pool, mixed: 128 x 4096 x 4096, 32, 16 25.3 / 31.4; 256 x 4096 x 4096, 64, 16 (32 MiB) 39.6 / 49.7;
+//   128 x 4096 x 4096 (64 MiB), 64, 64 71.5 / 71.8, 32, 64 52.0 / 46.4
+//   more, a small pool: 128 x 4096 x 4096, 1, 16 19.1 / 16.6, 8, 64 31.9 / 28.2, but 256 x 4096 x 4096, 8, 16 26.7 / 29.1
 bool dot_pays(int64_t m, int64_t k, int64_t rank, int64_t adapters) {
     const int64_t most = m <= 64 ? 128 : adapters > 16 ? 32 : 0;
     return m * k * rank * 2 <= most << 20;
@@ -440,7 +441,7 @@ bool dot_pays(int64_t m, int64_t k, int64_t rank, int64_t adapters) {
 
 // CTAs of a cluster over k: as many as keep the tiles within one wave and leave every CTA four k-blocks.  Fewer, beside
 // which the persistent GEMM kernels could begin, cost more: each occupies half an SM pair, and the tiles of the pairs
-// that come free late end late (1003 x 4104 x 5128, us with 1 / 2 / 4 / 8: 83 / 73 / 58 / 57).
+// that come free late end late (1003 x 4104 x 5128, us with 1 / 2 / 4 / 8: 75 / 57 / 59 / 56).
 int64_t choose_split(int64_t tiles, int64_t k_blocks, int sms) {
     int64_t split = 1;
     while (split < 8 && tiles * split * 2 <= sms && k_blocks >= 8 * split) split *= 2;

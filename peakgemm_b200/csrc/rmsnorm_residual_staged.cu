@@ -13,7 +13,7 @@
 //   * Rows of more than 4096 columns are shared by a cluster of 2, 4 or 8 CTAs, at most 4096 columns each: the gains and
 //     a few rows fit into shared memory, and two or more rows are in work per SM, which hides the sums' latency.  The
 //     warps of all CTAs send their sums to every CTA with st.async (data and arrival in one, no fence).
-// [32768, 4096] bf16, 8 gates, one res_scale: 330 us, 0.87 of the copy bandwidth; [4099, 5120] fp16, a gate per token, 75 us;
+// In a CUDA graph: [32768, 4096] bf16, 8 gates, one res_scale: 330 us, 0.87 of the copy bandwidth; [4099, 5120] fp16, a gate per token, 75 us;
 // [16384, 8192], 8 gates, res_scale per column, 437 us (0.66); [8192, 16384] 481-550 us (0.52-0.65).  What bounds it now is
 // issue and latency at 16 warps an SM (half of the issue slots busy, DRAM at 55 %): 128 registers a thread hold the column sums.
 // The workers' parts of the column sums go to tables that rmsnorm_residual.cu adds up in a fixed order.

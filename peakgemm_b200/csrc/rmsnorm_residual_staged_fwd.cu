@@ -10,7 +10,7 @@
 //     them send their two sums to every CTA with st.async, in two buffers in turn: who sends the sums of a row has those
 //     of the row before from everyone, and everyone sent them after reading the ones before.
 //   * The gains are kept in shared memory, the lower and upper halves of the vectors apart (no bank conflicts).
-// [32768, 4096] bf16, 8 gates: 181 us, 0.91 of the copy bandwidth; [65536, 2048] 0.95, [26112, 5120] 0.91-0.97,
+// In a CUDA graph: [32768, 4096] bf16, 8 gates: 181 us, 0.91 of the copy bandwidth; [65536, 2048] 0.95, [26112, 5120] 0.91-0.97,
 // [16384, 8192] 0.83-0.98, with res_scale per column 0.75; [8192, 16384] 222-244 us, 0.73-0.84 (280-316 with one block per
 // row), [4096, 32768] 259-284 us, 0.60-0.72 (398-436 with three passes).  A run of a few rows is bound by the latency of its first
 // loads and of the gains': [1003, 5120] fp16 13.8 us where its bytes take 6.3.
