@@ -1603,7 +1603,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
     const uint32_t bar_full = smem_base + C::kOffBar;
     const uint32_t bar_empty = bar_full + STAGES * 8;
     const uint32_t bar_acc_full = bar_empty + STAGES * 8;
-    const uint32_t bar_verdict = bar_acc_full + 8;     // LORA: every epilogue warp has said which slots are spoilt
+    const uint32_t bar_spoilt = bar_acc_full + 8;     // LORA: every epilogue warp has said which slots are spoilt
     const uint32_t tmem_slot = smem_base + C::kOffMisc;
     volatile uint32_t *tmem_slot_gen = reinterpret_cast<volatile uint32_t *>(smem_gen + C::kOffMisc);
     volatile uint32_t *abort_flag = tmem_slot_gen + 1;
@@ -1628,7 +1628,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
         }
         mbar_init(bar_acc_full, 1);
         if constexpr (LORA) {
-            mbar_init(bar_verdict, kEpiWarps);
+            mbar_init(bar_spoilt, kEpiWarps);
             spoilt_words[0] = spoilt_words[1] = 0;
         }
         *abort_flag = 0;
@@ -1700,7 +1700,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
                 if constexpr (LORA) {
-                    if (!ok || again || M == 1 || !wait_bar(bar_verdict, 0, ctx, kStProducerEmpty)) break;
+                    if (!ok || again || M == 1 || !wait_bar(bar_spoilt, 0, ctx, kStProducerEmpty)) break;
                     extra.skip = spoilt_slots();
                     again = extra.skip != 0;
                 }
@@ -1744,7 +1744,7 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                 }
                 if (ok) umma_commit<1>(bar_acc_full);
                 if constexpr (LORA) {
-                    if (!ok || again || M == 1 || !wait_bar(bar_verdict, 0, ctx, kStMmaAccEmpty)) break;
+                    if (!ok || again || M == 1 || !wait_bar(bar_spoilt, 0, ctx, kStMmaAccEmpty)) break;
                     tc_fence_after_sync();           // the epilogue has read the accumulator
                     again = spoilt_slots() != 0;
                 }
@@ -1789,11 +1789,11 @@ hgemm_skinny_kernel(const __grid_constant__ CUtensorMap tm_tok, const __grid_con
                         atomicOr(spoilt_words, static_cast<uint32_t>(spoilt));
                         atomicOr(spoilt_words + 1, static_cast<uint32_t>(spoilt >> 32));
                     }
-                    mbar_arrive(bar_verdict);
+                    mbar_arrive(bar_spoilt);
                 }
                 __syncwarp();
                 if (spoilt) {          // this warp's sums come again without the slots that any warp named
-                    ok = wait_bar(bar_verdict, 0, ctx, kStEpiAccFull) && wait_bar(bar_acc_full, 1, ctx, kStEpiAccFull);
+                    ok = wait_bar(bar_spoilt, 0, ctx, kStEpiAccFull) && wait_bar(bar_acc_full, 1, ctx, kStEpiAccFull);
                     ok = __all_sync(0xffffffffu, ok);
                     tc_fence_after_sync();
                     if (ok) {

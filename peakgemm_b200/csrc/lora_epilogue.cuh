@@ -17,9 +17,9 @@
 // 71 us with V in every stage, 49 so (48 with V as one term); 128 x 4096 x 4096, 64 of rank 64, 82 and 72 (64).  In large
 // batches it is the tensor pipe: each adapter of a tile multiplies all of its rows, hi and lo.  1024 x 4096 x 4096, 64 of
 // rank 32 in mixed order, 195 (182), of which the product alone takes 27.  Few adapters to a tile hide behind the product:
-// 4096 x 14336 x 4096, 8 of rank 64 in runs, 348 us.
+// 4096 x 14336 x 4096, 8 of rank 64 in runs, 348 us.  (All in a CUDA graph.)
 // Few tokens: a part is a slot's V beside its B_i, two in a stage up to rank 16.  64 x 14336 x 4096, 32 adapters of rank 16:
-// 42.4 us (with one term, four in a stage, 37.4), of which the product alone takes 24.5.  (All in a CUDA graph.)
+// 42.4 us a call (with one term, four in a stage, 37.4), of which the product alone takes 24.5.
 #pragma once
 
 #include <cuda.h>

@@ -23,7 +23,7 @@ def _reference_unavailable():
 
 
 def pytest_collection_modifyitems(config, items):
-    """GPU tests fail (not skip) on a GPU box if CUDA is missing; on a CPU box they are deselected by -m.  Only the
+    """GPU tests fail (not skip) where they are asked for and CUDA is missing; elsewhere -m deselects them.  Only the
     comparisons with the reference project's kernels are skipped, where these cannot be had."""
     why = _reference_unavailable()
     if why:
